@@ -568,6 +568,99 @@ TRNSPARSE_API int trnsparse_gather(int64_t count, int elem_bytes, const void* sr
 TRNSPARSE_API int trnsparse_bsr_blocks_transpose(int64_t count, int b, int elem_bytes, const void* src,
                                    const long long* idx, void* dst, void* stream);
 
+/* ---- decoder operators ------------------------------------------------------
+ * What a decoder runs beside the block-sparse attention: the norm and rotation
+ * that make its Q and K, attention to another sequence, and decoding over a
+ * prefix that a batch shares. The reference has no counterpart. */
+
+/* RMS norm of every query (index 0) and key (index 1) head with the position
+ * rotation in the same pass:
+ *   u = x / sqrt(mean(x^2) + eps),  n = u * weight,
+ *   y_a = n_a cos - n_b sin,  y_b = n_b cos + n_a sin   (angle = position * inv_freq[j])
+ * for the pairs j of the first rotary_dim elements ((j, j + rotary_dim / 2), or
+ * (2j, 2j + 1) when interleaved); the other elements pass. Tensors are
+ * (batch, heads, seq, head_dim) with unit stride along head_dim and the given
+ * strides (batch, head, token, in elements); dtype F32 or BF16, arithmetic in
+ * fp32, angles in 64 bits. weight: [head_dim] of weight_dtype, or NULL (ones).
+ * positions: integers of position_type, position_batch_stride 0 (one row for
+ * the batch) or seq. inv_freq: rotary_dim / 2 doubles on the device. heads[i]
+ * may be 0 (then that tensor is left out). */
+typedef struct trnsparse_qk_norm_rope_args {
+  int64_t batch, seq, head_dim, rotary_dim;
+  int64_t heads[2];
+  const void* x[2];
+  void* out[2];       /* y; backward: dx */
+  const void* dy[2];  /* backward only */
+  const void* weight[2];
+  void* dw[2];        /* backward: [head_dim] of weight_dtype, or NULL */
+  int64_t x_strides[2][3], out_strides[2][3], dy_strides[2][3];
+  const void* positions;
+  int64_t position_batch_stride;
+  const double* inv_freq;
+  double eps;
+  int dtype, weight_dtype, position_type, interleaved;
+} trnsparse_qk_norm_rope_args;
+
+TRNSPARSE_API int trnsparse_qk_norm_rope(const trnsparse_qk_norm_rope_args* args, void* stream);
+/* dx (args->out) and the weights' gradients from dy; sums over rows in a fixed
+ * order. Workspace: trnsparse_qk_norm_rope_workspace_size(args) bytes. */
+TRNSPARSE_API size_t trnsparse_qk_norm_rope_workspace_size(const trnsparse_qk_norm_rope_args* args);
+TRNSPARSE_API int trnsparse_qk_norm_rope_backward(const trnsparse_qk_norm_rope_args* args, void* ws, size_t ws_bytes,
+                                                  void* stream);
+
+/* Operands of the dense attention entry points. q, out, dout, dq are (batch,
+ * q_heads, q_len, head_dim); k, v, dk, dv (batch, kv_heads, k_len, head_dim);
+ * unit stride along head_dim, the other strides (batch, head, token) in
+ * elements. q_heads is a multiple of kv_heads: query head i reads key head
+ * i / (q_heads / kv_heads). F32 or BF16; softmax and sums in fp32.
+ *   key_lengths: [batch] kept keys of each sequence (clamped to [0, k_len]), or
+ *                NULL (all).
+ *   key_mask:    [batch] rows of k_len bytes, 0 = hidden, row stride
+ *                key_mask_stride, or NULL. Both given: a key must pass both.
+ * What hidden keys hold is never read into a result. A row without keys is
+ * zero. lse: [batch, q_heads, q_len] base-2 log-sum-exp of scale * q.k (-inf
+ * for a row without keys), written by the forward if not NULL, read by the
+ * backward. */
+typedef struct trnsparse_attention_args {
+  int64_t batch, q_heads, kv_heads, q_len, k_len, head_dim;
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3];
+  const int* key_lengths;
+  const unsigned char* key_mask;
+  int64_t key_mask_stride;
+  /* shared prefix: (kv_heads, prefix_len, head_dim), strides (head, token) */
+  const void *prefix_k, *prefix_v;
+  int64_t prefix_k_strides[2], prefix_v_strides[2];
+  int64_t prefix_len;
+  /* backward */
+  const void* dout;
+  void *dq, *dk, *dv;
+  int64_t dout_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
+  double scale;
+  int dtype;
+} trnsparse_attention_args;
+
+/* out = softmax(scale * q k^T over the kept keys) v. */
+TRNSPARSE_API size_t trnsparse_cross_attention_workspace_size(const trnsparse_attention_args* args);
+TRNSPARSE_API int trnsparse_cross_attention(const trnsparse_attention_args* args, void* ws, size_t ws_bytes,
+                                            void* stream);
+/* dq, dk, dv from dout, the forward's out and its lse; dq may be NULL, and dk and
+ * dv both, where they are not wanted. Every row of dk and dv is
+ * written (zero for hidden keys); results repeat bit for bit. batch, q_heads and
+ * q_len must be positive. */
+TRNSPARSE_API size_t trnsparse_cross_attention_backward_workspace_size(const trnsparse_attention_args* args);
+TRNSPARSE_API int trnsparse_cross_attention_backward(const trnsparse_attention_args* args, void* ws, size_t ws_bytes,
+                                                     void* stream);
+/* Decoding over a prefix shared by the batch: row (b, h, t) attends the whole
+ * prefix and the first key_lengths[b] - q_len + 1 + t keys of its own cache
+ * (k, v), i.e. key_lengths counts the q_len new tokens. The prefix is read once
+ * for all sequences. */
+TRNSPARSE_API size_t trnsparse_shared_prefix_attention_workspace_size(const trnsparse_attention_args* args);
+TRNSPARSE_API int trnsparse_shared_prefix_attention(const trnsparse_attention_args* args, void* ws, size_t ws_bytes,
+                                                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@ include/trnsparse_b200.h. There is no CPU compute path.
 
 __version__ = "0.6.0"
 
+from .attention import cross_attention, qk_norm_rope, shared_prefix_attention
 from .backend import HAS_NKI, get_backend, set_backend
 from .formats import BSRMatrix, COOMatrix, CSRMatrix, eye_sparse, from_dense, from_scipy
 from .iterative import (
@@ -47,6 +48,9 @@ __all__ = [
     "bsr_spmm",
     "screened_spmm",
     "block_sparse_attention_tiled",
+    "qk_norm_rope",
+    "cross_attention",
+    "shared_prefix_attention",
     "sparse_add",
     "sparse_scale",
     "sparse_transpose",

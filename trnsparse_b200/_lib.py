@@ -109,7 +109,52 @@ SIGNATURES.update({
     "trnsparse_gather": [_i64, _i32, _p, _p, _p, _p],
     "trnsparse_bsr_blocks_transpose": [_i64, _i32, _i32, _p, _p, _p, _p],
 })
+
+
+class QkNormRopeArgs(C.Structure):
+    """``trnsparse_qk_norm_rope_args`` of include/trnsparse_b200.h, field for field."""
+
+    _fields_ = [
+        ("batch", _i64), ("seq", _i64), ("head_dim", _i64), ("rotary_dim", _i64), ("heads", _i64 * 2),
+        ("x", _p * 2), ("out", _p * 2), ("dy", _p * 2), ("weight", _p * 2), ("dw", _p * 2),
+        ("x_strides", (_i64 * 3) * 2), ("out_strides", (_i64 * 3) * 2), ("dy_strides", (_i64 * 3) * 2),
+        ("positions", _p), ("position_batch_stride", _i64), ("inv_freq", _p), ("eps", _f64),
+        ("dtype", _i32), ("weight_dtype", _i32), ("position_type", _i32), ("interleaved", _i32),
+    ]
+
+
+class AttentionArgs(C.Structure):
+    """``trnsparse_attention_args`` of include/trnsparse_b200.h, field for field."""
+
+    _fields_ = [
+        ("batch", _i64), ("q_heads", _i64), ("kv_heads", _i64), ("q_len", _i64), ("k_len", _i64), ("head_dim", _i64),
+        ("q", _p), ("k", _p), ("v", _p), ("out", _p), ("lse", _p),
+        ("q_strides", _i64 * 3), ("k_strides", _i64 * 3), ("v_strides", _i64 * 3), ("out_strides", _i64 * 3),
+        ("key_lengths", _p), ("key_mask", _p), ("key_mask_stride", _i64),
+        ("prefix_k", _p), ("prefix_v", _p), ("prefix_k_strides", _i64 * 2), ("prefix_v_strides", _i64 * 2),
+        ("prefix_len", _i64),
+        ("dout", _p), ("dq", _p), ("dk", _p), ("dv", _p),
+        ("dout_strides", _i64 * 3), ("dq_strides", _i64 * 3), ("dk_strides", _i64 * 3), ("dv_strides", _i64 * 3),
+        ("scale", _f64), ("dtype", _i32),
+    ]
+
+
+SIGNATURES.update({
+    "trnsparse_qk_norm_rope": [C.POINTER(QkNormRopeArgs), _p],
+    "trnsparse_qk_norm_rope_workspace_size": [C.POINTER(QkNormRopeArgs)],
+    "trnsparse_qk_norm_rope_backward": [C.POINTER(QkNormRopeArgs), _p, _sz, _p],
+    "trnsparse_cross_attention_workspace_size": [C.POINTER(AttentionArgs)],
+    "trnsparse_cross_attention": [C.POINTER(AttentionArgs), _p, _sz, _p],
+    "trnsparse_cross_attention_backward_workspace_size": [C.POINTER(AttentionArgs)],
+    "trnsparse_cross_attention_backward": [C.POINTER(AttentionArgs), _p, _sz, _p],
+    "trnsparse_shared_prefix_attention_workspace_size": [C.POINTER(AttentionArgs)],
+    "trnsparse_shared_prefix_attention": [C.POINTER(AttentionArgs), _p, _sz, _p],
+})
 _RESTYPE = {
+    "trnsparse_qk_norm_rope_workspace_size": C.c_size_t,
+    "trnsparse_cross_attention_workspace_size": C.c_size_t,
+    "trnsparse_cross_attention_backward_workspace_size": C.c_size_t,
+    "trnsparse_shared_prefix_attention_workspace_size": C.c_size_t,
     "trnsparse_last_error": C.c_char_p,
     "trnsparse_bsr_cg_workspace_size": C.c_size_t,
     "trnsparse_bsr_power_workspace_size": C.c_size_t,
