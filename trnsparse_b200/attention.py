@@ -45,6 +45,22 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
+def _tiles(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as the attention kernels load it fastest: unit last stride, and where head_dim allows it rows that
+    start on 16 bytes (an operand that does not have them is copied once, which costs less than narrow loads)."""
+    if t.stride(-1) != 1:
+        return t.contiguous()
+    n = 16 // t.element_size()
+    if t.shape[-1] % n:
+        return t
+    for size, stride in zip(t.shape[:-1], t.stride()):
+        if size > 1 and (stride % n or stride < 0):
+            return t.contiguous()
+    if t.shape[-2] > 1 and t.stride(-2) == 0:
+        return t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def _to(t: torch.Tensor | None, dev: torch.device, dtype: torch.dtype | None = None) -> torch.Tensor | None:
     if t is None or (t.device == dev and (dtype is None or t.dtype == dtype)):
         return t
@@ -256,7 +272,7 @@ class _CrossAttentionFn(torch.autograd.Function):
         dk, dv = (_like(k), _like(v)) if want_kv else (None, None)
         if q.numel() == 0:
             return dq, None if dk is None else dk.zero_(), None if dv is None else dv.zero_(), None, None, None
-        dout = _rows(dout)
+        dout = _tiles(dout)
         a = _attention_args(q, k, v, out, lse, lengths, mask, ctx.scale)
         a.dout, a.dout_strides[:] = dout.data_ptr(), dout.stride()[:3]
         for t, ptr, strides in ((dq, "dq", a.dq_strides), (dk, "dk", a.dk_strides), (dv, "dv", a.dv_strides)):
@@ -318,7 +334,7 @@ def cross_attention(
         assert tuple(key_mask.shape) == (B, Sk), f"{name}: key_mask must be ({B}, {Sk}), got {tuple(key_mask.shape)}"
     scale = float(q.shape[3] ** -0.5 if scale is None else scale)
     dev = _dev_of(q, k, v)
-    qd, kd, vd = (_rows(_to(t, dev)) for t in (q, k, v))
+    qd, kd, vd = (_tiles(_to(t, dev)) for t in (q, k, v))
     lengths = None if key_lengths is None else _to(key_lengths, dev, torch.int32).contiguous()
     mask = None if key_mask is None else _rows(_to(key_mask, dev))
     if _grad_wanted(qd, kd, vd):
@@ -363,7 +379,7 @@ def shared_prefix_attention(
         raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or detach its operands")
     scale = float(D ** -0.5 if scale is None else scale)
     dev = _dev_of(q, prefix_k, k_cache)
-    qd, pk, pv, kc, vc = (_rows(_to(t, dev)) for t in (q, prefix_k, prefix_v, k_cache, v_cache))
+    qd, pk, pv, kc, vc = (_tiles(_to(t, dev)) for t in (q, prefix_k, prefix_v, k_cache, v_cache))
     lens = _to(lengths, dev, torch.int32).contiguous()
     out = _like(qd)
     if out.numel():

@@ -471,7 +471,7 @@ bool nothing(const trnsparse_attention_args* a) { return a->batch * a->q_heads *
 
 size_t attention_workspace(const trnsparse_attention_args* a, bool prefix) {
   if (check_attention(a, "attention") || nothing(a)) return 0;
-  return simt_workspace(a, prefix);
+  return xattn_tc_ok(a, prefix) ? xattn_tc_workspace(a, prefix) : simt_workspace(a, prefix);
 }
 
 int attention_run(const trnsparse_attention_args* a, bool prefix, void* ws, size_t ws_bytes, void* stream,
@@ -485,7 +485,8 @@ int attention_run(const trnsparse_attention_args* a, bool prefix, void* ws, size
   const size_t need = attention_workspace(a, prefix);
   TSB_REQUIRE(ws_bytes >= need && (need == 0 || ws), "%s: workspace too small (%zu bytes, needs %zu)", what, ws_bytes,
               need);
-  return simt_forward(a, prefix, ws, as_stream(stream));
+  return xattn_tc_ok(a, prefix) ? xattn_tc_forward(a, prefix, ws, as_stream(stream))
+                                : simt_forward(a, prefix, ws, as_stream(stream));
 }
 
 }  // namespace

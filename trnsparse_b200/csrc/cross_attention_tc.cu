@@ -1,0 +1,840 @@
+// Dense attention forward on the tensor cores (bf16 in and out, fp32 softmax
+// and sums; head_dim a multiple of 8 up to 128): cross attention and
+// shared-prefix attention, from one token per sequence to long prompts.
+//
+//   O = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m),  s = scale log2(e) q.k
+// in one pass over the key tiles with the running maximum m and sum l of every
+// row. P = 2^(s - m) is rounded to bf16 for its product with V (half a step,
+// 2^-9 relative on average, of the same size as the result's own rounding); l
+// sums the unrounded values in fp32. m moves only when a tile's maximum passes
+// it by more than 2^8, so the accumulator in TMEM is rarely rescaled and P <=
+// 2^8.
+//
+// An item is 256 packed rows (see xattn.cuh: query heads of one key head,
+// tokens, and for a shared prefix all sequences) against the keys of one (batch
+// entry, key head). One CTA per SM, 10 warps:
+//   warps 0-3 / 4-7  softmax of rows 0-127 / 128-255, a thread per row: reads
+//                    its 128 scores from TMEM, writes P over them as packed
+//                    bf16 (the A operand of the second product), keeps m and l;
+//                    loads the Q tile (any strides) and writes O.
+//   warp 8           TMA producer: K0, V0, K1, V1, ... through one ring of
+//                    tiles; a tile is read by both halves' products, so 64 KB
+//                    of K / V feed 2 x 2 products of 128 x 128 x 128.
+//   warp 9           MMA issuer: for each key tile P_A V, next S_A, P_B V,
+//                    next S_B; the tensor cores work on one half while the
+//                    other half's exponentials run.
+// The score and P columns of a half are the same TMEM columns: MMAs of a CTA
+// run in issue order, so the next S follows the P V that reads them.
+//
+// Work split: with many items each CTA takes whole items round robin (CTAs that
+// run at the same time share K / V in L2); the last one to two rounds - or all
+// of it when items are few, as in decoding - are cut into equal runs of key
+// tiles whatever the items' lengths, so every SM streams keys. A CTA has at
+// most one item it continues and one it leaves unfinished: their (O / l,
+// log-sum-exp) go to two slots of the workspace, joined by a second launch in
+// tile order (no atomics, results repeat bit for bit). The split depends on the
+// lengths, which stay on the device: no host synchronisation.
+//
+// Hidden keys (past a length, or masked): scores become -inf by selection, and
+// their V rows are zeroed in shared memory before the product, so NaN or
+// infinity in padding never meets a zero P. Only tiles that hold hidden keys
+// pay for it.
+#include "xattn_tc.cuh"
+
+namespace tsb {
+namespace {
+
+constexpr int kFwThreads = 320;
+constexpr int kFwRows = 256;  // rows of an item, two halves of 128
+constexpr int kFwKeys = 128;
+constexpr float kFwLazy = 8.f;
+
+template <int HD>
+struct FwLayout {
+  static constexpr int kChunks = HD / 64;
+  static constexpr int kTile = 128 * HD * 2;
+  static constexpr int kStages = HD == 128 ? 5 : 10;
+  static constexpr int kQ = 0;
+  static constexpr int kRing = 2 * kTile;
+  static constexpr int kBar = kRing + kStages * kTile;
+  static constexpr int kSmem = kBar + 512;
+  static constexpr uint32_t kTmemO = 256;  // S / P: [0, 128) and [128, 256); O: [256, +HD) and [384, +HD)
+};
+
+struct FwBars {
+  uint64_t full[10], empty[10], q_full[2], s_full[2], p_full[2], o_done[2];
+  // the run of key tiles this CTA takes after its whole items
+  long long count;
+  int side, item, k0;
+  uint32_t tmem_slot;
+  int abort_flag;
+};
+
+struct FwSide {
+  XSide s;
+  int row_tiles, items;
+  int mul_kh, mul_kb, mul_vh, mul_vb;
+};
+
+struct FwArgs {
+  FwSide side[2];
+  int sides, D, whole;         // whole: items per CTA taken whole (one side only)
+  int slot_rows;               // rows of a slot: min(256, most rows of an item)
+  int64_t rows_all;
+  float* slots;                // [2 G][slot_rows][D], then [2 G][slot_rows] log-sum-exp
+  float* slot_lse;
+  float* direct[2];            // two sides: (O, log-sum-exp) of items one CTA finished, by flat row
+  float* direct_lse[2];
+  int2* pieces;                // first and last CTA of every item of the split part
+  __nv_bfloat16* out;
+  float* lse;
+  float scale_log2;            // |scale| log2(e)
+  uint32_t q_flip;             // sign bits of a negative scale, applied to Q
+};
+
+__device__ __forceinline__ int fw_tiles(const FwSide& sd, int bi) {
+  return max(1, (side_len(sd.s, bi) + kFwKeys - 1) / kFwKeys);  // no key: one hidden tile
+}
+
+struct FwSeg {
+  int side, item, bi, h, rt, k0, k1, n;
+};
+
+// Walks this CTA's items: whole ones first, then its run of the split part.
+struct FwCursor {
+  const FwArgs& A;
+  long long left;  // tiles of the run still to take
+  int w, side, item, k;
+  __device__ FwCursor(const FwArgs& a, const FwBars& b)
+      : A(a), left(b.count), w(0), side(b.side), item(b.item), k(b.k0) {}
+  __device__ void decode(FwSeg& g) const {
+    const FwSide& sd = A.side[g.side];
+    const int per = sd.s.hkv * sd.row_tiles;
+    g.bi = g.item / per;
+    const int r = g.item - g.bi * per;
+    g.h = r / sd.row_tiles;
+    g.rt = r - g.h * sd.row_tiles;
+    g.n = fw_tiles(sd, g.bi);
+  }
+  __device__ bool next(FwSeg& g) {
+    if (w < A.whole) {
+      g.side = 0;
+      g.item = w * gridDim.x + blockIdx.x;
+      ++w;
+      decode(g);
+      g.k0 = 0;
+      g.k1 = g.n;
+      return true;
+    }
+    if (left <= 0) return false;
+    if (item >= A.side[side].items) {
+      ++side;
+      item = 0;
+    }
+    g.side = side;
+    g.item = item;
+    decode(g);
+    g.k0 = k;
+    g.k1 = static_cast<int>(min(static_cast<long long>(g.n), k + left));
+    left -= g.k1 - g.k0;
+    k = 0;
+    ++item;
+    return true;
+  }
+};
+
+// Sum of the side's tiles over batch entries [0, nb) times items per entry, and position lookups, by one warp.
+// Lane l holds 8 consecutive entries of every 256.
+struct FwScan {
+  long long total;  // tiles of the side
+  // Tiles before item `i`.
+  static __device__ long long before(const FwSide& sd, int i, int lane) {
+    const int per = sd.s.hkv * sd.row_tiles, b0 = i / per;
+    long long t = 0;
+    if (sd.s.lengths == nullptr) {
+      t = static_cast<long long>(b0) * fw_tiles(sd, 0);
+    } else {
+      for (int base = 0; base < b0; base += 256)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int b = base + lane * 8 + e;
+          if (b < b0) t += fw_tiles(sd, b);
+        }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    t *= per;
+    const int r = i - b0 * per;
+    return r == 0 ? t : t + static_cast<long long>(r) * fw_tiles(sd, b0);
+  }
+  // Item and tile within it at tile position x of the side (x below its total).
+  static __device__ void locate(const FwSide& sd, long long x, int lane, int& item, int& k) {
+    const int per = sd.s.hkv * sd.row_tiles;
+    if (sd.s.lengths == nullptr) {
+      const int n = fw_tiles(sd, 0);
+      item = static_cast<int>(x / n);
+      k = static_cast<int>(x - static_cast<long long>(item) * n);
+      return;
+    }
+    long long done = 0;
+    for (int base = 0; base < sd.s.nb; base += 256) {
+      int n[8];
+      long long s = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int b = base + lane * 8 + e;
+        n[e] = b < sd.s.nb ? fw_tiles(sd, b) : 0;
+        s += n[e];
+      }
+      long long inc = s;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      const long long all = __shfl_sync(0xffffffffu, inc, 31);
+      if ((done + all) * per > x) {
+        const unsigned hit = __ballot_sync(0xffffffffu, (done + inc) * per > x);
+        const int src = __ffs(hit) - 1;
+        long long at = done + inc - s;
+        int fi = 0, fk = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const long long end = at + n[e];
+          if (at * per <= x && x < end * per) {
+            const long long rel = x - at * per;
+            fi = (base + lane * 8 + e) * per + static_cast<int>(rel / n[e]);
+            fk = static_cast<int>(rel % n[e]);
+          }
+          at = end;
+        }
+        item = __shfl_sync(0xffffffffu, fi, src);
+        k = __shfl_sync(0xffffffffu, fk, src);
+        return;
+      }
+      done += all;
+    }
+    item = sd.items;  // past the end: never reached for x below the total
+    k = 0;
+  }
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kFwThreads, 1)
+xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_constant__ CUtensorMap tv0,
+                    const __grid_constant__ CUtensorMap tk1, const __grid_constant__ CUtensorMap tv1,
+                    const __grid_constant__ FwArgs A) {
+  using Lay = FwLayout<HD>;
+  // No static shared memory: the dynamic window then starts 1024-byte aligned, as the swizzled tiles need.
+  extern __shared__ __align__(16) uint8_t sb[];
+  FwBars& B = *reinterpret_cast<FwBars*>(sb + Lay::kBar);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < Lay::kStages; ++i) {
+      mbar_init(&B.full[i], 1);
+      mbar_init(&B.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&B.q_full[i], 128);
+      mbar_init(&B.s_full[i], 1);
+      mbar_init(&B.p_full[i], 128);
+      mbar_init(&B.o_done[i], 1);
+    }
+    B.abort_flag = (smem_u32(sb) & 1023u) ? 1 : 0;
+    if (B.abort_flag) record_device_error(DEVERR_SELFCHECK_SMEM);
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&B.tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (warp == 0) {
+    // this CTA's run: tiles [W c / G, W (c + 1) / G) of the W tiles behind the whole items, G the CTAs that
+    // get any (a piece list has no gaps)
+    const int first = A.whole * static_cast<int>(gridDim.x);
+    const long long t0 = FwScan::before(A.side[0], A.side[0].items, lane);
+    const long long t1 = A.sides > 1 ? FwScan::before(A.side[1], A.side[1].items, lane) : 0;
+    const long long s0 = first ? FwScan::before(A.side[0], first, lane) : 0;
+    const long long W = t0 + t1 - s0;
+    const long long G = W < gridDim.x ? W : gridDim.x, c = blockIdx.x;
+    const long long lo = c < G ? W * c / G : W, hi = c < G ? W * (c + 1) / G : W;
+    int side = 0, item = 0, k = 0;
+    if (hi > lo) {
+      long long x = s0 + lo;
+      if (x >= t0) {
+        side = 1;
+        x -= t0;
+      }
+      FwScan::locate(A.side[side], x, lane, item, k);
+      // items that begin in this run: which CTAs hold their pieces
+      if (A.pieces != nullptr) {
+        long long at = lo;
+        int sd = side, it = item, kk = k;
+        while (at < hi) {
+          if (it >= A.side[sd].items) {
+            ++sd;
+            it = 0;
+          }
+          const FwSide& S = A.side[sd];
+          const int n = fw_tiles(S, it / (S.s.hkv * S.row_tiles));
+          if (kk == 0 && lane == 0) {
+            const long long e = at + n - 1;  // its last tile
+            const int index = sd == 0 ? it - first : A.side[0].items + it;
+            A.pieces[index] = make_int2(blockIdx.x, static_cast<int>(((e + 1) * G - 1) / W));
+          }
+          at += n - kk;
+          kk = 0;
+          ++it;
+        }
+      }
+    }
+    if (lane == 0) {
+      B.count = hi - lo;
+      B.side = side;
+      B.item = item;
+      B.k0 = k;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = B.tmem_slot;
+  volatile int* abort_flag = &B.abort_flag;
+
+  if (warp == 8) {
+    // ---------------- TMA producer
+    if (lane == 0 && !*abort_flag) {
+      FwCursor cur(A, B);
+      FwSeg g;
+      int slot = 0, use = 0;
+      bool ok = true;
+      while (ok && cur.next(g)) {
+        const FwSide& sd = A.side[g.side];
+        const CUtensorMap* tk = g.side ? &tk1 : &tk0;
+        const CUtensorMap* tv = g.side ? &tv1 : &tv0;
+        for (int j = g.k0; ok && j < g.k1; ++j) {
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            if (*abort_flag || (use > 0 && !mbar_wait(&B.empty[slot], (use - 1) & 1))) {
+              ok = false;
+              break;
+            }
+            uint8_t* dst = sb + Lay::kRing + slot * Lay::kTile;
+            mbar_arrive_expect_tx(&B.full[slot], Lay::kTile);
+            for (int c = 0; c < Lay::kChunks; ++c)
+              tma_load_4d(dst + c * 16384, kv ? tv : tk, c * 64, j * kFwKeys, g.h * (kv ? sd.mul_vh : sd.mul_kh),
+                          g.bi * (kv ? sd.mul_vb : sd.mul_kb), &B.full[slot]);
+            if (++slot == Lay::kStages) {
+              slot = 0;
+              ++use;
+            }
+          }
+        }
+      }
+      if (!ok) {
+        atomicExch(&B.abort_flag, 1);
+        // copies in flight land before the CTA may end
+        for (int i = 0; i < Lay::kStages; ++i) {
+          const int u = use - (i < slot ? 0 : 1);
+          if (u >= 0) mbar_wait(&B.full[i], u & 1);
+        }
+      }
+    }
+  } else if (warp == 9) {
+    // ---------------- MMA issuer
+    if (lane == 0 && !*abort_flag) {
+      constexpr uint32_t idesc_s = make_idesc(MmaKind::BF16, 128, 128);
+      constexpr uint32_t idesc_o = make_idesc(MmaKind::BF16, 128, HD) | (1u << 16);  // V is MN-major
+      FwCursor cur(A, B);
+      FwSeg g;
+      int slot = 0, use = 0;
+      int segs[2] = {0, 0}, tiles[2] = {0, 0};
+      auto advance = [&] {
+        if (++slot == Lay::kStages) {
+          slot = 0;
+          ++use;
+        }
+      };
+      auto issue_s = [&](int half, int ks) {
+        const uint32_t q = smem_u32(sb + Lay::kQ + half * Lay::kTile), k = smem_u32(sb + Lay::kRing + ks * Lay::kTile);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
+          umma<MmaKind::BF16>(tmem + half * 128, smem_desc_sw128(q + off), smem_desc_sw128(k + off), idesc_s, kk > 0);
+        }
+        umma_commit(&B.s_full[half]);
+      };
+      bool ok = true;
+      while (ok && cur.next(g)) {
+        const int halves = static_cast<int64_t>(g.rt) * kFwRows + 128 < side_rows(A.side[g.side].s) ? 2 : 1;
+        const int n = g.k1 - g.k0;
+        // first scores
+        if (!mbar_wait(&B.full[slot], use & 1)) { ok = false; break; }
+        for (int half = 0; half < halves; ++half) {
+          if (!mbar_wait(&B.q_full[half], segs[half] & 1)) { ok = false; break; }
+          ++segs[half];
+          tc_fence_after();
+          issue_s(half, slot);
+        }
+        if (!ok) break;
+        umma_commit(&B.empty[slot]);
+        advance();
+        for (int j = 0; ok && j < n; ++j) {
+          const int vs = slot, vu = use;
+          advance();
+          const int ks = slot, ku = use;
+          if (*abort_flag || !mbar_wait(&B.full[vs], vu & 1)) { ok = false; break; }
+          for (int half = 0; half < halves; ++half) {
+            if (!mbar_wait(&B.p_full[half], tiles[half] & 1)) { ok = false; break; }
+            ++tiles[half];
+            tc_fence_after();
+            const uint32_t v = smem_u32(sb + Lay::kRing + vs * Lay::kTile);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              umma_ts_f16(tmem + Lay::kTmemO + half * 128, tmem + half * 128 + kk * 8,
+                          smem_desc_sw128_mn(v + kk * 2048, 16384), idesc_o, j > 0 || kk > 0);
+            if (j + 1 < n) {
+              if (half == 0 && !mbar_wait(&B.full[ks], ku & 1)) { ok = false; break; }
+              issue_s(half, ks);
+            } else {
+              umma_commit(&B.o_done[half]);
+            }
+          }
+          if (!ok) break;
+          umma_commit(&B.empty[vs]);
+          if (j + 1 < n) {
+            umma_commit(&B.empty[ks]);
+            advance();
+          }
+        }
+      }
+      if (!ok) atomicExch(&B.abort_flag, 1);
+    }
+  } else {
+    // ---------------- softmax, a thread per row
+    const int half = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + half * 128 + lane_base, t_o = tmem + Lay::kTmemO + half * 128 + lane_base;
+    const float sl = A.scale_log2;
+    uint8_t* const q_tile = sb + Lay::kQ + half * Lay::kTile;
+    int seg_no = 0, tile_no = 0;
+    int v_slot = 1, v_use = 0;  // ring position of the current tile's V
+    auto skip = [&](int tiles) {
+      const int64_t p = static_cast<int64_t>(v_use) * Lay::kStages + v_slot + 2ll * tiles;
+      v_use = static_cast<int>(p / Lay::kStages);
+      v_slot = static_cast<int>(p - static_cast<int64_t>(v_use) * Lay::kStages);
+    };
+    // Q rows of an item into the swizzled tile: a warp loads its own 32 rows, HD / 8 lanes a row
+    auto load_q = [&](const FwSeg& g) {
+      const XSide& s = A.side[g.side].s;
+      const int64_t R = side_rows(s), row = static_cast<int64_t>(g.rt) * kFwRows + half * 128 + r;
+      const int64_t mine = row < R ? q_offset(s, g.bi, g.h, side_row(s, row)) : -1;
+      constexpr int kLanes = HD / 8, kPer = 32 / kLanes;
+      const int c = lane % kLanes;
+#pragma unroll
+      for (int i = 0; i < 32 / kPer; ++i) {
+        const int rr = i * kPer + lane / kLanes;
+        const int64_t off = __shfl_sync(0xffffffffu, mine, rr);
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (off >= 0 && c * 8 < A.D)
+          v = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(s.q) + off + c * 8));
+        v.x ^= A.q_flip;
+        v.y ^= A.q_flip;
+        v.z ^= A.q_flip;
+        v.w ^= A.q_flip;
+        const int tr = (warp & 3) * 32 + rr;
+        *reinterpret_cast<uint4*>(q_tile + (c >> 3) * 16384 + tr * 128 + (((c & 7) ^ (tr & 7)) << 4)) = v;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&B.q_full[half]);
+    };
+    auto active = [&](const FwSeg& g) {
+      return half == 0 || static_cast<int64_t>(g.rt) * kFwRows + 128 < side_rows(A.side[g.side].s);
+    };
+
+    FwCursor cur(A, B);
+    FwSeg g, gn;
+    bool have = !*abort_flag && cur.next(g);
+    bool ok = true;
+    if (have && active(g)) load_q(g);
+    while (have && ok) {
+      const bool more = cur.next(gn);
+      if (!active(g)) {
+        skip(g.k1 - g.k0);
+        if (more && active(gn)) load_q(gn);
+        have = more;
+        g = gn;
+        continue;
+      }
+      const XSide& s = A.side[g.side].s;
+      const int64_t R = side_rows(s), row = static_cast<int64_t>(g.rt) * kFwRows + half * 128 + r;
+      const bool live = row < R;
+      const XRow x = side_row(s, live ? row : 0);
+      const int len = side_len(s, g.bi);
+      const int lim = live ? row_limit(s, x, len) : 0;
+      const uint8_t* mask = s.mask ? s.mask + g.bi * s.mask_stride : nullptr;
+      const bool warp_live = __any_sync(0xffffffffu, live);
+      float m = -INFINITY, l = 0.f;
+      for (int j = g.k0; j < g.k1; ++j, ++tile_no) {
+        const int key0 = j * kFwKeys;
+        // which keys of the tile count at all; `part`: some are hidden from this warp's rows
+        uint32_t kept[4] = {~0u, ~0u, ~0u, ~0u};
+        const bool clean = mask == nullptr && key0 + kFwKeys <= len;
+        if (!clean) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 32 * i + lane;
+            kept[i] = __ballot_sync(0xffffffffu, key < len && (mask == nullptr || mask[key] != 0));
+          }
+        }
+        const bool part = !clean || __any_sync(0xffffffffu, live && key0 + kFwKeys > lim);
+        if (*abort_flag || !mbar_wait(&B.s_full[half], tile_no & 1)) { ok = false; break; }
+        if (warp_live) {
+          tc_fence_after();
+          uint32_t v[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, v[c]);
+          tmem_wait_ld();
+          const int left = lim - key0;  // columns the row may see
+          float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
+          if (part) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int n = min(max(left - 32 * c, 0), 32);
+              const uint32_t vis = kept[c] & (n == 32 ? ~0u : (1u << n) - 1u);
+              kept[c] = vis;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[c][i] = (vis >> i) & 1u ? v[c][i] : 0xff800000u;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            a0 = fmaxf(a0, __uint_as_float(v[0][i]));
+            a1 = fmaxf(a1, __uint_as_float(v[1][i]));
+            a2 = fmaxf(a2, __uint_as_float(v[2][i]));
+            a3 = fmaxf(a3, __uint_as_float(v[3][i]));
+          }
+          a0 = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
+          const float bmax = a0 == -INFINITY ? a0 : a0 * sl;
+          const float mnew = bmax > m + kFwLazy ? bmax : m;
+          const float mu = mnew == -INFINITY ? 0.f : mnew;
+          const float corr = ex2(m - mu);  // 1 when m stays, 0 before the first key
+          float q0 = 0.f, q1 = 0.f, q2 = 0.f, q3 = 0.f;
+          uint32_t pk[2][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              float e0 = ex2(fmaf(__uint_as_float(v[c][i]), sl, -mu));
+              float e1 = ex2(fmaf(__uint_as_float(v[c][i + 1]), sl, -mu));
+              float e2 = ex2(fmaf(__uint_as_float(v[c][i + 2]), sl, -mu));
+              float e3 = ex2(fmaf(__uint_as_float(v[c][i + 3]), sl, -mu));
+              if (part && sl == 0.f) {  // -inf * 0 is not a hidden score
+                e0 = (kept[c] >> i) & 1u ? e0 : 0.f;
+                e1 = (kept[c] >> (i + 1)) & 1u ? e1 : 0.f;
+                e2 = (kept[c] >> (i + 2)) & 1u ? e2 : 0.f;
+                e3 = (kept[c] >> (i + 3)) & 1u ? e3 : 0.f;
+              }
+              q0 += e0;
+              q1 += e1;
+              q2 += e2;
+              q3 += e3;
+              pk[c >> 1][(c & 1) * 16 + i / 2] = pack_bf16(e0, e1);
+              pk[c >> 1][(c & 1) * 16 + i / 2 + 1] = pack_bf16(e2, e3);
+            }
+          l = l * corr + ((q0 + q1) + (q2 + q3));
+          // s_full of this tile implies the previous P V has completed: O may be rescaled
+          if (j > g.k0 && __any_sync(0xffffffffu, mnew != m)) {
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(t_o + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_st32(t_o + c * 32, o);
+            }
+          }
+          m = mnew;
+          tmem_st32(t_s, pk[0]);
+          tmem_st32(t_s + 32, pk[1]);
+          tmem_wait_st();
+        }
+        if (half == 0 && !clean) {
+          // V rows of hidden keys become zeros before any product reads the tile (the second
+          // half's P V is issued after the first half's)
+          if (!mbar_wait(&B.full[v_slot], v_use & 1)) { ok = false; break; }
+          const int key = key0 + r;
+          if (!(key < len && (mask == nullptr || mask[key] != 0))) {
+            uint8_t* vr = sb + Lay::kRing + v_slot * Lay::kTile + r * 128;
+#pragma unroll
+            for (int c = 0; c < Lay::kChunks; ++c)
+#pragma unroll
+              for (int u = 0; u < 8; ++u) *reinterpret_cast<uint4*>(vr + c * 16384 + u * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        mbar_arrive(&B.p_full[half]);
+        skip(1);
+      }
+      if (!ok) break;
+      // every score product of this item has run: the next item's Q may take the tile
+      if (more && active(gn)) load_q(gn);
+      if (!mbar_wait(&B.o_done[half], seg_no & 1) || *abort_flag) { ok = false; break; }
+      ++seg_no;
+      tc_fence_after();
+      if (warp_live) {
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        const float ls = l == 0.f ? -INFINITY : m + log2f(l);
+        const bool all = g.k0 == 0 && g.k1 == g.n;
+        float* po = nullptr;
+        __nv_bfloat16* ob = nullptr;
+        if (live) {
+          if (!all) {
+            const int64_t at = (2ll * blockIdx.x + (g.k0 == 0 ? 1 : 0)) * A.slot_rows + half * 128 + r;
+            po = A.slots + at * A.D;
+            A.slot_lse[at] = ls;
+          } else {
+            const int64_t fr = flat_row(s, g.bi, g.h, x);
+            if (A.direct[g.side] != nullptr) {
+              po = A.direct[g.side] + fr * A.D;
+              A.direct_lse[g.side][fr] = ls;
+            } else {
+              ob = A.out + o_offset(s, g.bi, g.h, x);
+              if (A.lse != nullptr) A.lse[fr] = ls;
+            }
+          }
+        }
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + c * 32, o);
+          tmem_wait_ld();
+          auto f = [&](int i) { return __uint_as_float(o[i]) * inv; };
+          if (po != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              if (c * 32 + i < A.D)
+                *reinterpret_cast<float4*>(po + c * 32 + i) = make_float4(f(i), f(i + 1), f(i + 2), f(i + 3));
+          } else if (ob != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              if (c * 32 + i < A.D)
+                *reinterpret_cast<uint4*>(ob + c * 32 + i) =
+                    make_uint4(pack_bf16(f(i), f(i + 1)), pack_bf16(f(i + 2), f(i + 3)), pack_bf16(f(i + 4), f(i + 5)),
+                               pack_bf16(f(i + 6), f(i + 7)));
+          }
+        }
+      }
+      tc_fence_before();  // O is read before the next item's first P V (ordered by p_full)
+      have = more;
+      g = gn;
+    }
+    if (!ok) atomicExch(&B.abort_flag, 1);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the pieces of every row of the split part. One side: block (item, 8 rows), items that one CTA
+// finished are done already. Two sides: block = 8 output rows, each with a prefix and an own part.
+__global__ void __launch_bounds__(256) xattn_join_kernel(const __grid_constant__ FwArgs A, int G) {
+  grid_dep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int64_t fr;
+  int bi, h;
+  XRow x;
+  float mx = -INFINITY;
+  float den = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](const float* po, float ls) {
+    if (ls == -INFINITY) return;
+    if (ls > mx) {
+      const float c = exp2f(mx - ls);
+      den *= c;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] *= c;
+      mx = ls;
+    }
+    const float w = exp2f(ls - mx);
+    den += w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 32 * i < A.D) acc[i] = fmaf(w, po[lane + 32 * i], acc[i]);
+  };
+  auto add_pieces = [&](int2 p, int in_tile) {
+    for (int c = p.x; c <= p.y; ++c) {
+      const int64_t at = (2ll * c + (c == p.x ? 1 : 0)) * A.slot_rows + in_tile;
+      add(A.slots + at * A.D, A.slot_lse[at]);
+    }
+  };
+  if (A.sides == 1) {
+    const FwSide& S = A.side[0];
+    const int2 p = A.pieces[blockIdx.x];
+    if (p.x == p.y) return;
+    const int item = blockIdx.x + A.whole * G, per = S.s.hkv * S.row_tiles;
+    bi = item / per;
+    const int rem = item - bi * per, in_tile = blockIdx.y * 8 + warp;
+    h = rem / S.row_tiles;
+    const int64_t row = static_cast<int64_t>(rem - h * S.row_tiles) * kFwRows + in_tile;
+    if (row >= side_rows(S.s)) return;
+    x = side_row(S.s, row);
+    fr = flat_row(S.s, bi, h, x);
+    add_pieces(p, in_tile);
+  } else {
+    fr = static_cast<int64_t>(blockIdx.x) * 8 + warp;
+    if (fr >= A.rows_all) return;
+    const XSide& s = A.side[1].s;
+    x.t = static_cast<int>(fr % s.T);
+    const int64_t bh = fr / s.T;
+    const int hq = static_cast<int>(bh % (s.hkv * s.G));
+    bi = static_cast<int>(bh / (s.hkv * s.G));
+    h = hq / s.G;
+    x.g = hq - h * s.G;
+    x.b2 = 0;
+    for (int sd = 0; sd < 2; ++sd) {
+      const FwSide& S = A.side[sd];
+      const int64_t row = ((sd == 0 ? static_cast<int64_t>(bi) * s.G : 0) + x.g) * s.T + x.t;
+      const int rt = static_cast<int>(row / kFwRows);
+      const int item = ((sd == 0 ? 0 : bi) * s.hkv + h) * S.row_tiles + rt;
+      const int2 p = A.pieces[(sd == 0 ? 0 : A.side[0].items) + item];
+      if (p.x == p.y) add(A.direct[sd] + fr * A.D, A.direct_lse[sd][fr]);
+      else add_pieces(p, static_cast<int>(row - static_cast<int64_t>(rt) * kFwRows));
+    }
+  }
+  const XSide& s = A.side[A.sides - 1].s;
+  __nv_bfloat16* po = A.out + o_offset(s, bi, h, x);
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 32 * i < A.D) po[lane + 32 * i] = __float2bfloat16_rn(acc[i] * inv);
+  if (A.lse != nullptr && lane == 0) A.lse[fr] = den == 0.f ? -INFINITY : mx + log2f(den);
+}
+
+struct FwPlan {
+  int grid, whole, slot_rows, split_items;
+  size_t slots, slot_lse, direct, direct_lse, pieces, total;  // byte offsets
+};
+
+FwPlan fw_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n) {
+  FwPlan p = {};
+  const int sms = sm_count();
+  int64_t most = 0, tiles = 0, items = 0;
+  for (int i = 0; i < n; ++i) {
+    const int64_t R = side_rows(s[i]), it = (R + kFwRows - 1) / kFwRows * s[i].nb * s[i].hkv;
+    most = most > R ? most : R;
+    items += it;
+    tiles += it * ((s[i].klen + kFwKeys - 1) / kFwKeys);
+  }
+  p.grid = static_cast<int>(tiles < sms ? (tiles > 0 ? tiles : 1) : sms);
+  // one side: whole items for all but the last one to two rounds
+  if (n == 1 && items >= 2ll * p.grid) p.whole = static_cast<int>(items / p.grid - 1);
+  p.split_items = static_cast<int>(items - static_cast<int64_t>(p.whole) * p.grid);
+  p.slot_rows = static_cast<int>(most < kFwRows ? most : kFwRows);
+  const int64_t D = a->head_dim, slot = 2ll * p.grid * p.slot_rows, rows = a->batch * a->q_heads * a->q_len;
+  p.slots = 0;
+  p.slot_lse = align256(sizeof(float) * slot * D);
+  p.direct = p.slot_lse + align256(sizeof(float) * slot);
+  p.direct_lse = p.direct + (n > 1 ? align256(2 * sizeof(float) * rows * D) : 0);
+  p.pieces = p.direct_lse + (n > 1 ? align256(2 * sizeof(float) * rows) : 0);
+  p.total = p.pieces + align256(sizeof(int2) * p.split_items);
+  return p;
+}
+
+template <int HD>
+int fw_launch(const FwArgs& A, const XMap (&m)[4], int grid, cudaStream_t st) {
+  using Lay = FwLayout<HD>;
+  auto kern = xattn_fwd_tc_kernel<HD>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kSmem);
+  if (e != cudaSuccess) return cuda_status(e, "attention (tensor cores): set smem");
+  kern<<<grid, kFwThreads, Lay::kSmem, st>>>(m[0].map, m[1].map, m[2].map, m[3].map, A);
+  TSB_CHECK_LAUNCH("attention (tensor cores) launch");
+  return debug_sync(st, "attention (tensor cores)");
+}
+
+}  // namespace
+
+bool xattn_tc_ok(const trnsparse_attention_args* a, bool prefix) {
+  if (a->dtype != TRNSPARSE_BF16 || a->head_dim % 8 || a->head_dim > 128) return false;
+  if (prefix ? a->prefix_len + a->k_len == 0 : a->k_len == 0) return false;
+  if (!aligned16(a->q) || !aligned16(a->out)) return false;
+  if (!strides_ok(a->q_strides, a->batch, a->q_heads, a->q_len, false) ||
+      !strides_ok(a->out_strides, a->batch, a->q_heads, a->q_len, false))
+    return false;
+  if (a->k_len > 0 && (!aligned16(a->k) || !aligned16(a->v) ||
+                       !strides_ok(a->k_strides, a->batch, a->kv_heads, a->k_len, true) ||
+                       !strides_ok(a->v_strides, a->batch, a->kv_heads, a->k_len, true)))
+    return false;
+  if (prefix && a->prefix_len > 0) {
+    const int64_t ks[3] = {0, a->prefix_k_strides[0], a->prefix_k_strides[1]};
+    const int64_t vs[3] = {0, a->prefix_v_strides[0], a->prefix_v_strides[1]};
+    if (!aligned16(a->prefix_k) || !aligned16(a->prefix_v) || !strides_ok(ks, 1, a->kv_heads, a->prefix_len, true) ||
+        !strides_ok(vs, 1, a->kv_heads, a->prefix_len, true))
+      return false;
+  }
+  return true;
+}
+
+size_t xattn_tc_workspace(const trnsparse_attention_args* a, bool prefix) {
+  XSide s[2];
+  int n = 0;
+  if (make_sides(a, prefix, s, &n)) return 0;
+  return fw_plan(a, s, n).total;
+}
+
+int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, cudaStream_t st) {
+  XSide s[2];
+  int n = 0;
+  int rc = make_sides(a, prefix, s, &n);
+  if (rc) return rc;
+  const FwPlan p = fw_plan(a, s, n);
+  FwArgs A = {};
+  XMap m[4];
+  char* w = static_cast<char*>(ws);
+  const int64_t rows = a->batch * a->q_heads * a->q_len, D = a->head_dim;
+  for (int i = 0; i < n; ++i) {
+    FwSide& S = A.side[i];
+    S.s = s[i];
+    S.row_tiles = static_cast<int>((side_rows(s[i]) + kFwRows - 1) / kFwRows);
+    S.items = S.row_tiles * s[i].nb * s[i].hkv;
+    rc = make_xmap(&m[2 * i], s[i].k, D, s[i].klen, s[i].hkv, s[i].nb, s[i].k_t, s[i].k_h, s[i].k_b, 128);
+    if (rc) return rc;
+    rc = make_xmap(&m[2 * i + 1], s[i].v, D, s[i].klen, s[i].hkv, s[i].nb, s[i].v_t, s[i].v_h, s[i].v_b, 128);
+    if (rc) return rc;
+    S.mul_kh = m[2 * i].mul_h;
+    S.mul_kb = m[2 * i].mul_b;
+    S.mul_vh = m[2 * i + 1].mul_h;
+    S.mul_vb = m[2 * i + 1].mul_b;
+    if (n > 1) {
+      A.direct[i] = reinterpret_cast<float*>(w + p.direct) + i * rows * D;
+      A.direct_lse[i] = reinterpret_cast<float*>(w + p.direct_lse) + i * rows;
+    }
+  }
+  for (int i = 2 * n; i < 4; ++i) m[i] = m[i - 2];
+  A.sides = n;
+  A.D = static_cast<int>(D);
+  A.whole = p.whole;
+  A.slot_rows = p.slot_rows;
+  A.rows_all = rows;
+  A.slots = reinterpret_cast<float*>(w + p.slots);
+  A.slot_lse = reinterpret_cast<float*>(w + p.slot_lse);
+  A.pieces = reinterpret_cast<int2*>(w + p.pieces);
+  A.out = static_cast<__nv_bfloat16*>(a->out);
+  A.lse = a->lse;
+  A.scale_log2 = static_cast<float>(fabs(a->scale) * 1.4426950408889634);
+  A.q_flip = a->scale < 0 ? 0x80008000u : 0u;
+  rc = D <= 64 ? fw_launch<64>(A, m, p.grid, st) : fw_launch<128>(A, m, p.grid, st);
+  if (rc) return rc;
+  const dim3 grid = n == 1 ? dim3(p.split_items, (p.slot_rows + 7) / 8) : dim3((unsigned)((rows + 7) / 8));
+  cudaError_t e = launch_pdl(xattn_join_kernel, grid, dim3(256), 0, st, A, p.grid);
+  if (e != cudaSuccess) return cuda_status(e, "attention (tensor cores): join");
+  return debug_sync(st, "attention (tensor cores): join");
+}
+
+}  // namespace tsb

@@ -73,5 +73,9 @@ int check_attention(const trnsparse_attention_args* a, const char* what);
 int combine_pieces(const float* part_o, const float* part_lse, int pieces, const trnsparse_attention_args* a,
                    cudaStream_t st);
 
+// Tensor-core forms (bf16, head_dim a multiple of 8 up to 128, 16-byte rows).
+bool xattn_tc_ok(const trnsparse_attention_args* a, bool prefix);
+size_t xattn_tc_workspace(const trnsparse_attention_args* a, bool prefix);
+int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, cudaStream_t st);
 
 }  // namespace tsb
