@@ -442,6 +442,7 @@ using namespace tsb;
 
 extern "C" size_t trnsparse_cross_attention_backward_workspace_size(const trnsparse_attention_args* a) {
   if (check_attention(a, "cross_attention backward") || a->batch * a->q_heads * a->q_len == 0) return 0;
+  if (xattn_bwd_tc_ok(a)) return xattn_bwd_tc_workspace(a);
   XSide s[2];
   int n = 0;
   make_sides(a, false, s, &n);
@@ -459,5 +460,6 @@ extern "C" int trnsparse_cross_attention_backward(const trnsparse_attention_args
   TSB_REQUIRE(ws && ws_bytes >= need, "cross_attention backward: workspace too small (%zu bytes, needs %zu)", ws_bytes,
               need);
   cudaStream_t st = as_stream(stream);
+  if (xattn_bwd_tc_ok(a)) return xattn_bwd_tc(a, ws, st);
   return a->dtype == TRNSPARSE_F32 ? bwd_simt<float>(a, ws, st) : bwd_simt<__nv_bfloat16>(a, ws, st);
 }

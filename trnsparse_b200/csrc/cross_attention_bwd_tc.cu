@@ -1,0 +1,657 @@
+// Backward of cross attention on the tensor cores (bf16 operands, fp32 sums;
+// head_dim a multiple of 8 up to 128):
+//   P = 2^(s2 - lse), dP = dO V^T, dS = P (dP - D), D = rowsum(dO o O),
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO   (dK, dV over the group's heads).
+// P and dS are formed in fp32 and rounded to bf16 once, as operands of their
+// products (half a step each, of the size of the results' own rounding).
+//
+// Two launches of one kernel, each owning what it writes (fixed order, no
+// atomics, seven products for the mathematics' five):
+//   rows     fixed Q, dO of 128 query rows; walks the key tiles       -> dQ
+//   columns  fixed K, V of 128 keys; walks the 128-row tiles of every
+//            query head of the group                                  -> dK, dV
+// A step multiplies two fixed tiles F1, F2 and two walked tiles X1, X2:
+//   S = F1 X1^T, dP = F2 X2^T, acc0 += dS X1, and in columns acc1 += P X2.
+// One CTA per SM, 10 warps: warp 8 TMA producer, warp 9 MMA issuer, warps 0-7
+// the pointwise part (thread = TMEM lane warp % 4, 64 of the 128 columns). P
+// overwrites S and dS overwrites dP in TMEM (A operands of the second
+// products), each half of the columns at the start of its own 64. MMAs run in
+// issue order, so per step: acc1 += P_j X2_j, S_{j+1}, acc0 += dS_j X1_j,
+// dP_{j+1}: the next scores are there when the pointwise warps return.
+//
+// What bounds it: the walked tiles, 64 KB a step at head_dim 128 from L2 at
+// 40-50 GB/s per SM (about 1.4 us), against 3 (rows) or 4 (columns) products of
+// 0.26 us.
+//
+// Hidden keys: P and dS are set to zero by selection; in rows the K rows of
+// hidden keys are zeroed in shared memory before dS K, so NaN in padding meets
+// no product that is kept. In columns a hidden key is a lane of its own.
+#include "xattn_tc.cuh"
+
+namespace tsb {
+namespace {
+
+constexpr int kBwThreads = 320;
+
+template <int HD>
+struct BwLayout {
+  static constexpr int kChunks = HD / 64;
+  static constexpr int kTile = 128 * HD * 2;
+  static constexpr int kX1Stages = 3, kX2Stages = 2;
+  static constexpr int kX2Stage = kTile + 1024;  // with the walked rows' log-sum-exp and D
+  static constexpr int kF1 = 0, kF2 = kTile, kX1 = 2 * kTile;
+  static constexpr int kX2 = kX1 + kX1Stages * kTile;
+  static constexpr int kBar = kX2 + kX2Stages * kX2Stage;
+  static constexpr int kSmem = kBar + 256;
+  static constexpr uint32_t kTmemS = 0, kTmemDP = 128, kTmemAcc0 = 256, kTmemAcc1 = 384;
+};
+
+struct BwBars {
+  uint64_t f_full, f_empty, x1_full[3], x1_empty[3], x2_full[2], x2_empty[2];
+  uint64_t s_full, dp_full, p_full, ds_full, acc_full;
+  uint32_t tmem_slot;
+  int abort_flag;
+};
+
+struct BwArgs {
+  const int* lengths;
+  const uint8_t* mask;
+  int64_t mask_stride;
+  const float *lse, *delta;  // [batch, q_heads, padded tokens]
+  void *out0, *out1;         // dQ, or dK and dV
+  int64_t s0[3], s1[3];      // their strides
+  float *part0, *part1;      // fp32 parts [parts][rows][D], or null
+  int64_t part_rows;
+  int B, Hq, Hkv, G, Sq, Sk, D, q_tiles, k_tiles, parts, chunk;
+  int mul_h[4], mul_b[4];    // q, dout, k, v
+  float scale, scale_log2;
+};
+
+__device__ __forceinline__ int bw_len(const BwArgs& A, int b) {
+  return A.lengths == nullptr ? A.Sk : max(0, min(A.lengths[b], A.Sk));
+}
+
+// Unit u: part p of the walk of a fixed tile; b outermost, so round-robin CTAs see every length alike.
+struct BwUnit {
+  int b, h, tile, part, beg, end;  // h: query head (rows) or key head (columns)
+};
+template <bool COL>
+__device__ __forceinline__ BwUnit bw_unit(const BwArgs& A, int u) {
+  const int heads = COL ? A.Hkv : A.Hq, tiles = COL ? A.k_tiles : A.q_tiles;
+  BwUnit x;
+  x.part = u % A.parts;
+  u /= A.parts;
+  x.tile = u % tiles;
+  u /= tiles;
+  x.h = u % heads;
+  x.b = u / heads;
+  const int len = bw_len(A, x.b);
+  const int steps = COL ? (x.tile * 128 < len ? A.G * A.q_tiles : 0) : (len + 127) / 128;
+  x.beg = min(steps, x.part * A.chunk);
+  x.end = min(steps, x.beg + A.chunk);
+  return x;
+}
+
+template <int HD, bool COL>
+__global__ void __launch_bounds__(kBwThreads, 1)
+xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tg,
+                    const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                    const __grid_constant__ BwArgs A, int units) {
+  using Lay = BwLayout<HD>;
+  extern __shared__ __align__(16) uint8_t sb[];  // no static shared memory: 1024-byte aligned
+  BwBars& B = *reinterpret_cast<BwBars*>(sb + Lay::kBar);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(&B.f_full, 1);
+    mbar_init(&B.f_empty, 1);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&B.x1_full[i], 1);
+      mbar_init(&B.x1_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&B.x2_full[i], 1);
+      mbar_init(&B.x2_empty[i], 1);
+    }
+    mbar_init(&B.s_full, 1);
+    mbar_init(&B.dp_full, 1);
+    mbar_init(&B.p_full, 256);
+    mbar_init(&B.ds_full, 256);
+    mbar_init(&B.acc_full, 1);
+    B.abort_flag = (smem_u32(sb) & 1023u) ? 1 : 0;
+    if (B.abort_flag) record_device_error(DEVERR_SELFCHECK_SMEM);
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&B.tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  grid_dep_wait();  // the row sums come from the kernel before
+  const uint32_t tmem = B.tmem_slot;
+  volatile int* abort_flag = &B.abort_flag;
+  const int padded = A.q_tiles * 128;
+
+  if (warp == 8) {
+    // ---------------- producers: lane 0 the fixed tiles and X1, lane 1 X2
+    if (lane < 2 && !*abort_flag) {
+      int n = 0, nu = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+        const BwUnit x = bw_unit<COL>(A, u);
+        if (x.beg >= x.end) continue;
+        if (lane == 0) {
+          if (nu > 0 && !mbar_wait(&B.f_empty, (nu - 1) & 1)) { ok = false; break; }
+          mbar_arrive_expect_tx(&B.f_full, 2 * Lay::kTile);
+          for (int c = 0; c < Lay::kChunks; ++c) {
+            if (COL) {
+              tma_load_4d(sb + Lay::kF1 + c * 16384, &tk, c * 64, x.tile * 128, x.h * A.mul_h[2], x.b * A.mul_b[2], &B.f_full);
+              tma_load_4d(sb + Lay::kF2 + c * 16384, &tv, c * 64, x.tile * 128, x.h * A.mul_h[3], x.b * A.mul_b[3], &B.f_full);
+            } else {
+              tma_load_4d(sb + Lay::kF1 + c * 16384, &tq, c * 64, x.tile * 128, x.h * A.mul_h[0], x.b * A.mul_b[0], &B.f_full);
+              tma_load_4d(sb + Lay::kF2 + c * 16384, &tg, c * 64, x.tile * 128, x.h * A.mul_h[1], x.b * A.mul_b[1], &B.f_full);
+            }
+          }
+        }
+        ++nu;
+        for (int s = x.beg; s < x.end; ++s, ++n) {
+          int h, row;
+          if (COL) {
+            const int g = s / A.q_tiles;
+            h = x.h * A.G + g;
+            row = (s - g * A.q_tiles) * 128;
+          } else {
+            h = x.h / A.G;
+            row = s * 128;
+          }
+          if (lane == 0) {
+            const int st = n % Lay::kX1Stages, use = n / Lay::kX1Stages;
+            if (*abort_flag || (use > 0 && !mbar_wait(&B.x1_empty[st], (use - 1) & 1))) { ok = false; break; }
+            uint8_t* dst = sb + Lay::kX1 + st * Lay::kTile;
+            mbar_arrive_expect_tx(&B.x1_full[st], Lay::kTile);
+            constexpr int w = COL ? 0 : 2;
+            for (int c = 0; c < Lay::kChunks; ++c)
+              tma_load_4d(dst + c * 16384, COL ? &tq : &tk, c * 64, row, h * A.mul_h[w], x.b * A.mul_b[w], &B.x1_full[st]);
+          } else {
+            const int st = n % Lay::kX2Stages, use = n / Lay::kX2Stages;
+            if (*abort_flag || (use > 0 && !mbar_wait(&B.x2_empty[st], (use - 1) & 1))) { ok = false; break; }
+            uint8_t* dst = sb + Lay::kX2 + st * Lay::kX2Stage;
+            mbar_arrive_expect_tx(&B.x2_full[st], Lay::kTile + (COL ? 1024 : 0));
+            constexpr int w = COL ? 1 : 3;
+            for (int c = 0; c < Lay::kChunks; ++c)
+              tma_load_4d(dst + c * 16384, COL ? &tg : &tv, c * 64, row, h * A.mul_h[w], x.b * A.mul_b[w], &B.x2_full[st]);
+            if (COL) {
+              const int64_t at = (static_cast<int64_t>(x.b) * A.Hq + h) * padded + row;
+              bulk_g2s(dst + Lay::kTile, A.lse + at, 512, &B.x2_full[st]);
+              bulk_g2s(dst + Lay::kTile + 512, A.delta + at, 512, &B.x2_full[st]);
+            }
+          }
+        }
+      }
+      if (!ok) {
+        atomicExch(&B.abort_flag, 1);
+        // copies in flight land before the CTA may end
+        if (lane == 0) {
+          if (nu > 0) mbar_wait(&B.f_full, (nu - 1) & 1);
+          for (int i = max(0, n - Lay::kX1Stages); i < n; ++i)
+            mbar_wait(&B.x1_full[i % Lay::kX1Stages], (i / Lay::kX1Stages) & 1);
+        } else {
+          for (int i = max(0, n - Lay::kX2Stages); i < n; ++i)
+            mbar_wait(&B.x2_full[i % Lay::kX2Stages], (i / Lay::kX2Stages) & 1);
+        }
+      }
+    }
+  } else if (warp == 9) {
+    // ---------------- MMA issuer
+    if (lane == 0 && !*abort_flag) {
+      constexpr uint32_t idesc_s = make_idesc(MmaKind::BF16, 128, 128);
+      constexpr uint32_t idesc_a = make_idesc(MmaKind::BF16, 128, HD) | (1u << 16);  // walked tile MN-major
+      const uint32_t f1 = smem_u32(sb + Lay::kF1), f2 = smem_u32(sb + Lay::kF2);
+      auto product = [&](uint32_t d, uint32_t fa, uint32_t xa) {
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
+          umma<MmaKind::BF16>(d, smem_desc_sw128(fa + off), smem_desc_sw128(xa + off), idesc_s, kk > 0);
+        }
+      };
+      // acc += A X with A packed in TMEM: columns 64 h .. of half h
+      auto accumulate = [&](uint32_t acc, uint32_t a, uint32_t xa, bool first) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_ts_f16(acc, a + (kk >> 2) * 64 + (kk & 3) * 8, smem_desc_sw128_mn(xa + kk * 2048, 16384), idesc_a,
+                      !first || kk > 0);
+      };
+      auto x1_addr = [&](int i) { return smem_u32(sb + Lay::kX1 + (i % Lay::kX1Stages) * Lay::kTile); };
+      auto x2_addr = [&](int i) { return smem_u32(sb + Lay::kX2 + (i % Lay::kX2Stages) * Lay::kX2Stage); };
+      auto wait_x1 = [&](int i) { return mbar_wait(&B.x1_full[i % Lay::kX1Stages], (i / Lay::kX1Stages) & 1); };
+      auto wait_x2 = [&](int i) { return mbar_wait(&B.x2_full[i % Lay::kX2Stages], (i / Lay::kX2Stages) & 1); };
+      int n = 0, nu = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+        const BwUnit x = bw_unit<COL>(A, u);
+        const int steps = x.end - x.beg;
+        if (steps <= 0) continue;
+        if (!mbar_wait(&B.f_full, nu & 1) || !wait_x1(n)) { ok = false; break; }
+        ++nu;
+        tc_fence_after();
+        product(tmem + Lay::kTmemS, f1, x1_addr(n));
+        umma_commit(&B.s_full);
+        if (!wait_x2(n)) { ok = false; break; }
+        product(tmem + Lay::kTmemDP, f2, x2_addr(n));
+        umma_commit(&B.dp_full);
+        if (!COL) umma_commit(&B.x2_empty[n % Lay::kX2Stages]);
+        if (steps == 1) umma_commit(&B.f_empty);
+        for (int j = 0; j < steps; ++j, ++n) {
+          const bool more = j + 1 < steps;
+          if (*abort_flag || !mbar_wait(&B.p_full, n & 1)) { ok = false; break; }
+          tc_fence_after();
+          if (COL) accumulate(tmem + Lay::kTmemAcc1, tmem + Lay::kTmemS, x2_addr(n), j == 0);
+          if (more) {
+            if (!wait_x1(n + 1)) { ok = false; break; }
+            product(tmem + Lay::kTmemS, f1, x1_addr(n + 1));
+            umma_commit(&B.s_full);
+          }
+          if (!mbar_wait(&B.ds_full, n & 1)) { ok = false; break; }
+          tc_fence_after();
+          accumulate(tmem + Lay::kTmemAcc0, tmem + Lay::kTmemDP, x1_addr(n), j == 0);
+          umma_commit(&B.x1_empty[n % Lay::kX1Stages]);
+          // not before ds_full: the pointwise warps read D from the stage until then
+          if (COL) umma_commit(&B.x2_empty[n % Lay::kX2Stages]);
+          if (more) {
+            if (!wait_x2(n + 1)) { ok = false; break; }
+            product(tmem + Lay::kTmemDP, f2, x2_addr(n + 1));
+            umma_commit(&B.dp_full);
+            if (!COL) umma_commit(&B.x2_empty[(n + 1) % Lay::kX2Stages]);
+            if (j + 2 == steps) umma_commit(&B.f_empty);  // the last use of the fixed tiles
+          } else {
+            umma_commit(&B.acc_full);
+          }
+        }
+      }
+      if (!ok) atomicExch(&B.abort_flag, 1);
+    }
+  } else {
+    // ---------------- pointwise part: lane = fixed row, 64 columns a thread
+    const int half = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + Lay::kTmemS + lane_base + half * 64, t_dp = tmem + Lay::kTmemDP + lane_base + half * 64;
+    const float sl = A.scale_log2;
+    int n = 0, nu = 0;
+    bool ok = !*abort_flag;
+    for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+      const BwUnit x = bw_unit<COL>(A, u);
+      const int len = bw_len(A, x.b);
+      const uint8_t* mask = A.mask ? A.mask + x.b * A.mask_stride : nullptr;
+      const int fixed = x.tile * 128 + r;
+      float row_lse = 0.f, row_delta = 0.f;
+      bool dead = false;  // columns: this key is hidden
+      if (COL) {
+        dead = fixed >= len || (mask && !mask[fixed]);
+      } else {
+        const int64_t at = (static_cast<int64_t>(x.b) * A.Hq + x.h) * padded + fixed;
+        row_lse = A.lse[at];
+        row_delta = A.delta[at];
+      }
+      for (int s = x.beg; s < x.end; ++s, ++n) {
+        uint32_t kept[2] = {~0u, ~0u};
+        bool part = false;
+        if (!COL) {
+          part = mask != nullptr || s * 128 + 128 > len;
+          if (part) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int key = s * 128 + half * 64 + 32 * i + lane;
+              kept[i] = __ballot_sync(0xffffffffu, key < len && (mask == nullptr || mask[key] != 0));
+            }
+          }
+        }
+        const float* st = reinterpret_cast<const float*>(sb + Lay::kX2 + (n % Lay::kX2Stages) * Lay::kX2Stage + Lay::kTile) + half * 64;
+        if (*abort_flag || !mbar_wait(&B.s_full, n & 1)) { ok = false; break; }
+        if (COL && !mbar_wait(&B.x2_full[n % Lay::kX2Stages], (n / Lay::kX2Stages) & 1)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t p[2][32];
+        tmem_ld32(t_s, p[0]);
+        tmem_ld32(t_s + 32, p[1]);
+        tmem_wait_ld();
+        if (!COL) {
+          tc_fence_before();
+          mbar_arrive(&B.p_full);  // the score columns may be written again
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            float4 ls = make_float4(row_lse, row_lse, row_lse, row_lse);
+            if (COL) ls = *reinterpret_cast<const float4*>(st + c * 32 + i);
+            float e[4];
+            e[0] = ex2(fmaf(__uint_as_float(p[c][i]), sl, -ls.x));
+            e[1] = ex2(fmaf(__uint_as_float(p[c][i + 1]), sl, -ls.y));
+            e[2] = ex2(fmaf(__uint_as_float(p[c][i + 2]), sl, -ls.z));
+            e[3] = ex2(fmaf(__uint_as_float(p[c][i + 3]), sl, -ls.w));
+#pragma unroll
+            for (int q = 0; q < 4; ++q) p[c][i + q] = __float_as_uint(COL && dead ? 0.f : e[q]);
+          }
+        if (!COL && part) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) p[c][i] = (kept[c] >> i) & 1u ? p[c][i] : 0u;
+          // hidden keys' K rows become zeros before dS K (their scores are read already)
+          if (half == 0) {
+            const int key = s * 128 + r;
+            if (!(key < len && (mask == nullptr || mask[key] != 0))) {
+              uint8_t* kr = sb + Lay::kX1 + (n % Lay::kX1Stages) * Lay::kTile + r * 128;
+#pragma unroll
+              for (int c = 0; c < Lay::kChunks; ++c)
+#pragma unroll
+                for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(kr + c * 16384 + q * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+          }
+        }
+        if (COL) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+              pk[c * 16 + i / 2] = pack_bf16(__uint_as_float(p[c][i]), __uint_as_float(p[c][i + 1]));
+          tmem_st32(t_s, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&B.p_full);
+        }
+        if (!mbar_wait(&B.dp_full, n & 1)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t ds[32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t dp[32];
+          tmem_ld32(t_dp + c * 32, dp);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            float4 de = make_float4(row_delta, row_delta, row_delta, row_delta);
+            if (COL) de = *reinterpret_cast<const float4*>(st + 128 + c * 32 + i);
+            float t[4];
+            t[0] = __uint_as_float(p[c][i]) * (__uint_as_float(dp[i]) - de.x);
+            t[1] = __uint_as_float(p[c][i + 1]) * (__uint_as_float(dp[i + 1]) - de.y);
+            t[2] = __uint_as_float(p[c][i + 2]) * (__uint_as_float(dp[i + 2]) - de.z);
+            t[3] = __uint_as_float(p[c][i + 3]) * (__uint_as_float(dp[i + 3]) - de.w);
+            if (COL) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) t[q] = dead ? 0.f : t[q];
+            } else if (part) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) t[q] = (kept[c] >> (i + q)) & 1u ? t[q] : 0.f;
+            }
+            ds[c * 16 + i / 2] = pack_bf16(t[0], t[1]);
+            ds[c * 16 + i / 2 + 1] = pack_bf16(t[2], t[3]);
+          }
+        }
+        tmem_st32(t_dp, ds);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&B.ds_full);
+      }
+      if (!ok) break;
+      // ---- accumulators -> global; a unit without steps writes zeros
+      const bool worked = x.beg < x.end;
+      if (worked) {
+        if (!mbar_wait(&B.acc_full, nu & 1) || *abort_flag) { ok = false; break; }
+        ++nu;
+        tc_fence_after();
+      }
+      const bool live = fixed < (COL ? A.Sk : A.Sq);
+      const int64_t fr = (static_cast<int64_t>(x.b) * (COL ? A.Hkv : A.Hq) + x.h) * (COL ? A.Sk : A.Sq) + fixed;
+#pragma unroll
+      for (int a = 0; a < (COL ? 2 : 1); ++a) {
+        const int64_t* os = a ? A.s1 : A.s0;
+        const float f = a ? 1.f : A.scale;
+        float* po = a ? A.part1 : A.part0;
+        __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(a ? A.out1 : A.out0) + x.b * os[0] + x.h * os[1] + fixed * os[2];
+        if (po != nullptr) po += (static_cast<int64_t>(x.part) * A.part_rows + fr) * A.D;
+#pragma unroll 1
+        for (int c = 0; c < HD / 64; ++c) {  // half h: columns h HD / 2 ..
+          const int d0 = half * (HD / 2) + c * 32;
+          uint32_t v[32];
+          if (worked) {
+            tmem_ld32(tmem + (a ? Lay::kTmemAcc1 : Lay::kTmemAcc0) + lane_base + d0, v);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0u;
+          }
+          auto val = [&](int i) { return __uint_as_float(v[i]) * f; };
+          if (live && po != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              if (d0 + i < A.D)
+                *reinterpret_cast<float4*>(po + d0 + i) = make_float4(val(i), val(i + 1), val(i + 2), val(i + 3));
+          } else if (live) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              if (d0 + i < A.D)
+                *reinterpret_cast<uint4*>(ob + d0 + i) =
+                    make_uint4(pack_bf16(val(i), val(i + 1)), pack_bf16(val(i + 2), val(i + 3)),
+                               pack_bf16(val(i + 4), val(i + 5)), pack_bf16(val(i + 6), val(i + 7)));
+          }
+        }
+      }
+      tc_fence_before();  // the accumulators are read before the next unit's first product (ordered by p_full, ds_full)
+    }
+    if (!ok) atomicExch(&B.abort_flag, 1);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// D = rowsum(dO o O) and the log-sum-exp, padded to whole 128-row tiles (lse = +inf there: P = 0). 16 lanes a row.
+__global__ void __launch_bounds__(256) xattn_row_sums_kernel(const __nv_bfloat16* __restrict__ dout,
+                                                             const __nv_bfloat16* __restrict__ out,
+                                                             const float* __restrict__ lse, int64_t rows, int Hq,
+                                                             int Sq, int padded, int D, int64_t g_b, int64_t g_h,
+                                                             int64_t g_t, int64_t o_b, int64_t o_h, int64_t o_t,
+                                                             float* lse_pad, float* delta) {
+  grid_dep_launch();
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const int c = threadIdx.x & 15;
+  const bool in = row < rows;
+  const int64_t bh = in ? row / padded : 0;
+  const int t = in ? static_cast<int>(row - bh * padded) : 0;
+  float s = 0.f;
+  if (in && t < Sq && c * 8 < D) {
+    const int64_t b = bh / Hq, h = bh - b * Hq;
+    const uint4 g = *reinterpret_cast<const uint4*>(dout + b * g_b + h * g_h + t * g_t + c * 8);
+    const uint4 o = *reinterpret_cast<const uint4*>(out + b * o_b + h * o_h + t * o_t + c * 8);
+    const uint32_t gw[4] = {g.x, g.y, g.z, g.w}, ow[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s = fmaf(__uint_as_float(gw[i] << 16), __uint_as_float(ow[i] << 16), s);
+      s = fmaf(__uint_as_float(gw[i] & 0xffff0000u), __uint_as_float(ow[i] & 0xffff0000u), s);
+    }
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (in && c == 0) {
+    delta[row] = s;
+    lse_pad[row] = t < Sq ? lse[bh * Sq + t] : INFINITY;
+  }
+}
+
+// out[b, h, t, :] = sum of the parts, in order; 8 elements a thread.
+__global__ void __launch_bounds__(256) xattn_sum_bf16_kernel(const float* __restrict__ part, int parts, int64_t rows,
+                                                             __nv_bfloat16* out, int H, int L, int D, int64_t o_b,
+                                                             int64_t o_h, int64_t o_t) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8;
+  if (i >= rows * D) return;
+  const int64_t row = i / D;
+  const int d = static_cast<int>(i - row * D);
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < parts; ++p) {
+    const float4 a = *reinterpret_cast<const float4*>(part + p * rows * D + i);
+    const float4 b = *reinterpret_cast<const float4*>(part + p * rows * D + i + 4);
+    s[0] += a.x; s[1] += a.y; s[2] += a.z; s[3] += a.w;
+    s[4] += b.x; s[5] += b.y; s[6] += b.z; s[7] += b.w;
+  }
+  const int64_t bh = row / L, t = row - bh * L, b = bh / H, h = bh - b * H;
+  *reinterpret_cast<uint4*>(out + b * o_b + h * o_h + t * o_t + d) =
+      make_uint4(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]), pack_bf16(s[4], s[5]), pack_bf16(s[6], s[7]));
+}
+
+struct BwPlan {
+  int q_tiles, k_tiles, parts[2], chunk[2], units[2];  // [0] rows, [1] columns
+  size_t delta, part, total;
+};
+
+BwPlan bw_plan(const trnsparse_attention_args* a) {
+  BwPlan p = {};
+  const int sms = sm_count();
+  const int64_t G = a->q_heads / a->kv_heads;
+  p.q_tiles = static_cast<int>((a->q_len + 127) / 128);
+  p.k_tiles = static_cast<int>((a->k_len + 127) / 128);
+  const int64_t items[2] = {a->batch * a->q_heads * p.q_tiles, a->batch * a->kv_heads * p.k_tiles};
+  const int64_t steps[2] = {p.k_tiles, G * p.q_tiles};
+  const int64_t rows[2] = {a->batch * a->q_heads * a->q_len, 2 * a->batch * a->kv_heads * a->k_len};
+  size_t part = 0;
+  for (int i = 0; i < 2; ++i) {
+    // cut the walks where tiles are fewer than SMs; a part is at least four steps
+    int64_t parts = items[i] > 0 ? sms / items[i] : 1;
+    if (parts > steps[i] / 4) parts = steps[i] / 4;
+    if (parts < 1) parts = 1;
+    const int64_t chunk = steps[i] > 0 ? (steps[i] + parts - 1) / parts : 1;
+    p.chunk[i] = static_cast<int>(chunk);
+    p.parts[i] = static_cast<int>(steps[i] > 0 ? (steps[i] + chunk - 1) / chunk : 1);
+    p.units[i] = static_cast<int>(items[i] * p.parts[i]);
+    if (p.parts[i] > 1) {
+      const size_t b = sizeof(float) * static_cast<size_t>(p.parts[i]) * rows[i] * a->head_dim;
+      part = part > b ? part : b;
+    }
+  }
+  const size_t stats = align256(sizeof(float) * a->batch * a->q_heads * p.q_tiles * 128);
+  p.delta = stats;
+  p.part = 2 * stats;
+  p.total = p.part + part;
+  return p;
+}
+
+template <int HD, bool COL>
+int bw_launch(const BwArgs& A, const XMap (&m)[4], int units, cudaStream_t st) {
+  using Lay = BwLayout<HD>;
+  auto kern = xattn_bwd_tc_kernel<HD, COL>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kSmem);
+  if (e != cudaSuccess) return cuda_status(e, "cross_attention backward: set smem");
+  const int sms = sm_count();
+  e = launch_pdl(kern, dim3(units < sms ? units : sms), dim3(kBwThreads), Lay::kSmem, st, m[0].map, m[1].map,
+                 m[2].map, m[3].map, A, units);
+  if (e != cudaSuccess) return cuda_status(e, "cross_attention backward launch");
+  return debug_sync(st, COL ? "cross_attention backward: dK, dV" : "cross_attention backward: dQ");
+}
+
+int bw_sum(const float* part, int parts, int64_t rows, void* out, int H, int L, int D, const int64_t* os,
+           cudaStream_t st) {
+  const int64_t n = rows * D / 8;
+  xattn_sum_bf16_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(
+      part, parts, rows, static_cast<__nv_bfloat16*>(out), H, L, D, os[0], os[1], os[2]);
+  TSB_CHECK_LAUNCH("cross_attention backward: sum of parts");
+  return TRNSPARSE_OK;
+}
+
+}  // namespace
+
+bool xattn_bwd_tc_ok(const trnsparse_attention_args* a) {
+  if (!xattn_tc_ok(a, false)) return false;
+  const int64_t B = a->batch, Hq = a->q_heads, Hk = a->kv_heads, Sq = a->q_len, Sk = a->k_len;
+  if (!aligned16(a->dout) || !strides_ok(a->dout_strides, B, Hq, Sq, true) ||
+      !strides_ok(a->q_strides, B, Hq, Sq, true))
+    return false;
+  if (a->dq && (!aligned16(a->dq) || !strides_ok(a->dq_strides, B, Hq, Sq, false))) return false;
+  if (a->dk && (!aligned16(a->dk) || !aligned16(a->dv) || !strides_ok(a->dk_strides, B, Hk, Sk, false) ||
+                !strides_ok(a->dv_strides, B, Hk, Sk, false)))
+    return false;
+  // units and padded rows are counted in 31 bits
+  const int64_t qt = (Sq + 127) / 128, kt = (Sk + 127) / 128;
+  return B * Hq * qt < (1ll << 23) && B * Hk * kt < (1ll << 23) && (Hq / Hk) * qt < (1ll << 30);
+}
+
+size_t xattn_bwd_tc_workspace(const trnsparse_attention_args* a) { return bw_plan(a).total; }
+
+int xattn_bwd_tc(const trnsparse_attention_args* a, void* ws, cudaStream_t st) {
+  const BwPlan p = bw_plan(a);
+  const int64_t B = a->batch, Hq = a->q_heads, Hk = a->kv_heads, Sq = a->q_len, Sk = a->k_len, D = a->head_dim;
+  XMap m[4];
+  const int64_t *qs = a->q_strides, *gs = a->dout_strides, *ks = a->k_strides, *vs = a->v_strides;
+  int rc = make_xmap(&m[0], a->q, D, Sq, Hq, B, qs[2], qs[1], qs[0], 128);
+  if (!rc) rc = make_xmap(&m[1], a->dout, D, Sq, Hq, B, gs[2], gs[1], gs[0], 128);
+  if (!rc) rc = make_xmap(&m[2], a->k, D, Sk, Hk, B, ks[2], ks[1], ks[0], 128);
+  if (!rc) rc = make_xmap(&m[3], a->v, D, Sk, Hk, B, vs[2], vs[1], vs[0], 128);
+  if (rc) return rc;
+  char* w = static_cast<char*>(ws);
+  float *lse = reinterpret_cast<float*>(w), *delta = reinterpret_cast<float*>(w + p.delta);
+  float* part = reinterpret_cast<float*>(w + p.part);
+  const int64_t rows = B * Hq * p.q_tiles * 128;
+  const int64_t* os = a->out_strides;
+  xattn_row_sums_kernel<<<static_cast<unsigned>((rows + 15) / 16), 256, 0, st>>>(
+      static_cast<const __nv_bfloat16*>(a->dout), static_cast<const __nv_bfloat16*>(a->out), a->lse, rows, (int)Hq,
+      (int)Sq, p.q_tiles * 128, (int)D, gs[0], gs[1], gs[2], os[0], os[1], os[2], lse, delta);
+  TSB_CHECK_LAUNCH("cross_attention backward: row sums");
+  BwArgs A = {};
+  A.lengths = a->key_lengths;
+  A.mask = a->key_mask;
+  A.mask_stride = a->key_mask_stride;
+  A.lse = lse;
+  A.delta = delta;
+  A.B = (int)B;
+  A.Hq = (int)Hq;
+  A.Hkv = (int)Hk;
+  A.G = (int)(Hq / Hk);
+  A.Sq = (int)Sq;
+  A.Sk = (int)Sk;
+  A.D = (int)D;
+  A.q_tiles = p.q_tiles;
+  A.k_tiles = p.k_tiles;
+  for (int i = 0; i < 4; ++i) {
+    A.mul_h[i] = m[i].mul_h;
+    A.mul_b[i] = m[i].mul_b;
+  }
+  A.scale = static_cast<float>(a->scale);
+  A.scale_log2 = static_cast<float>(a->scale * 1.4426950408889634);
+  if (a->dk) {
+    A.out0 = a->dk;
+    A.out1 = a->dv;
+    for (int i = 0; i < 3; ++i) {
+      A.s0[i] = a->dk_strides[i];
+      A.s1[i] = a->dv_strides[i];
+    }
+    A.parts = p.parts[1];
+    A.chunk = p.chunk[1];
+    A.part_rows = B * Hk * Sk;
+    A.part0 = A.parts > 1 ? part : nullptr;
+    A.part1 = A.parts > 1 ? part + A.parts * A.part_rows * D : nullptr;
+    rc = D <= 64 ? bw_launch<64, true>(A, m, p.units[1], st) : bw_launch<128, true>(A, m, p.units[1], st);
+    if (!rc && A.parts > 1) rc = bw_sum(A.part0, A.parts, A.part_rows, a->dk, (int)Hk, (int)Sk, (int)D, a->dk_strides, st);
+    if (!rc && A.parts > 1) rc = bw_sum(A.part1, A.parts, A.part_rows, a->dv, (int)Hk, (int)Sk, (int)D, a->dv_strides, st);
+    if (rc) return rc;
+  }
+  if (a->dq) {
+    A.out0 = a->dq;
+    A.out1 = nullptr;
+    for (int i = 0; i < 3; ++i) A.s0[i] = a->dq_strides[i];
+    A.parts = p.parts[0];
+    A.chunk = p.chunk[0];
+    A.part_rows = B * Hq * Sq;
+    A.part0 = A.parts > 1 ? part : nullptr;
+    A.part1 = nullptr;
+    rc = D <= 64 ? bw_launch<64, false>(A, m, p.units[0], st) : bw_launch<128, false>(A, m, p.units[0], st);
+    if (!rc && A.parts > 1) rc = bw_sum(A.part0, A.parts, A.part_rows, a->dq, (int)Hq, (int)Sq, (int)D, a->dq_strides, st);
+  }
+  return rc;
+}
+
+}  // namespace tsb

@@ -411,7 +411,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
       }
       if (!ok) atomicExch(&B.abort_flag, 1);
     }
-  } else {
+  } else if (warp < 8) {
     // ---------------- softmax, a thread per row
     const int half = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -492,57 +492,70 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
         if (*abort_flag || !mbar_wait(&B.s_full[half], tile_no & 1)) { ok = false; break; }
         if (warp_live) {
           tc_fence_after();
-          uint32_t v[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, v[c]);
-          tmem_wait_ld();
+          // Scores come in two halves of 64 columns and the first half is read again after the maximum is
+          // known: all 128 do not fit beside the rest of a thread's 168 registers, and a spill is slow
+          // (224 KB of shared memory leave local memory no L1).
+          uint32_t va[2][32], vb[2][32];
           const int left = lim - key0;  // columns the row may see
-          float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
-          if (part) {
+          auto hide = [&](uint32_t (&v)[2][32], int c0) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int n = min(max(left - 32 * c, 0), 32);
-              const uint32_t vis = kept[c] & (n == 32 ? ~0u : (1u << n) - 1u);
-              kept[c] = vis;
+            for (int c = 0; c < 2; ++c) {
+              const int n = min(max(left - 32 * (c0 + c), 0), 32);
+              const uint32_t vis = kept[c0 + c] & (n == 32 ? ~0u : (1u << n) - 1u);
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[c][i] = (vis >> i) & 1u ? v[c][i] : 0xff800000u;
             }
-          }
+          };
+          float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
+          auto maxes = [&](uint32_t (&v)[2][32]) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            a0 = fmaxf(a0, __uint_as_float(v[0][i]));
-            a1 = fmaxf(a1, __uint_as_float(v[1][i]));
-            a2 = fmaxf(a2, __uint_as_float(v[2][i]));
-            a3 = fmaxf(a3, __uint_as_float(v[3][i]));
-          }
+            for (int i = 0; i < 32; i += 2) {
+              a0 = fmaxf(a0, __uint_as_float(v[0][i]));
+              a1 = fmaxf(a1, __uint_as_float(v[0][i + 1]));
+              a2 = fmaxf(a2, __uint_as_float(v[1][i]));
+              a3 = fmaxf(a3, __uint_as_float(v[1][i + 1]));
+            }
+          };
+          tmem_ld32(t_s, va[0]);
+          tmem_ld32(t_s + 32, va[1]);
+          tmem_wait_ld();
+          tmem_ld32(t_s + 64, vb[0]);
+          tmem_ld32(t_s + 96, vb[1]);
+          if (part) hide(va, 0);
+          maxes(va);
+          tmem_wait_ld();
+          if (part) hide(vb, 2);
+          maxes(vb);
           a0 = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
           const float bmax = a0 == -INFINITY ? a0 : a0 * sl;
           const float mnew = bmax > m + kFwLazy ? bmax : m;
           const float mu = mnew == -INFINITY ? 0.f : mnew;
           const float corr = ex2(m - mu);  // 1 when m stays, 0 before the first key
           float q0 = 0.f, q1 = 0.f, q2 = 0.f, q3 = 0.f;
-          uint32_t pk[2][32];
+          uint32_t pa[32], pb[32];
+          auto probs = [&](uint32_t (&v)[2][32], uint32_t (&pk)[32]) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              float e0 = ex2(fmaf(__uint_as_float(v[c][i]), sl, -mu));
-              float e1 = ex2(fmaf(__uint_as_float(v[c][i + 1]), sl, -mu));
-              float e2 = ex2(fmaf(__uint_as_float(v[c][i + 2]), sl, -mu));
-              float e3 = ex2(fmaf(__uint_as_float(v[c][i + 3]), sl, -mu));
-              if (part && sl == 0.f) {  // -inf * 0 is not a hidden score
-                e0 = (kept[c] >> i) & 1u ? e0 : 0.f;
-                e1 = (kept[c] >> (i + 1)) & 1u ? e1 : 0.f;
-                e2 = (kept[c] >> (i + 2)) & 1u ? e2 : 0.f;
-                e3 = (kept[c] >> (i + 3)) & 1u ? e3 : 0.f;
+              for (int i = 0; i < 32; i += 4) {
+                const float e0 = ex2(fmaf(__uint_as_float(v[c][i]), sl, -mu));
+                const float e1 = ex2(fmaf(__uint_as_float(v[c][i + 1]), sl, -mu));
+                const float e2 = ex2(fmaf(__uint_as_float(v[c][i + 2]), sl, -mu));
+                const float e3 = ex2(fmaf(__uint_as_float(v[c][i + 3]), sl, -mu));
+                q0 += e0;
+                q1 += e1;
+                q2 += e2;
+                q3 += e3;
+                pk[c * 16 + i / 2] = pack_bf16(e0, e1);
+                pk[c * 16 + i / 2 + 1] = pack_bf16(e2, e3);
               }
-              q0 += e0;
-              q1 += e1;
-              q2 += e2;
-              q3 += e3;
-              pk[c >> 1][(c & 1) * 16 + i / 2] = pack_bf16(e0, e1);
-              pk[c >> 1][(c & 1) * 16 + i / 2 + 1] = pack_bf16(e2, e3);
-            }
+          };
+          probs(vb, pb);
+          tmem_ld32(t_s, va[0]);
+          tmem_ld32(t_s + 32, va[1]);
+          tmem_wait_ld();
+          if (part) hide(va, 0);
+          probs(va, pa);
           l = l * corr + ((q0 + q1) + (q2 + q3));
           // s_full of this tile implies the previous P V has completed: O may be rescaled
           if (j > g.k0 && __any_sync(0xffffffffu, mnew != m)) {
@@ -557,8 +570,8 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
             }
           }
           m = mnew;
-          tmem_st32(t_s, pk[0]);
-          tmem_st32(t_s + 32, pk[1]);
+          tmem_st32(t_s, pa);
+          tmem_st32(t_s + 32, pb);
           tmem_wait_st();
         }
         if (half == 0 && !clean) {
@@ -827,7 +840,8 @@ int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, c
   A.pieces = reinterpret_cast<int2*>(w + p.pieces);
   A.out = static_cast<__nv_bfloat16*>(a->out);
   A.lse = a->lse;
-  A.scale_log2 = static_cast<float>(fabs(a->scale) * 1.4426950408889634);
+  // a scale of 0 (or too small for fp32) stays above 0, so that a hidden score of -inf stays -inf
+  A.scale_log2 = fmaxf(static_cast<float>(fabs(a->scale) * 1.4426950408889634), 1e-37f);
   A.q_flip = a->scale < 0 ? 0x80008000u : 0u;
   rc = D <= 64 ? fw_launch<64>(A, m, p.grid, st) : fw_launch<128>(A, m, p.grid, st);
   if (rc) return rc;

@@ -77,5 +77,8 @@ int combine_pieces(const float* part_o, const float* part_lse, int pieces, const
 bool xattn_tc_ok(const trnsparse_attention_args* a, bool prefix);
 size_t xattn_tc_workspace(const trnsparse_attention_args* a, bool prefix);
 int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, cudaStream_t st);
+bool xattn_bwd_tc_ok(const trnsparse_attention_args* a);
+size_t xattn_bwd_tc_workspace(const trnsparse_attention_args* a);
+int xattn_bwd_tc(const trnsparse_attention_args* a, void* ws, cudaStream_t st);
 
 }  // namespace tsb
