@@ -48,6 +48,7 @@ constexpr int kFwThreads = 320;
 constexpr int kFwRows = 256;  // rows of an item, two halves of 128
 constexpr int kFwKeys = 128;
 constexpr float kFwLazy = 8.f;
+constexpr int kFwItemCost = 1;  // in key tiles; see fw_cost
 
 template <int HD>
 struct FwLayout {
@@ -63,9 +64,9 @@ struct FwLayout {
 
 struct FwBars {
   uint64_t full[10], empty[10], q_full[2], s_full[2], p_full[2], o_done[2];
-  // the run of key tiles this CTA takes after its whole items
-  long long count;
-  int side, item, k0;
+  // the run this CTA takes after its whole items, in units of cost, out of `all` over `ctas` CTAs
+  long long begin, count, all;
+  int ctas, side, item, k0;
   uint32_t tmem_slot;
   int abort_flag;
 };
@@ -79,12 +80,10 @@ struct FwSide {
 struct FwArgs {
   FwSide side[2];
   int sides, D, whole;         // whole: items per CTA taken whole (one side only)
-  int slot_rows;               // rows of a slot: min(256, most rows of an item)
-  int64_t rows_all;
-  float* slots;                // [2 G][slot_rows][D], then [2 G][slot_rows] log-sum-exp
-  float* slot_lse;
-  float* direct[2];            // two sides: (O, log-sum-exp) of items one CTA finished, by flat row
-  float* direct_lse[2];
+  // Slots of (O / l, log-sum-exp) as [D / 4][rows][4], so that a warp's 32 rows write whole lines: two per CTA
+  // and, with two sides, one per item that a single CTA finished.
+  float *slots, *slot_lse, *item_slots[2], *item_lse[2];
+  int slot_rows, item_rows[2];  // min(256, rows of an item), the largest and each side's
   int2* pieces;                // first and last CTA of every item of the split part
   __nv_bfloat16* out;
   float* lse;
@@ -92,21 +91,44 @@ struct FwArgs {
   uint32_t q_flip;             // sign bits of a negative scale, applied to Q
 };
 
-__device__ __forceinline__ int fw_tiles(const FwSide& sd, int bi) {
-  return max(1, (side_len(sd.s, bi) + kFwKeys - 1) / kFwKeys);  // no key: one hidden tile
+__device__ __forceinline__ uint4 shfl_xor4(uint4 v, int m) {
+  return make_uint4(__shfl_xor_sync(0xffffffffu, v.x, m), __shfl_xor_sync(0xffffffffu, v.y, m),
+                    __shfl_xor_sync(0xffffffffu, v.z, m), __shfl_xor_sync(0xffffffffu, v.w, m));
 }
+// Lane i of four holds q[0..3]; afterwards q[k] is what lane k held as q[i].
+__device__ __forceinline__ void quad_transpose(uint4 (&q)[4], int i) {
+#pragma unroll
+  for (int m = 1; m <= 2; m <<= 1) {
+    const bool up = i & m;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      if (a & m) continue;
+      // swap q[a | m] of the lower lane with q[a] of the upper lane
+      const uint4 give = up ? q[a] : q[a | m];
+      const uint4 got = shfl_xor4(give, m);
+      if (up) q[a] = got;
+      else q[a | m] = got;
+    }
+  }
+}
+
+__device__ __forceinline__ int fw_tiles(const FwSide& sd, int bi) { return (side_len(sd.s, bi) + kFwKeys - 1) / kFwKeys; }
+// Cost of an item in key tiles: its tiles and, unless it has none, kFwItemCost for its Q, drain and output.
+__device__ __forceinline__ int fw_cost(int tiles) { return tiles > 0 ? tiles + kFwItemCost : 0; }
 
 struct FwSeg {
   int side, item, bi, h, rt, k0, k1, n;
 };
 
-// Walks this CTA's items: whole ones first, then its run of the split part.
+// Walks this CTA's items: whole ones first (also those without keys), then its run of the split part.
 struct FwCursor {
   const FwArgs& A;
-  long long left;  // tiles of the run still to take
+  const FwBars& B;
+  long long left;  // cost of the run still to take
+  long long at;    // where the last item begins, in the split part's cost
   int w, side, item, k;
   __device__ FwCursor(const FwArgs& a, const FwBars& b)
-      : A(a), left(b.count), w(0), side(b.side), item(b.item), k(b.k0) {}
+      : A(a), B(b), left(b.count), at(0), w(0), side(b.side), item(b.item), k(b.k0) {}
   __device__ void decode(FwSeg& g) const {
     const FwSide& sd = A.side[g.side];
     const int per = sd.s.hkv * sd.row_tiles;
@@ -126,52 +148,58 @@ struct FwCursor {
       g.k1 = g.n;
       return true;
     }
-    if (left <= 0) return false;
-    if (item >= A.side[side].items) {
-      ++side;
-      item = 0;
+    while (left > 0) {
+      if (item >= A.side[side].items) {
+        ++side;
+        item = 0;
+      }
+      g.side = side;
+      g.item = item++;
+      decode(g);
+      const int k0 = k;
+      k = 0;
+      if (g.n == 0) continue;
+      at = B.begin + B.count - left - k0;
+      const long long take = min(static_cast<long long>(fw_cost(g.n) - k0), left);
+      g.k0 = k0;
+      g.k1 = static_cast<int>(min(static_cast<long long>(g.n), k0 + take));
+      left -= take;
+      if (g.k0 < g.k1) return true;
     }
-    g.side = side;
-    g.item = item;
-    decode(g);
-    g.k0 = k;
-    g.k1 = static_cast<int>(min(static_cast<long long>(g.n), k + left));
-    left -= g.k1 - g.k0;
-    k = 0;
-    ++item;
-    return true;
+    return false;
   }
+  // CTA of the last tile of an item that begins in this run; call right after next().
+  __device__ int last_cta(const FwSeg& g) const { return static_cast<int>(((at + g.n) * B.ctas - 1) / B.all); }
 };
 
-// Sum of the side's tiles over batch entries [0, nb) times items per entry, and position lookups, by one warp.
+// Sums of the items' costs, and position lookups, by one warp.
 // Lane l holds 8 consecutive entries of every 256.
 struct FwScan {
-  long long total;  // tiles of the side
-  // Tiles before item `i`.
+  // Cost of the items before item `i`.
   static __device__ long long before(const FwSide& sd, int i, int lane) {
     const int per = sd.s.hkv * sd.row_tiles, b0 = i / per;
     long long t = 0;
     if (sd.s.lengths == nullptr) {
-      t = static_cast<long long>(b0) * fw_tiles(sd, 0);
+      t = static_cast<long long>(b0) * fw_cost(fw_tiles(sd, 0));
     } else {
       for (int base = 0; base < b0; base += 256)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int b = base + lane * 8 + e;
-          if (b < b0) t += fw_tiles(sd, b);
+          if (b < b0) t += fw_cost(fw_tiles(sd, b));
         }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     }
     t *= per;
     const int r = i - b0 * per;
-    return r == 0 ? t : t + static_cast<long long>(r) * fw_tiles(sd, b0);
+    return r == 0 ? t : t + static_cast<long long>(r) * fw_cost(fw_tiles(sd, b0));
   }
-  // Item and tile within it at tile position x of the side (x below its total).
+  // Item and place within it at position x of the side (x below its total).
   static __device__ void locate(const FwSide& sd, long long x, int lane, int& item, int& k) {
     const int per = sd.s.hkv * sd.row_tiles;
     if (sd.s.lengths == nullptr) {
-      const int n = fw_tiles(sd, 0);
+      const int n = fw_cost(fw_tiles(sd, 0));
       item = static_cast<int>(x / n);
       k = static_cast<int>(x - static_cast<long long>(item) * n);
       return;
@@ -183,7 +211,7 @@ struct FwScan {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int b = base + lane * 8 + e;
-        n[e] = b < sd.s.nb ? fw_tiles(sd, b) : 0;
+        n[e] = b < sd.s.nb ? fw_cost(fw_tiles(sd, b)) : 0;
         s += n[e];
       }
       long long inc = s;
@@ -250,8 +278,8 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
     tmem_relinquish();
   }
   if (warp == 0) {
-    // this CTA's run: tiles [W c / G, W (c + 1) / G) of the W tiles behind the whole items, G the CTAs that
-    // get any (a piece list has no gaps)
+    // this CTA's run: [W c / G, W (c + 1) / G) of the cost W behind the whole items, G the CTAs that get any (a
+    // piece list has no gaps)
     const int first = A.whole * static_cast<int>(gridDim.x);
     const long long t0 = FwScan::before(A.side[0], A.side[0].items, lane);
     const long long t1 = A.sides > 1 ? FwScan::before(A.side[1], A.side[1].items, lane) : 0;
@@ -267,30 +295,12 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
         x -= t0;
       }
       FwScan::locate(A.side[side], x, lane, item, k);
-      // items that begin in this run: which CTAs hold their pieces
-      if (A.pieces != nullptr) {
-        long long at = lo;
-        int sd = side, it = item, kk = k;
-        while (at < hi) {
-          if (it >= A.side[sd].items) {
-            ++sd;
-            it = 0;
-          }
-          const FwSide& S = A.side[sd];
-          const int n = fw_tiles(S, it / (S.s.hkv * S.row_tiles));
-          if (kk == 0 && lane == 0) {
-            const long long e = at + n - 1;  // its last tile
-            const int index = sd == 0 ? it - first : A.side[0].items + it;
-            A.pieces[index] = make_int2(blockIdx.x, static_cast<int>(((e + 1) * G - 1) / W));
-          }
-          at += n - kk;
-          kk = 0;
-          ++it;
-        }
-      }
     }
     if (lane == 0) {
+      B.begin = lo;
       B.count = hi - lo;
+      B.all = W;
+      B.ctas = static_cast<int>(G);
       B.side = side;
       B.item = item;
       B.k0 = k;
@@ -369,6 +379,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
       while (ok && cur.next(g)) {
         const int halves = static_cast<int64_t>(g.rt) * kFwRows + 128 < side_rows(A.side[g.side].s) ? 2 : 1;
         const int n = g.k1 - g.k0;
+        if (n == 0) continue;
         // first scores
         if (!mbar_wait(&B.full[slot], use & 1)) { ok = false; break; }
         for (int half = 0; half < halves; ++half) {
@@ -450,16 +461,37 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
       mbar_arrive(&B.q_full[half]);
     };
     auto active = [&](const FwSeg& g) {
+      if (g.k0 == g.k1) return false;
       return half == 0 || static_cast<int64_t>(g.rt) * kFwRows + 128 < side_rows(A.side[g.side].s);
     };
 
     FwCursor cur(A, B);
     FwSeg g, gn;
-    bool have = !*abort_flag && cur.next(g);
+    // the next segment; thread 0 notes who holds the pieces of an item that begins here
+    auto advance = [&](FwSeg& x) {
+      const int w = cur.w;
+      if (!cur.next(x)) return false;
+      if (threadIdx.x == 0 && cur.w == w && x.k0 == 0) {
+        const int index = x.side == 0 ? x.item - A.whole * static_cast<int>(gridDim.x) : A.side[0].items + x.item;
+        A.pieces[index] = make_int2(blockIdx.x, cur.last_cta(x));
+      }
+      return true;
+    };
+    bool have = !*abort_flag && advance(g);
     bool ok = true;
     if (have && active(g)) load_q(g);
     while (have && ok) {
-      const bool more = cur.next(gn);
+      const bool more = advance(gn);
+      if (g.k0 == g.k1) {  // a whole item without keys: zeros
+        const XSide& s = A.side[0].s;
+        const int64_t row = static_cast<int64_t>(g.rt) * kFwRows + half * 128 + r;
+        if (row < side_rows(s)) {
+          const XRow x = side_row(s, row);
+          __nv_bfloat16* ob = A.out + o_offset(s, g.bi, g.h, x);
+          for (int d = 0; d < A.D; d += 8) *reinterpret_cast<uint4*>(ob + d) = make_uint4(0u, 0u, 0u, 0u);
+          if (A.lse != nullptr) A.lse[flat_row(s, g.bi, g.h, x)] = -INFINITY;
+        }
+      }
       if (!active(g)) {
         skip(g.k1 - g.k0);
         if (more && active(gn)) load_q(gn);
@@ -492,40 +524,45 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
         if (*abort_flag || !mbar_wait(&B.s_full[half], tile_no & 1)) { ok = false; break; }
         if (warp_live) {
           tc_fence_after();
-          // Scores come in two halves of 64 columns and the first half is read again after the maximum is
-          // known: all 128 do not fit beside the rest of a thread's 168 registers, and a spill is slow
-          // (224 KB of shared memory leave local memory no L1).
-          uint32_t va[2][32], vb[2][32];
+          // Scores come in chunks of 32 columns, and the first two are read again once the maximum is known:
+          // all 128 do not fit beside the rest of a thread's 168 registers, and a spill is slow (224 KB of
+          // shared memory leave local memory no L1). A chunk is in flight while the one before is used.
+          uint32_t v0[32], v1[32], v2[32], v3[32];
           const int left = lim - key0;  // columns the row may see
-          auto hide = [&](uint32_t (&v)[2][32], int c0) {
+          auto hide = [&](uint32_t (&v)[32], int c) {
+            if (part) {
+              const int n = min(max(left - 32 * c, 0), 32);
+              const uint32_t vis = kept[c] & (n == 32 ? ~0u : (1u << n) - 1u);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int n = min(max(left - 32 * (c0 + c), 0), 32);
-              const uint32_t vis = kept[c0 + c] & (n == 32 ? ~0u : (1u << n) - 1u);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[c][i] = (vis >> i) & 1u ? v[c][i] : 0xff800000u;
+              for (int i = 0; i < 32; ++i) v[i] = (vis >> i) & 1u ? v[i] : 0xff800000u;
             }
           };
           float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
-          auto maxes = [&](uint32_t (&v)[2][32]) {
+          auto maxes = [&](uint32_t (&v)[32]) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              a0 = fmaxf(a0, __uint_as_float(v[0][i]));
-              a1 = fmaxf(a1, __uint_as_float(v[0][i + 1]));
-              a2 = fmaxf(a2, __uint_as_float(v[1][i]));
-              a3 = fmaxf(a3, __uint_as_float(v[1][i + 1]));
+            for (int i = 0; i < 32; i += 4) {
+              a0 = fmaxf(a0, __uint_as_float(v[i]));
+              a1 = fmaxf(a1, __uint_as_float(v[i + 1]));
+              a2 = fmaxf(a2, __uint_as_float(v[i + 2]));
+              a3 = fmaxf(a3, __uint_as_float(v[i + 3]));
             }
           };
-          tmem_ld32(t_s, va[0]);
-          tmem_ld32(t_s + 32, va[1]);
-          tmem_wait_ld();
-          tmem_ld32(t_s + 64, vb[0]);
-          tmem_ld32(t_s + 96, vb[1]);
-          if (part) hide(va, 0);
-          maxes(va);
-          tmem_wait_ld();
-          if (part) hide(vb, 2);
-          maxes(vb);
+          tmem_ld32(t_s, v0);
+          tmem_wait_ld32(v0);
+          tmem_ld32(t_s + 32, v1);
+          hide(v0, 0);
+          maxes(v0);
+          tmem_wait_ld32(v1);
+          tmem_ld32(t_s + 64, v2);
+          hide(v1, 1);
+          maxes(v1);
+          tmem_wait_ld32(v2);
+          tmem_ld32(t_s + 96, v3);
+          hide(v2, 2);
+          maxes(v2);
+          tmem_wait_ld32(v3);
+          hide(v3, 3);
+          maxes(v3);
           a0 = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
           const float bmax = a0 == -INFINITY ? a0 : a0 * sl;
           const float mnew = bmax > m + kFwLazy ? bmax : m;
@@ -533,29 +570,31 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
           const float corr = ex2(m - mu);  // 1 when m stays, 0 before the first key
           float q0 = 0.f, q1 = 0.f, q2 = 0.f, q3 = 0.f;
           uint32_t pa[32], pb[32];
-          auto probs = [&](uint32_t (&v)[2][32], uint32_t (&pk)[32]) {
+          auto probs = [&](uint32_t (&v)[32], uint32_t* pk) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                const float e0 = ex2(fmaf(__uint_as_float(v[c][i]), sl, -mu));
-                const float e1 = ex2(fmaf(__uint_as_float(v[c][i + 1]), sl, -mu));
-                const float e2 = ex2(fmaf(__uint_as_float(v[c][i + 2]), sl, -mu));
-                const float e3 = ex2(fmaf(__uint_as_float(v[c][i + 3]), sl, -mu));
-                q0 += e0;
-                q1 += e1;
-                q2 += e2;
-                q3 += e3;
-                pk[c * 16 + i / 2] = pack_bf16(e0, e1);
-                pk[c * 16 + i / 2 + 1] = pack_bf16(e2, e3);
-              }
+            for (int i = 0; i < 32; i += 4) {
+              const float e0 = ex2(fmaf(__uint_as_float(v[i]), sl, -mu));
+              const float e1 = ex2(fmaf(__uint_as_float(v[i + 1]), sl, -mu));
+              const float e2 = ex2(fmaf(__uint_as_float(v[i + 2]), sl, -mu));
+              const float e3 = ex2(fmaf(__uint_as_float(v[i + 3]), sl, -mu));
+              q0 += e0;
+              q1 += e1;
+              q2 += e2;
+              q3 += e3;
+              pk[i / 2] = pack_bf16(e0, e1);
+              pk[i / 2 + 1] = pack_bf16(e2, e3);
+            }
           };
-          probs(vb, pb);
-          tmem_ld32(t_s, va[0]);
-          tmem_ld32(t_s + 32, va[1]);
-          tmem_wait_ld();
-          if (part) hide(va, 0);
-          probs(va, pa);
+          probs(v2, pb);
+          tmem_ld32(t_s, v0);
+          probs(v3, pb + 16);
+          tmem_wait_ld32(v0);
+          tmem_ld32(t_s + 32, v1);
+          hide(v0, 0);
+          probs(v0, pa);
+          tmem_wait_ld32(v1);
+          hide(v1, 1);
+          probs(v1, pa + 16);
           l = l * corr + ((q0 + q1) + (q2 + q3));
           // s_full of this tile implies the previous P V has completed: O may be rescaled
           if (j > g.k0 && __any_sync(0xffffffffu, mnew != m)) {
@@ -602,42 +641,53 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
         const float ls = l == 0.f ? -INFINITY : m + log2f(l);
         const bool all = g.k0 == 0 && g.k1 == g.n;
+        const bool to_slot = !all || A.sides > 1;
         float* po = nullptr;
         __nv_bfloat16* ob = nullptr;
-        if (live) {
-          if (!all) {
-            const int64_t at = (2ll * blockIdx.x + (g.k0 == 0 ? 1 : 0)) * A.slot_rows + half * 128 + r;
-            po = A.slots + at * A.D;
-            A.slot_lse[at] = ls;
+        int slot_stride = 0;
+        if (to_slot) {
+          if (all) {
+            slot_stride = A.item_rows[g.side];
+            po = A.item_slots[g.side] + static_cast<int64_t>(g.item) * slot_stride * A.D;
+            if (live) A.item_lse[g.side][static_cast<int64_t>(g.item) * slot_stride + half * 128 + r] = ls;
           } else {
-            const int64_t fr = flat_row(s, g.bi, g.h, x);
-            if (A.direct[g.side] != nullptr) {
-              po = A.direct[g.side] + fr * A.D;
-              A.direct_lse[g.side][fr] = ls;
-            } else {
-              ob = A.out + o_offset(s, g.bi, g.h, x);
-              if (A.lse != nullptr) A.lse[fr] = ls;
-            }
+            const int64_t slot = 2ll * blockIdx.x + (g.k0 == 0 ? 1 : 0);
+            slot_stride = A.slot_rows;
+            po = A.slots + slot * slot_stride * A.D;
+            if (live) A.slot_lse[slot * slot_stride + half * 128 + r] = ls;
           }
+          po += (half * 128 + r) * 4;
+        } else if (live) {
+          ob = A.out + o_offset(s, g.bi, g.h, x);
+          if (A.lse != nullptr) A.lse[flat_row(s, g.bi, g.h, x)] = ls;
         }
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t o[32];
           tmem_ld32(t_o + c * 32, o);
-          tmem_wait_ld();
+          tmem_wait_ld32(o);
           auto f = [&](int i) { return __uint_as_float(o[i]) * inv; };
-          if (po != nullptr) {
+          if (to_slot) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4)
-              if (c * 32 + i < A.D)
-                *reinterpret_cast<float4*>(po + c * 32 + i) = make_float4(f(i), f(i + 1), f(i + 2), f(i + 3));
-          } else if (ob != nullptr) {
+              if (live && c * 32 + i < A.D)
+                *reinterpret_cast<float4*>(po + static_cast<int64_t>(c * 8 + i / 4) * slot_stride * 4) =
+                    make_float4(f(i), f(i + 1), f(i + 2), f(i + 3));
+          } else {
+            // four lanes exchange their four 16-byte pieces, so that a store writes 64 contiguous bytes of a row
+            uint4 q[4];
 #pragma unroll
-            for (int i = 0; i < 32; i += 8)
-              if (c * 32 + i < A.D)
-                *reinterpret_cast<uint4*>(ob + c * 32 + i) =
-                    make_uint4(pack_bf16(f(i), f(i + 1)), pack_bf16(f(i + 2), f(i + 3)), pack_bf16(f(i + 4), f(i + 5)),
-                               pack_bf16(f(i + 6), f(i + 7)));
+            for (int i = 0; i < 4; ++i)
+              q[i] = make_uint4(pack_bf16(f(8 * i), f(8 * i + 1)), pack_bf16(f(8 * i + 2), f(8 * i + 3)),
+                                pack_bf16(f(8 * i + 4), f(8 * i + 5)), pack_bf16(f(8 * i + 6), f(8 * i + 7)));
+            quad_transpose(q, lane & 3);
+            const int d = c * 32 + (lane & 3) * 8;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              __nv_bfloat16* row = reinterpret_cast<__nv_bfloat16*>(
+                  __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ob), (lane & ~3) + k));
+              if (row != nullptr && d < A.D) *reinterpret_cast<uint4*>(row + d) = q[k];
+            }
           }
         }
       }
@@ -656,83 +706,57 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
   }
 }
 
-// Joins the pieces of every row of the split part. One side: block (item, 8 rows), items that one CTA
-// finished are done already. Two sides: block = 8 output rows, each with a prefix and an own part.
+// Joins the pieces of every row of the split part: a thread per (row, 4 elements), rows fastest, as the slots
+// are laid out. One side: blocks walk its split items (those that one CTA finished are done). Two sides: blocks
+// walk the own side's items, whose rows r of sequence b are rows b G T + r of the prefix's item of that key head.
 __global__ void __launch_bounds__(256) xattn_join_kernel(const __grid_constant__ FwArgs A, int G) {
   grid_dep_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int64_t fr;
-  int bi, h;
-  XRow x;
-  float mx = -INFINITY;
-  float den = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  auto add = [&](const float* po, float ls) {
-    if (ls == -INFINITY) return;
-    if (ls > mx) {
-      const float c = exp2f(mx - ls);
-      den *= c;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] *= c;
-      mx = ls;
+  const FwSide& S = A.side[A.sides - 1];
+  const int item = blockIdx.x + A.whole * G, per = S.s.hkv * S.row_tiles;
+  const int bi = item / per, rem = item - bi * per, h = rem / S.row_tiles, rt = rem - h * S.row_tiles;
+  const int64_t R = side_rows(S.s), row0 = static_cast<int64_t>(rt) * kFwRows;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kFwRows), R - row0));
+  const int index = A.sides > 1 ? A.side[0].items + static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x);
+  const int n = fw_tiles(S, bi);
+  const int2 p = n > 0 ? A.pieces[index] : make_int2(0, -1);
+  if (A.sides == 1 && n > 0 && p.x == p.y) return;
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * (A.D / 4); i += gridDim.y * 256) {
+    const int c4 = i / rows, r = i - c4 * rows;
+    float mx = -INFINITY, den = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float* slots, const float* lse, int stride, int64_t slot, int at) {
+      const float ls = lse[slot * stride + at];
+      const float4 o = *reinterpret_cast<const float4*>(slots + slot * stride * A.D +
+                                                        (static_cast<int64_t>(c4) * stride + at) * 4);
+      if (ls == -INFINITY) return;
+      const float mn = fmaxf(mx, ls), c = exp2f(mx - mn), w = exp2f(ls - mn);
+      den = den * c + w;
+      acc = make_float4(acc.x * c + w * o.x, acc.y * c + w * o.y, acc.z * c + w * o.z, acc.w * c + w * o.w);
+      mx = mn;
+    };
+    auto add_item = [&](int2 q, int side, int it, int at) {
+      if (A.sides > 1 && q.x == q.y) add(A.item_slots[side], A.item_lse[side], A.item_rows[side], it, at);
+      else
+        for (int c = q.x; c <= q.y; ++c) add(A.slots, A.slot_lse, A.slot_rows, 2ll * c + (c == q.x ? 1 : 0), at);
+    };
+    if (A.sides > 1) {
+      const FwSide& P = A.side[0];
+      const int64_t pr = static_cast<int64_t>(bi) * S.s.G * S.s.T + row0 + r;
+      const int pi = h * P.row_tiles + static_cast<int>(pr / kFwRows);
+      add_item(A.pieces[pi], 0, pi, static_cast<int>(pr % kFwRows));
     }
-    const float w = exp2f(ls - mx);
-    den += w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 32 * i < A.D) acc[i] = fmaf(w, po[lane + 32 * i], acc[i]);
-  };
-  auto add_pieces = [&](int2 p, int in_tile) {
-    for (int c = p.x; c <= p.y; ++c) {
-      const int64_t at = (2ll * c + (c == p.x ? 1 : 0)) * A.slot_rows + in_tile;
-      add(A.slots + at * A.D, A.slot_lse[at]);
-    }
-  };
-  if (A.sides == 1) {
-    const FwSide& S = A.side[0];
-    const int2 p = A.pieces[blockIdx.x];
-    if (p.x == p.y) return;
-    const int item = blockIdx.x + A.whole * G, per = S.s.hkv * S.row_tiles;
-    bi = item / per;
-    const int rem = item - bi * per, in_tile = blockIdx.y * 8 + warp;
-    h = rem / S.row_tiles;
-    const int64_t row = static_cast<int64_t>(rem - h * S.row_tiles) * kFwRows + in_tile;
-    if (row >= side_rows(S.s)) return;
-    x = side_row(S.s, row);
-    fr = flat_row(S.s, bi, h, x);
-    add_pieces(p, in_tile);
-  } else {
-    fr = static_cast<int64_t>(blockIdx.x) * 8 + warp;
-    if (fr >= A.rows_all) return;
-    const XSide& s = A.side[1].s;
-    x.t = static_cast<int>(fr % s.T);
-    const int64_t bh = fr / s.T;
-    const int hq = static_cast<int>(bh % (s.hkv * s.G));
-    bi = static_cast<int>(bh / (s.hkv * s.G));
-    h = hq / s.G;
-    x.g = hq - h * s.G;
-    x.b2 = 0;
-    for (int sd = 0; sd < 2; ++sd) {
-      const FwSide& S = A.side[sd];
-      const int64_t row = ((sd == 0 ? static_cast<int64_t>(bi) * s.G : 0) + x.g) * s.T + x.t;
-      const int rt = static_cast<int>(row / kFwRows);
-      const int item = ((sd == 0 ? 0 : bi) * s.hkv + h) * S.row_tiles + rt;
-      const int2 p = A.pieces[(sd == 0 ? 0 : A.side[0].items) + item];
-      if (p.x == p.y) add(A.direct[sd] + fr * A.D, A.direct_lse[sd][fr]);
-      else add_pieces(p, static_cast<int>(row - static_cast<int64_t>(rt) * kFwRows));
-    }
+    add_item(p, A.sides - 1, item, r);
+    const XRow x = side_row(S.s, row0 + r);
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    __nv_bfloat16* po = A.out + o_offset(S.s, bi, h, x) + c4 * 4;
+    *reinterpret_cast<uint2*>(po) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    if (A.lse != nullptr && c4 == 0) A.lse[flat_row(S.s, bi, h, x)] = den == 0.f ? -INFINITY : mx + log2f(den);
   }
-  const XSide& s = A.side[A.sides - 1].s;
-  __nv_bfloat16* po = A.out + o_offset(s, bi, h, x);
-  const float inv = den == 0.f ? 0.f : 1.f / den;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i < A.D) po[lane + 32 * i] = __float2bfloat16_rn(acc[i] * inv);
-  if (A.lse != nullptr && lane == 0) A.lse[fr] = den == 0.f ? -INFINITY : mx + log2f(den);
 }
 
 struct FwPlan {
   int grid, whole, slot_rows, split_items;
-  size_t slots, slot_lse, direct, direct_lse, pieces, total;  // byte offsets
+  size_t o[3], lse[3], pieces, total;  // byte offsets: the CTAs' slots, each side's item slots
 };
 
 FwPlan fw_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n) {
@@ -750,12 +774,22 @@ FwPlan fw_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n) {
   if (n == 1 && items >= 2ll * p.grid) p.whole = static_cast<int>(items / p.grid - 1);
   p.split_items = static_cast<int>(items - static_cast<int64_t>(p.whole) * p.grid);
   p.slot_rows = static_cast<int>(most < kFwRows ? most : kFwRows);
-  const int64_t D = a->head_dim, slot = 2ll * p.grid * p.slot_rows, rows = a->batch * a->q_heads * a->q_len;
-  p.slots = 0;
-  p.slot_lse = align256(sizeof(float) * slot * D);
-  p.direct = p.slot_lse + align256(sizeof(float) * slot);
-  p.direct_lse = p.direct + (n > 1 ? align256(2 * sizeof(float) * rows * D) : 0);
-  p.pieces = p.direct_lse + (n > 1 ? align256(2 * sizeof(float) * rows) : 0);
+  // slots and their log-sum-exps, then (two sides) each side's item slots
+  int64_t slots = 2ll * p.grid, at = 0;
+  for (int i = 0; i < 3; ++i) {
+    int64_t rows = p.slot_rows;
+    if (i > 0) {
+      if (n < 2) break;
+      const int64_t R = side_rows(s[i - 1]);
+      rows = R < kFwRows ? R : kFwRows;
+      slots = (R + kFwRows - 1) / kFwRows * s[i - 1].nb * s[i - 1].hkv;
+    }
+    p.o[i] = at;
+    at += align256(sizeof(float) * slots * rows * a->head_dim);
+    p.lse[i] = at;
+    at += align256(sizeof(float) * slots * rows);
+  }
+  p.pieces = at;
   p.total = p.pieces + align256(sizeof(int2) * p.split_items);
   return p;
 }
@@ -810,7 +844,7 @@ int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, c
   FwArgs A = {};
   XMap m[4];
   char* w = static_cast<char*>(ws);
-  const int64_t rows = a->batch * a->q_heads * a->q_len, D = a->head_dim;
+  const int64_t D = a->head_dim;
   for (int i = 0; i < n; ++i) {
     FwSide& S = A.side[i];
     S.s = s[i];
@@ -824,19 +858,20 @@ int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, c
     S.mul_kb = m[2 * i].mul_b;
     S.mul_vh = m[2 * i + 1].mul_h;
     S.mul_vb = m[2 * i + 1].mul_b;
-    if (n > 1) {
-      A.direct[i] = reinterpret_cast<float*>(w + p.direct) + i * rows * D;
-      A.direct_lse[i] = reinterpret_cast<float*>(w + p.direct_lse) + i * rows;
-    }
   }
   for (int i = 2 * n; i < 4; ++i) m[i] = m[i - 2];
   A.sides = n;
   A.D = static_cast<int>(D);
   A.whole = p.whole;
   A.slot_rows = p.slot_rows;
-  A.rows_all = rows;
-  A.slots = reinterpret_cast<float*>(w + p.slots);
-  A.slot_lse = reinterpret_cast<float*>(w + p.slot_lse);
+  A.slots = reinterpret_cast<float*>(w + p.o[0]);
+  A.slot_lse = reinterpret_cast<float*>(w + p.lse[0]);
+  for (int i = 0; i < 2; ++i) {
+    A.item_slots[i] = reinterpret_cast<float*>(w + p.o[i + 1]);
+    A.item_lse[i] = reinterpret_cast<float*>(w + p.lse[i + 1]);
+    const int64_t R = i < n ? side_rows(s[i]) : 0;
+    A.item_rows[i] = static_cast<int>(R < kFwRows ? R : kFwRows);
+  }
   A.pieces = reinterpret_cast<int2*>(w + p.pieces);
   A.out = static_cast<__nv_bfloat16*>(a->out);
   A.lse = a->lse;
@@ -845,7 +880,8 @@ int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, c
   A.q_flip = a->scale < 0 ? 0x80008000u : 0u;
   rc = D <= 64 ? fw_launch<64>(A, m, p.grid, st) : fw_launch<128>(A, m, p.grid, st);
   if (rc) return rc;
-  const dim3 grid = n == 1 ? dim3(p.split_items, (p.slot_rows + 7) / 8) : dim3((unsigned)((rows + 7) / 8));
+  const int64_t last = side_rows(s[n - 1]), rows = last < kFwRows ? last : kFwRows;
+  const dim3 grid(n == 1 ? p.split_items : A.side[1].items, static_cast<unsigned>((rows * (D / 4) + 255) / 256));
   cudaError_t e = launch_pdl(xattn_join_kernel, grid, dim3(256), 0, st, A, p.grid);
   if (e != cudaSuccess) return cuda_status(e, "attention (tensor cores): join");
   return debug_sync(st, "attention (tensor cores): join");
