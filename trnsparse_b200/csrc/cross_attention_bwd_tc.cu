@@ -204,72 +204,124 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     }
   } else if (warp == 9) {
     // ---------------- MMA issuer
-    if (lane == 0 && !*abort_flag) {
+    if (warp_all(!*abort_flag)) {
       constexpr uint32_t idesc_s = make_idesc(MmaKind::BF16, 128, 128);
       constexpr uint32_t idesc_a = make_idesc(MmaKind::BF16, 128, HD) | (1u << 16);  // walked tile MN-major
-      const uint32_t f1 = smem_u32(sb + Lay::kF1), f2 = smem_u32(sb + Lay::kF2);
-      auto product = [&](uint32_t d, uint32_t fa, uint32_t xa) {
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-          umma<MmaKind::BF16>(d, smem_desc_sw128(fa + off), smem_desc_sw128(xa + off), idesc_s, kk > 0);
-        }
+      const bool lead = elect_one();
+      // descriptors are formed once and moved by adding to their address field (16-byte units)
+      const uint64_t dk = smem_desc_sw128(smem_u32(sb + Lay::kF1)), dm = smem_desc_sw128_mn(smem_u32(sb + Lay::kF1), 16384);
+      const uint32_t base = static_cast<uint32_t>(dk);
+      constexpr uint32_t kF2 = (Lay::kF2 - Lay::kF1) >> 4, kX1 = (Lay::kX1 - Lay::kF1) >> 4, kX2 = (Lay::kX2 - Lay::kF1) >> 4;
+      auto product = [&](uint32_t d, uint32_t f, uint32_t x, int kk) {
+        const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+        umma<MmaKind::BF16>(d, desc_at(dk, base + f + off), desc_at(dk, base + x + off), idesc_s, kk > 0);
       };
       // acc += A X with A packed in TMEM: columns 64 h .. of half h
-      auto accumulate = [&](uint32_t acc, uint32_t a, uint32_t xa, bool first) {
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_ts_f16(acc, a + (kk >> 2) * 64 + (kk & 3) * 8, smem_desc_sw128_mn(xa + kk * 2048, 16384), idesc_a,
-                      !first || kk > 0);
+      auto accumulate = [&](uint32_t acc, uint32_t a, uint32_t x, int kk, bool add) {
+        umma_ts_f16(acc, a + (kk >> 2) * 64 + (kk & 3) * 8, desc_at(dm, static_cast<uint32_t>(dm) + x + kk * (2048 >> 4)),
+                    idesc_a, add);
       };
-      auto x1_addr = [&](int i) { return smem_u32(sb + Lay::kX1 + (i % Lay::kX1Stages) * Lay::kTile); };
-      auto x2_addr = [&](int i) { return smem_u32(sb + Lay::kX2 + (i % Lay::kX2Stages) * Lay::kX2Stage); };
-      auto wait_x1 = [&](int i) { return mbar_wait(&B.x1_full[i % Lay::kX1Stages], (i / Lay::kX1Stages) & 1); };
-      auto wait_x2 = [&](int i) { return mbar_wait(&B.x2_full[i % Lay::kX2Stages], (i / Lay::kX2Stages) & 1); };
+      // ring positions of the current and the next step
+      int s1 = 0, u1 = 0, s2 = 0, u2 = 0;
+      auto next1 = [&] {
+        if (++s1 == Lay::kX1Stages) {
+          s1 = 0;
+          ++u1;
+        }
+      };
+      auto next2 = [&] {
+        if (++s2 == Lay::kX2Stages) {
+          s2 = 0;
+          ++u2;
+        }
+      };
+      auto x1_at = [&] { return kX1 + s1 * (Lay::kTile >> 4); };
+      auto x2_at = [&] { return kX2 + s2 * (Lay::kX2Stage >> 4); };
+      auto ensure = [&](bool seen, uint64_t* bar, int parity) { return warp_all(seen || mbar_wait(bar, parity & 1)); };
+      constexpr int kK = HD / 16;
       int n = 0, nu = 0;
       bool ok = true;
       for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
         const BwUnit x = bw_unit<COL>(A, u);
         const int steps = x.end - x.beg;
         if (steps <= 0) continue;
-        if (!mbar_wait(&B.f_full, nu & 1) || !wait_x1(n)) { ok = false; break; }
+        if (!ensure(false, &B.f_full, nu) || !ensure(false, &B.x1_full[s1], u1)) { ok = false; break; }
         ++nu;
         tc_fence_after();
-        product(tmem + Lay::kTmemS, f1, x1_addr(n));
-        umma_commit(&B.s_full);
-        if (!wait_x2(n)) { ok = false; break; }
-        product(tmem + Lay::kTmemDP, f2, x2_addr(n));
-        umma_commit(&B.dp_full);
-        if (!COL) umma_commit(&B.x2_empty[n % Lay::kX2Stages]);
-        if (steps == 1) umma_commit(&B.f_empty);
+        if (lead) {
+#pragma unroll
+          for (int kk = 0; kk < kK; ++kk) product(tmem + Lay::kTmemS, 0, x1_at(), kk);
+          umma_commit(&B.s_full);
+        }
+        if (!ensure(false, &B.x2_full[s2], u2)) { ok = false; break; }
+        if (lead) {
+#pragma unroll
+          for (int kk = 0; kk < kK; ++kk) product(tmem + Lay::kTmemDP, kF2, x2_at(), kk);
+          umma_commit(&B.dp_full);
+          if (!COL) umma_commit(&B.x2_empty[s2]);
+          if (steps == 1) umma_commit(&B.f_empty);
+        }
+        // s1, s2: this step's tiles. Barriers are looked at before the last MMA of a burst and waited for only if
+        // they were not complete then (cross_attention_tc.cu).
+        bool p_seen = false;
         for (int j = 0; j < steps; ++j, ++n) {
           const bool more = j + 1 < steps;
-          if (*abort_flag || !mbar_wait(&B.p_full, n & 1)) { ok = false; break; }
+          const uint32_t x1_now = x1_at(), x2_now = x2_at();
+          const int e1 = s1, e2 = s2;
+          next1();
+          next2();
+          if (!ensure(p_seen, &B.p_full, n)) { ok = false; break; }
           tc_fence_after();
-          if (COL) accumulate(tmem + Lay::kTmemAcc1, tmem + Lay::kTmemS, x2_addr(n), j == 0);
-          if (more) {
-            if (!wait_x1(n + 1)) { ok = false; break; }
-            product(tmem + Lay::kTmemS, f1, x1_addr(n + 1));
-            umma_commit(&B.s_full);
+          bool x1_seen = !more, ds_seen = false, x2_seen = !more;
+          if (COL) {
+#pragma unroll
+            for (int kk = 0; kk < 7; ++kk)
+              if (lead) accumulate(tmem + Lay::kTmemAcc1, tmem + Lay::kTmemS, x2_now, kk, j > 0 || kk > 0);
+            if (more) x1_seen = mbar_test_wait(&B.x1_full[s1], u1 & 1);
+            else ds_seen = mbar_test_wait(&B.ds_full, n & 1);
+            if (lead) accumulate(tmem + Lay::kTmemAcc1, tmem + Lay::kTmemS, x2_now, 7, true);
           }
-          if (!mbar_wait(&B.ds_full, n & 1)) { ok = false; break; }
-          tc_fence_after();
-          accumulate(tmem + Lay::kTmemAcc0, tmem + Lay::kTmemDP, x1_addr(n), j == 0);
-          umma_commit(&B.x1_empty[n % Lay::kX1Stages]);
-          // not before ds_full: the pointwise warps read D from the stage until then
-          if (COL) umma_commit(&B.x2_empty[n % Lay::kX2Stages]);
           if (more) {
-            if (!wait_x2(n + 1)) { ok = false; break; }
-            product(tmem + Lay::kTmemDP, f2, x2_addr(n + 1));
-            umma_commit(&B.dp_full);
-            if (!COL) umma_commit(&B.x2_empty[(n + 1) % Lay::kX2Stages]);
-            if (j + 2 == steps) umma_commit(&B.f_empty);  // the last use of the fixed tiles
-          } else {
+            if (!ensure(x1_seen, &B.x1_full[s1], u1)) { ok = false; break; }
+#pragma unroll
+            for (int kk = 0; kk < kK - 1; ++kk)
+              if (lead) product(tmem + Lay::kTmemS, 0, x1_at(), kk);
+            ds_seen = mbar_test_wait(&B.ds_full, n & 1);
+            if (lead) {
+              product(tmem + Lay::kTmemS, 0, x1_at(), kK - 1);
+              umma_commit(&B.s_full);
+            }
+          }
+          if (!ensure(ds_seen, &B.ds_full, n)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 7; ++kk)
+            if (lead) accumulate(tmem + Lay::kTmemAcc0, tmem + Lay::kTmemDP, x1_now, kk, j > 0 || kk > 0);
+          if (more) x2_seen = mbar_test_wait(&B.x2_full[s2], u2 & 1);
+          if (lead) {
+            accumulate(tmem + Lay::kTmemAcc0, tmem + Lay::kTmemDP, x1_now, 7, true);
+            umma_commit(&B.x1_empty[e1]);
+            // not before ds_full: the pointwise warps read D from the stage until then
+            if (COL) umma_commit(&B.x2_empty[e2]);
+          }
+          if (more) {
+            if (!ensure(x2_seen, &B.x2_full[s2], u2)) { ok = false; break; }
+#pragma unroll
+            for (int kk = 0; kk < kK - 1; ++kk)
+              if (lead) product(tmem + Lay::kTmemDP, kF2, x2_at(), kk);
+            p_seen = mbar_test_wait(&B.p_full, (n + 1) & 1);
+            if (lead) {
+              product(tmem + Lay::kTmemDP, kF2, x2_at(), kK - 1);
+              umma_commit(&B.dp_full);
+              if (!COL) umma_commit(&B.x2_empty[s2]);
+              if (j + 2 == steps) umma_commit(&B.f_empty);  // the last use of the fixed tiles
+            }
+          } else if (lead) {
             umma_commit(&B.acc_full);
           }
         }
       }
-      if (!ok) atomicExch(&B.abort_flag, 1);
+      if (!ok && lead) atomicExch(&B.abort_flag, 1);
     }
   } else {
     // ---------------- pointwise part: lane = fixed row, 64 columns a thread
@@ -278,7 +330,7 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     const uint32_t t_s = tmem + Lay::kTmemS + lane_base + half * 64, t_dp = tmem + Lay::kTmemDP + lane_base + half * 64;
     const float sl = A.scale_log2;
     int n = 0, nu = 0;
-    bool ok = !*abort_flag;
+    bool ok = warp_all(!*abort_flag);
     for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
       const BwUnit x = bw_unit<COL>(A, u);
       const int len = bw_len(A, x.b);
@@ -307,8 +359,8 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           }
         }
         const float* st = reinterpret_cast<const float*>(sb + Lay::kX2 + (n % Lay::kX2Stages) * Lay::kX2Stage + Lay::kTile) + half * 64;
-        if (*abort_flag || !mbar_wait(&B.s_full, n & 1)) { ok = false; break; }
-        if (COL && !mbar_wait(&B.x2_full[n % Lay::kX2Stages], (n / Lay::kX2Stages) & 1)) { ok = false; break; }
+        if (!warp_all(!*abort_flag && mbar_wait(&B.s_full, n & 1))) { ok = false; break; }
+        if (COL && !warp_all(mbar_wait(&B.x2_full[n % Lay::kX2Stages], (n / Lay::kX2Stages) & 1))) { ok = false; break; }
         tc_fence_after();
         uint32_t p[2][32];
         tmem_ld32(t_s, p[0]);
@@ -362,7 +414,7 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           tc_fence_before();
           mbar_arrive(&B.p_full);
         }
-        if (!mbar_wait(&B.dp_full, n & 1)) { ok = false; break; }
+        if (!warp_all(mbar_wait(&B.dp_full, n & 1))) { ok = false; break; }
         tc_fence_after();
         uint32_t ds[32];
 #pragma unroll
@@ -399,7 +451,7 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       // ---- accumulators -> global; a unit without steps writes zeros
       const bool worked = x.beg < x.end;
       if (worked) {
-        if (!mbar_wait(&B.acc_full, nu & 1) || *abort_flag) { ok = false; break; }
+        if (!warp_all(mbar_wait(&B.acc_full, nu & 1) && !*abort_flag)) { ok = false; break; }
         ++nu;
         tc_fence_after();
       }

@@ -12,7 +12,7 @@
 //
 // An item is 256 packed rows (see xattn.cuh: query heads of one key head,
 // tokens, and for a shared prefix all sequences) against the keys of one (batch
-// entry, key head). One CTA per SM, 10 warps:
+// entry, key head). One CTA per SM, 11 warps:
 //   warps 0-3 / 4-7  softmax of rows 0-127 / 128-255, a thread per row: reads
 //                    its 128 scores from TMEM, writes P over them as packed
 //                    bf16 (the A operand of the second product), keeps m and l;
@@ -20,6 +20,7 @@
 //   warp 8           TMA producer: K0, V0, K1, V1, ... through one ring of
 //                    tiles; a tile is read by both halves' products, so 64 KB
 //                    of K / V feed 2 x 2 products of 128 x 128 x 128.
+//   warp 10          the list of (item, key tiles) this CTA works through
 //   warp 9           MMA issuer: for each key tile P_A V, next S_A, P_B V,
 //                    next S_B; the tensor cores work on one half while the
 //                    other half's exponentials run.
@@ -44,7 +45,7 @@
 namespace tsb {
 namespace {
 
-constexpr int kFwThreads = 320;
+constexpr int kFwThreads = 352;
 constexpr int kFwRows = 256;  // rows of an item, two halves of 128
 constexpr int kFwKeys = 128;
 constexpr float kFwLazy = 8.f;
@@ -62,18 +63,43 @@ struct FwLayout {
   static constexpr uint32_t kTmemO = 256;  // S / P: [0, 128) and [128, 256); O: [256, +HD) and [384, +HD)
 };
 
+// A run of key tiles of one item; side < 0 ends the list. Made by one warp, read by all roles from a ring in
+// shared memory: the walk's state and divisions stay out of the other warps' registers.
+struct FwSeg {
+  int side, item, bi, h, rt, k0, k1, n, len;
+};
+constexpr int kFwSegs = 4;
+
 struct FwBars {
-  uint64_t full[10], empty[10], q_full[2], s_full[2], p_full[2], o_done[2];
-  // the run this CTA takes after its whole items, in units of cost, out of `all` over `ctas` CTAs
-  long long begin, count, all;
-  int ctas, side, item, k0;
+  uint64_t full[10], empty[10], q_full[2], s_full[2], p_half[2], p_full[2], o_done[2];
+  uint64_t seg_full[kFwSegs], seg_empty[kFwSegs];
+  FwSeg seg[kFwSegs];
   uint32_t tmem_slot;
   int abort_flag;
 };
 
+// Division by a run-time constant: n / d for 0 <= n < 2^31 is the high word of n * mul, shifted by s, with
+// 2^s < d <= 2^(s + 1) and mul = 2^(32 + s) / d rounded up (below 2^32): the rounding adds less than d n to n 2^(32 +
+// s), so less than one part in n to the quotient.
+struct FastDiv {
+  uint32_t d, mul, shift;
+};
+inline FastDiv fast_div(int d) {
+  FastDiv f = {static_cast<uint32_t>(d), 0u, 0u};
+  while ((2u << f.shift) < static_cast<uint32_t>(d)) ++f.shift;
+  if (d > 1) f.mul = static_cast<uint32_t>(((1ull << (32 + f.shift)) + d - 1) / d);
+  return f;
+}
+__device__ __forceinline__ int fdiv(const FastDiv& f, int n) {
+  return f.d == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), f.mul) >> f.shift);
+}
+
+static_assert(sizeof(FwBars) <= 512, "FwLayout::kSmem");
+
 struct FwSide {
   XSide s;
   int row_tiles, items;
+  FastDiv by_T, by_G;
   int mul_kh, mul_kb, mul_vh, mul_vb;
 };
 
@@ -116,19 +142,22 @@ __device__ __forceinline__ int fw_tiles(const FwSide& sd, int bi) { return (side
 // Cost of an item in key tiles: its tiles and, unless it has none, kFwItemCost for its Q, drain and output.
 __device__ __forceinline__ int fw_cost(int tiles) { return tiles > 0 ? tiles + kFwItemCost : 0; }
 
-struct FwSeg {
-  int side, item, bi, h, rt, k0, k1, n;
-};
+__device__ __forceinline__ XRow fw_row(const FwSide& sd, int64_t r) {
+  const int n = static_cast<int>(r), u = fdiv(sd.by_T, n), b2 = fdiv(sd.by_G, u);
+  XRow x;
+  x.t = n - u * sd.s.T;
+  x.g = u - b2 * sd.s.G;
+  x.b2 = b2;
+  return x;
+}
 
-// Walks this CTA's items: whole ones first (also those without keys), then its run of the split part.
+// Walks a CTA's items: whole ones first (also those without keys), then its run [begin, begin + left) of the
+// split part's cost.
 struct FwCursor {
   const FwArgs& A;
-  const FwBars& B;
-  long long left;  // cost of the run still to take
-  long long at;    // where the last item begins, in the split part's cost
+  long long begin, left;
+  long long at;  // where the last item begins
   int w, side, item, k;
-  __device__ FwCursor(const FwArgs& a, const FwBars& b)
-      : A(a), B(b), left(b.count), at(0), w(0), side(b.side), item(b.item), k(b.k0) {}
   __device__ void decode(FwSeg& g) const {
     const FwSide& sd = A.side[g.side];
     const int per = sd.s.hkv * sd.row_tiles;
@@ -136,7 +165,8 @@ struct FwCursor {
     const int r = g.item - g.bi * per;
     g.h = r / sd.row_tiles;
     g.rt = r - g.h * sd.row_tiles;
-    g.n = fw_tiles(sd, g.bi);
+    g.len = side_len(sd.s, g.bi);
+    g.n = (g.len + kFwKeys - 1) / kFwKeys;
   }
   __device__ bool next(FwSeg& g) {
     if (w < A.whole) {
@@ -159,17 +189,16 @@ struct FwCursor {
       const int k0 = k;
       k = 0;
       if (g.n == 0) continue;
-      at = B.begin + B.count - left - k0;
+      at = begin - k0;
       const long long take = min(static_cast<long long>(fw_cost(g.n) - k0), left);
       g.k0 = k0;
       g.k1 = static_cast<int>(min(static_cast<long long>(g.n), k0 + take));
+      begin += take;
       left -= take;
       if (g.k0 < g.k1) return true;
     }
     return false;
   }
-  // CTA of the last tile of an item that begins in this run; call right after next().
-  __device__ int last_cta(const FwSeg& g) const { return static_cast<int>(((at + g.n) * B.ctas - 1) / B.all); }
 };
 
 // Sums of the items' costs, and position lookups, by one warp.
@@ -258,7 +287,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
   FwBars& B = *reinterpret_cast<FwBars*>(sb + Lay::kBar);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 32) {
+  if (threadIdx.x == 0) {
     for (int i = 0; i < Lay::kStages; ++i) {
       mbar_init(&B.full[i], 1);
       mbar_init(&B.empty[i], 1);
@@ -266,8 +295,13 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
     for (int i = 0; i < 2; ++i) {
       mbar_init(&B.q_full[i], 128);
       mbar_init(&B.s_full[i], 1);
+      mbar_init(&B.p_half[i], 128);
       mbar_init(&B.p_full[i], 128);
       mbar_init(&B.o_done[i], 1);
+    }
+    for (int i = 0; i < kFwSegs; ++i) {
+      mbar_init(&B.seg_full[i], 1);
+      mbar_init(&B.seg_empty[i], 10);  // producer, MMA issuer, eight softmax warps
     }
     B.abort_flag = (smem_u32(sb) & 1023u) ? 1 : 0;
     if (B.abort_flag) record_device_error(DEVERR_SELFCHECK_SMEM);
@@ -277,54 +311,74 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
     tmem_alloc(&B.tmem_slot, 512);
     tmem_relinquish();
   }
-  if (warp == 0) {
-    // this CTA's run: [W c / G, W (c + 1) / G) of the cost W behind the whole items, G the CTAs that get any (a
-    // piece list has no gaps)
-    const int first = A.whole * static_cast<int>(gridDim.x);
-    const long long t0 = FwScan::before(A.side[0], A.side[0].items, lane);
-    const long long t1 = A.sides > 1 ? FwScan::before(A.side[1], A.side[1].items, lane) : 0;
-    const long long s0 = first ? FwScan::before(A.side[0], first, lane) : 0;
-    const long long W = t0 + t1 - s0;
-    const long long G = W < gridDim.x ? W : gridDim.x, c = blockIdx.x;
-    const long long lo = c < G ? W * c / G : W, hi = c < G ? W * (c + 1) / G : W;
-    int side = 0, item = 0, k = 0;
-    if (hi > lo) {
-      long long x = s0 + lo;
-      if (x >= t0) {
-        side = 1;
-        x -= t0;
-      }
-      FwScan::locate(A.side[side], x, lane, item, k);
-    }
-    if (lane == 0) {
-      B.begin = lo;
-      B.count = hi - lo;
-      B.all = W;
-      B.ctas = static_cast<int>(G);
-      B.side = side;
-      B.item = item;
-      B.k0 = k;
-    }
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = B.tmem_slot;
   volatile int* abort_flag = &B.abort_flag;
+  // The i-th segment of the list (false: the list was given up). One reader of each consumer then arrives on
+  // seg_empty.
+  auto read_seg = [&](int i, FwSeg& g) {
+    if (!mbar_wait(&B.seg_full[i % kFwSegs], (i / kFwSegs) & 1)) return false;
+    g = B.seg[i % kFwSegs];
+    return true;
+  };
 
-  if (warp == 8) {
+  if (warp == 10) {
+    // ---------------- the list of segments
+    if (!*abort_flag) {
+      // this CTA's run: [W c / G, W (c + 1) / G) of the cost W behind the whole items, G the CTAs that get any (a
+      // piece list has no gaps)
+      const int first = A.whole * static_cast<int>(gridDim.x);
+      const long long t0 = FwScan::before(A.side[0], A.side[0].items, lane);
+      const long long t1 = A.sides > 1 ? FwScan::before(A.side[1], A.side[1].items, lane) : 0;
+      const long long s0 = first ? FwScan::before(A.side[0], first, lane) : 0;
+      const long long W = t0 + t1 - s0;
+      const long long G = W < gridDim.x ? W : gridDim.x, c = blockIdx.x;
+      const long long lo = c < G ? W * c / G : W, hi = c < G ? W * (c + 1) / G : W;
+      FwCursor cur{A, lo, hi - lo, 0, 0, 0, 0, 0};
+      if (hi > lo) {
+        long long x = s0 + lo;
+        if (x >= t0) {
+          cur.side = 1;
+          x -= t0;
+        }
+        FwScan::locate(A.side[cur.side], x, lane, cur.item, cur.k);
+      }
+      if (lane == 0) {
+        FwSeg g;
+        for (int i = 0;; ++i) {
+          const bool whole = cur.w < A.whole, more = cur.next(g);
+          if (!more) g.side = -1;
+          if (i >= kFwSegs && !mbar_wait(&B.seg_empty[i % kFwSegs], (i / kFwSegs - 1) & 1)) {
+            atomicExch(&B.abort_flag, 1);
+            break;
+          }
+          B.seg[i % kFwSegs] = g;
+          mbar_arrive(&B.seg_full[i % kFwSegs]);
+          if (!more || *abort_flag) break;
+          if (!whole && g.k0 == 0)  // an item that begins here: which CTAs hold its pieces
+            A.pieces[g.side == 0 ? g.item - first : A.side[0].items + g.item] =
+                make_int2(blockIdx.x, static_cast<int>(((cur.at + g.n) * G - 1) / W));
+        }
+      }
+    }
+  } else if (warp == 8) {
     // ---------------- TMA producer
     if (lane == 0 && !*abort_flag) {
-      FwCursor cur(A, B);
       FwSeg g;
       int slot = 0, use = 0;
       bool ok = true;
-      while (ok && cur.next(g)) {
+      for (int i = 0; ok; ++i) {
+        if (!read_seg(i, g)) { ok = false; break; }
+        mbar_arrive(&B.seg_empty[i % kFwSegs]);
+        if (g.side < 0) break;
         const FwSide& sd = A.side[g.side];
         const CUtensorMap* tk = g.side ? &tk1 : &tk0;
         const CUtensorMap* tv = g.side ? &tv1 : &tv0;
+        const int kh = g.h * sd.mul_kh, kb = g.bi * sd.mul_kb, vh = g.h * sd.mul_vh, vb = g.bi * sd.mul_vb;
         for (int j = g.k0; ok && j < g.k1; ++j) {
-#pragma unroll
+#pragma unroll 1
           for (int kv = 0; kv < 2; ++kv) {
             if (*abort_flag || (use > 0 && !mbar_wait(&B.empty[slot], (use - 1) & 1))) {
               ok = false;
@@ -333,8 +387,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
             uint8_t* dst = sb + Lay::kRing + slot * Lay::kTile;
             mbar_arrive_expect_tx(&B.full[slot], Lay::kTile);
             for (int c = 0; c < Lay::kChunks; ++c)
-              tma_load_4d(dst + c * 16384, kv ? tv : tk, c * 64, j * kFwKeys, g.h * (kv ? sd.mul_vh : sd.mul_kh),
-                          g.bi * (kv ? sd.mul_vb : sd.mul_kb), &B.full[slot]);
+              tma_load_4d(dst + c * 16384, kv ? tv : tk, c * 64, j * kFwKeys, kv ? vh : kh, kv ? vb : kb, &B.full[slot]);
             if (++slot == Lay::kStages) {
               slot = 0;
               ++use;
@@ -353,82 +406,125 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
     }
   } else if (warp == 9) {
     // ---------------- MMA issuer
-    if (lane == 0 && !*abort_flag) {
+    if (warp_all(!*abort_flag)) {
       constexpr uint32_t idesc_s = make_idesc(MmaKind::BF16, 128, 128);
       constexpr uint32_t idesc_o = make_idesc(MmaKind::BF16, 128, HD) | (1u << 16);  // V is MN-major
-      FwCursor cur(A, B);
+      const bool lead = elect_one();
+      // Descriptors are formed once and moved by adding to their address field (16-byte units). The tensor
+      // cores take the next MMA only a moment before they are through with the last (64 clocks each), so a
+      // barrier is looked at before the last MMA of a burst is issued, and waited for only if it was not
+      // complete then: a wait that is already over would cost more than an MMA each.
+      const uint64_t k_desc = smem_desc_sw128(smem_u32(sb + Lay::kRing));
+      const uint64_t v_desc = smem_desc_sw128_mn(smem_u32(sb + Lay::kRing), 16384);
+      const uint32_t q_lo = static_cast<uint32_t>(smem_desc_sw128(smem_u32(sb + Lay::kQ)));
+      constexpr uint32_t kStep = Lay::kTile >> 4;
       FwSeg g;
       int slot = 0, use = 0;
-      int segs[2] = {0, 0}, tiles[2] = {0, 0};
+      uint32_t q_ph = 0, p_ph = 0;  // phase bit of each half (no arrays: an index would put them in local memory)
       auto advance = [&] {
         if (++slot == Lay::kStages) {
           slot = 0;
           ++use;
         }
       };
-      auto issue_s = [&](int half, int ks) {
-        const uint32_t q = smem_u32(sb + Lay::kQ + half * Lay::kTile), k = smem_u32(sb + Lay::kRing + ks * Lay::kTile);
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-          umma<MmaKind::BF16>(tmem + half * 128, smem_desc_sw128(q + off), smem_desc_sw128(k + off), idesc_s, kk > 0);
-        }
-        umma_commit(&B.s_full[half]);
+      auto ensure = [&](bool seen, uint64_t* bar, int parity) { return warp_all(seen || mbar_wait(bar, parity & 1)); };
+      auto score = [&](int half, int ks, int kk) {
+        const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+        umma<MmaKind::BF16>(tmem + half * 128, desc_at(k_desc, q_lo + half * kStep + off),
+                            desc_at(k_desc, static_cast<uint32_t>(k_desc) + ks * kStep + off), idesc_s, kk > 0);
       };
       bool ok = true;
-      while (ok && cur.next(g)) {
-        const int halves = static_cast<int64_t>(g.rt) * kFwRows + 128 < side_rows(A.side[g.side].s) ? 2 : 1;
+      for (int i = 0; ok; ++i) {
+        if (!warp_all(read_seg(i, g))) { ok = false; break; }
+        if (lead) mbar_arrive(&B.seg_empty[i % kFwSegs]);
+        if (g.side < 0) break;
         const int n = g.k1 - g.k0;
         if (n == 0) continue;
+        const int halves = static_cast<int64_t>(g.rt) * kFwRows + 128 < side_rows(A.side[g.side].s) ? 2 : 1;
         // first scores
-        if (!mbar_wait(&B.full[slot], use & 1)) { ok = false; break; }
+        if (!ensure(false, &B.full[slot], use)) { ok = false; break; }
         for (int half = 0; half < halves; ++half) {
-          if (!mbar_wait(&B.q_full[half], segs[half] & 1)) { ok = false; break; }
-          ++segs[half];
+          if (!ensure(false, &B.q_full[half], q_ph >> half)) { ok = false; break; }
+          q_ph ^= 1u << half;
           tc_fence_after();
-          issue_s(half, slot);
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk)
+            if (lead) score(half, slot, kk);
+          if (lead) umma_commit(&B.s_full[half]);
         }
         if (!ok) break;
-        umma_commit(&B.empty[slot]);
+        if (lead) umma_commit(&B.empty[slot]);
         advance();
+        bool v_seen = false, p_seen = false;
         for (int j = 0; ok && j < n; ++j) {
           const int vs = slot, vu = use;
           advance();
-          const int ks = slot, ku = use;
-          if (*abort_flag || !mbar_wait(&B.full[vs], vu & 1)) { ok = false; break; }
+          const bool more = j + 1 < n;
+          if (!ensure(v_seen, &B.full[vs], vu)) { ok = false; break; }
+          const uint32_t v_lo = static_cast<uint32_t>(v_desc) + vs * kStep;
+          bool k_seen = !more;
           for (int half = 0; half < halves; ++half) {
-            if (!mbar_wait(&B.p_full[half], tiles[half] & 1)) { ok = false; break; }
-            ++tiles[half];
+            // P is packed at the start of its own 64 score columns; the last 64 keys come first
+            auto pv = [&](int kk, bool add) {
+              umma_ts_f16(tmem + Lay::kTmemO + half * 128, tmem + half * 128 + (kk >> 2) * 64 + (kk & 3) * 8,
+                          desc_at(v_desc, v_lo + kk * (2048 >> 4)), idesc_o, add);
+            };
+            const int ph = (p_ph >> half) & 1;
+            if (!ensure(p_seen, &B.p_half[half], ph)) { ok = false; break; }
             tc_fence_after();
-            const uint32_t v = smem_u32(sb + Lay::kRing + vs * Lay::kTile);
+            if (lead) {
+              pv(4, j > 0);
+              pv(5, true);
+              pv(6, true);
+            }
+            bool f_seen = mbar_test_wait(&B.p_full[half], ph);
+            if (!k_seen) k_seen = mbar_test_wait(&B.full[slot], use & 1);
+            if (lead) pv(7, true);
+            if (!ensure(f_seen, &B.p_full[half], ph)) { ok = false; break; }
+            p_ph ^= 1u << half;
+            tc_fence_after();
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              umma_ts_f16(tmem + Lay::kTmemO + half * 128, tmem + half * 128 + kk * 8,
-                          smem_desc_sw128_mn(v + kk * 2048, 16384), idesc_o, j > 0 || kk > 0);
-            if (j + 1 < n) {
-              if (half == 0 && !mbar_wait(&B.full[ks], ku & 1)) { ok = false; break; }
-              issue_s(half, ks);
+            for (int kk = 0; kk < 4; ++kk)
+              if (lead) pv(kk, true);
+            const int nh = half + 1 < halves ? half + 1 : 0;  // whose P comes next
+            if (more) {
+              if (!ensure(k_seen, &B.full[slot], use)) { ok = false; break; }
+              k_seen = true;
+#pragma unroll
+              for (int kk = 0; kk < HD / 16 - 1; ++kk)
+                if (lead) score(half, slot, kk);
+              p_seen = mbar_test_wait(&B.p_half[nh], (p_ph >> nh) & 1);
+              if (nh == 0) {
+                const int ns = slot + 1 == Lay::kStages ? 0 : slot + 1;
+                v_seen = mbar_test_wait(&B.full[ns], (ns == 0 ? use + 1 : use) & 1);
+              }
+              if (lead) {
+                score(half, slot, HD / 16 - 1);
+                umma_commit(&B.s_full[half]);
+              }
             } else {
-              umma_commit(&B.o_done[half]);
+              if (lead) umma_commit(&B.o_done[half]);
+              p_seen = nh > 0 && mbar_test_wait(&B.p_half[nh], (p_ph >> nh) & 1);
             }
           }
           if (!ok) break;
-          umma_commit(&B.empty[vs]);
-          if (j + 1 < n) {
-            umma_commit(&B.empty[ks]);
+          if (lead) umma_commit(&B.empty[vs]);
+          if (more) {
+            if (lead) umma_commit(&B.empty[slot]);
             advance();
           }
         }
       }
-      if (!ok) atomicExch(&B.abort_flag, 1);
+      if (!ok && lead) atomicExch(&B.abort_flag, 1);
     }
-  } else if (warp < 8) {
+  } else {
     // ---------------- softmax, a thread per row
     const int half = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + half * 128 + lane_base, t_o = tmem + Lay::kTmemO + half * 128 + lane_base;
     const float sl = A.scale_log2;
     uint8_t* const q_tile = sb + Lay::kQ + half * Lay::kTile;
+    // a wait that gave up ends the whole warp's work (its lanes vote and exchange below)
     int seg_no = 0, tile_no = 0;
     int v_slot = 1, v_use = 0;  // ring position of the current tile's V
     auto skip = [&](int tiles) {
@@ -436,187 +532,89 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
       v_use = static_cast<int>(p / Lay::kStages);
       v_slot = static_cast<int>(p - static_cast<int64_t>(v_use) * Lay::kStages);
     };
-    // Q rows of an item into the swizzled tile: a warp loads its own 32 rows, HD / 8 lanes a row
+    // Q rows of an item into the swizzled tile: a warp loads its own 32 rows, HD / 8 lanes a row, eight loads
+    // in flight
     auto load_q = [&](const FwSeg& g) {
-      const XSide& s = A.side[g.side].s;
+      const FwSide& sd = A.side[g.side];
+      const XSide& s = sd.s;
       const int64_t R = side_rows(s), row = static_cast<int64_t>(g.rt) * kFwRows + half * 128 + r;
-      const int64_t mine = row < R ? q_offset(s, g.bi, g.h, side_row(s, row)) : -1;
+      const int64_t mine = row < R ? q_offset(s, g.bi, g.h, fw_row(sd, row)) : -1;
       constexpr int kLanes = HD / 8, kPer = 32 / kLanes;
       const int c = lane % kLanes;
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(s.q) + c * 8;
 #pragma unroll
-      for (int i = 0; i < 32 / kPer; ++i) {
-        const int rr = i * kPer + lane / kLanes;
-        const int64_t off = __shfl_sync(0xffffffffu, mine, rr);
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (off >= 0 && c * 8 < A.D)
-          v = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(s.q) + off + c * 8));
-        v.x ^= A.q_flip;
-        v.y ^= A.q_flip;
-        v.z ^= A.q_flip;
-        v.w ^= A.q_flip;
-        const int tr = (warp & 3) * 32 + rr;
-        *reinterpret_cast<uint4*>(q_tile + (c >> 3) * 16384 + tr * 128 + (((c & 7) ^ (tr & 7)) << 4)) = v;
+      for (int i0 = 0; i0 < 32 / kPer; i0 += 8) {
+        uint4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int64_t off = __shfl_sync(0xffffffffu, mine, (i0 + i) * kPer + lane / kLanes);
+          v[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (off >= 0 && c * 8 < A.D) v[i] = __ldg(reinterpret_cast<const uint4*>(q + off));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int tr = (warp & 3) * 32 + (i0 + i) * kPer + lane / kLanes;
+          *reinterpret_cast<uint4*>(q_tile + (c >> 3) * 16384 + tr * 128 + (((c & 7) ^ (tr & 7)) << 4)) =
+              make_uint4(v[i].x ^ A.q_flip, v[i].y ^ A.q_flip, v[i].z ^ A.q_flip, v[i].w ^ A.q_flip);
+        }
       }
       fence_proxy_async_smem();
       mbar_arrive(&B.q_full[half]);
     };
     auto active = [&](const FwSeg& g) {
-      if (g.k0 == g.k1) return false;
+      if (g.side < 0 || g.k0 == g.k1) return false;
       return half == 0 || static_cast<int64_t>(g.rt) * kFwRows + 128 < side_rows(A.side[g.side].s);
     };
-
-    FwCursor cur(A, B);
-    FwSeg g, gn;
-    // the next segment; thread 0 notes who holds the pieces of an item that begins here
-    auto advance = [&](FwSeg& x) {
-      const int w = cur.w;
-      if (!cur.next(x)) return false;
-      if (threadIdx.x == 0 && cur.w == w && x.k0 == 0) {
-        const int index = x.side == 0 ? x.item - A.whole * static_cast<int>(gridDim.x) : A.side[0].items + x.item;
-        A.pieces[index] = make_int2(blockIdx.x, cur.last_cta(x));
-      }
+    int seg_i = 0;
+    auto next_seg = [&](FwSeg& x) {
+      if (!warp_all(read_seg(seg_i, x))) return false;
+      if (lane == 0) mbar_arrive(&B.seg_empty[seg_i % kFwSegs]);
+      ++seg_i;
       return true;
     };
-    bool have = !*abort_flag && advance(g);
-    bool ok = true;
-    if (have && active(g)) load_q(g);
-    while (have && ok) {
-      const bool more = advance(gn);
-      if (g.k0 == g.k1) {  // a whole item without keys: zeros
-        const XSide& s = A.side[0].s;
-        const int64_t row = static_cast<int64_t>(g.rt) * kFwRows + half * 128 + r;
-        if (row < side_rows(s)) {
-          const XRow x = side_row(s, row);
-          __nv_bfloat16* ob = A.out + o_offset(s, g.bi, g.h, x);
-          for (int d = 0; d < A.D; d += 8) *reinterpret_cast<uint4*>(ob + d) = make_uint4(0u, 0u, 0u, 0u);
-          if (A.lse != nullptr) A.lse[flat_row(s, g.bi, g.h, x)] = -INFINITY;
-        }
-      }
+
+    FwSeg g, gn;
+    bool ok = warp_all(!*abort_flag) && next_seg(g);
+    if (ok && active(g)) load_q(g);
+    while (ok && g.side >= 0) {
       if (!active(g)) {
+        if (g.k0 == g.k1) {  // a whole item without keys: zeros
+          const XSide& s = A.side[0].s;
+          const int64_t row = static_cast<int64_t>(g.rt) * kFwRows + half * 128 + r;
+          if (row < side_rows(s)) {
+            const XRow x = fw_row(A.side[0], row);
+            __nv_bfloat16* ob = A.out + o_offset(s, g.bi, g.h, x);
+            for (int d = 0; d < A.D; d += 8) *reinterpret_cast<uint4*>(ob + d) = make_uint4(0u, 0u, 0u, 0u);
+            if (A.lse != nullptr) A.lse[flat_row(s, g.bi, g.h, x)] = -INFINITY;
+          }
+        }
         skip(g.k1 - g.k0);
-        if (more && active(gn)) load_q(gn);
-        have = more;
+        if (!next_seg(gn)) { ok = false; break; }
+        if (active(gn)) load_q(gn);
         g = gn;
         continue;
       }
-      const XSide& s = A.side[g.side].s;
+      const FwSide& sd = A.side[g.side];
+      const XSide& s = sd.s;
       const int64_t R = side_rows(s), row = static_cast<int64_t>(g.rt) * kFwRows + half * 128 + r;
       const bool live = row < R;
-      const XRow x = side_row(s, live ? row : 0);
-      const int len = side_len(s, g.bi);
-      const int lim = live ? row_limit(s, x, len) : 0;
+      const int len = g.len;
+      int lim = 0;
+      if (live) lim = s.causal ? row_limit(s, fw_row(sd, row), len) : len;
       const uint8_t* mask = s.mask ? s.mask + g.bi * s.mask_stride : nullptr;
       const bool warp_live = __any_sync(0xffffffffu, live);
       float m = -INFINITY, l = 0.f;
       for (int j = g.k0; j < g.k1; ++j, ++tile_no) {
         const int key0 = j * kFwKeys;
-        // which keys of the tile count at all; `part`: some are hidden from this warp's rows
-        uint32_t kept[4] = {~0u, ~0u, ~0u, ~0u};
+        // clean: every key of the tile counts; part: some are hidden from a row of this warp
         const bool clean = mask == nullptr && key0 + kFwKeys <= len;
-        if (!clean) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = key0 + 32 * i + lane;
-            kept[i] = __ballot_sync(0xffffffffu, key < len && (mask == nullptr || mask[key] != 0));
-          }
-        }
         const bool part = !clean || __any_sync(0xffffffffu, live && key0 + kFwKeys > lim);
-        if (*abort_flag || !mbar_wait(&B.s_full[half], tile_no & 1)) { ok = false; break; }
-        if (warp_live) {
-          tc_fence_after();
-          // Scores come in chunks of 32 columns, and the first two are read again once the maximum is known:
-          // all 128 do not fit beside the rest of a thread's 168 registers, and a spill is slow (224 KB of
-          // shared memory leave local memory no L1). A chunk is in flight while the one before is used.
-          uint32_t v0[32], v1[32], v2[32], v3[32];
-          const int left = lim - key0;  // columns the row may see
-          auto hide = [&](uint32_t (&v)[32], int c) {
-            if (part) {
-              const int n = min(max(left - 32 * c, 0), 32);
-              const uint32_t vis = kept[c] & (n == 32 ? ~0u : (1u << n) - 1u);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = (vis >> i) & 1u ? v[i] : 0xff800000u;
-            }
-          };
-          float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
-          auto maxes = [&](uint32_t (&v)[32]) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              a0 = fmaxf(a0, __uint_as_float(v[i]));
-              a1 = fmaxf(a1, __uint_as_float(v[i + 1]));
-              a2 = fmaxf(a2, __uint_as_float(v[i + 2]));
-              a3 = fmaxf(a3, __uint_as_float(v[i + 3]));
-            }
-          };
-          tmem_ld32(t_s, v0);
-          tmem_wait_ld32(v0);
-          tmem_ld32(t_s + 32, v1);
-          hide(v0, 0);
-          maxes(v0);
-          tmem_wait_ld32(v1);
-          tmem_ld32(t_s + 64, v2);
-          hide(v1, 1);
-          maxes(v1);
-          tmem_wait_ld32(v2);
-          tmem_ld32(t_s + 96, v3);
-          hide(v2, 2);
-          maxes(v2);
-          tmem_wait_ld32(v3);
-          hide(v3, 3);
-          maxes(v3);
-          a0 = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
-          const float bmax = a0 == -INFINITY ? a0 : a0 * sl;
-          const float mnew = bmax > m + kFwLazy ? bmax : m;
-          const float mu = mnew == -INFINITY ? 0.f : mnew;
-          const float corr = ex2(m - mu);  // 1 when m stays, 0 before the first key
-          float q0 = 0.f, q1 = 0.f, q2 = 0.f, q3 = 0.f;
-          uint32_t pa[32], pb[32];
-          auto probs = [&](uint32_t (&v)[32], uint32_t* pk) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float e0 = ex2(fmaf(__uint_as_float(v[i]), sl, -mu));
-              const float e1 = ex2(fmaf(__uint_as_float(v[i + 1]), sl, -mu));
-              const float e2 = ex2(fmaf(__uint_as_float(v[i + 2]), sl, -mu));
-              const float e3 = ex2(fmaf(__uint_as_float(v[i + 3]), sl, -mu));
-              q0 += e0;
-              q1 += e1;
-              q2 += e2;
-              q3 += e3;
-              pk[i / 2] = pack_bf16(e0, e1);
-              pk[i / 2 + 1] = pack_bf16(e2, e3);
-            }
-          };
-          probs(v2, pb);
-          tmem_ld32(t_s, v0);
-          probs(v3, pb + 16);
-          tmem_wait_ld32(v0);
-          tmem_ld32(t_s + 32, v1);
-          hide(v0, 0);
-          probs(v0, pa);
-          tmem_wait_ld32(v1);
-          hide(v1, 1);
-          probs(v1, pa + 16);
-          l = l * corr + ((q0 + q1) + (q2 + q3));
-          // s_full of this tile implies the previous P V has completed: O may be rescaled
-          if (j > g.k0 && __any_sync(0xffffffffu, mnew != m)) {
-#pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(t_o + c * 32, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-              tmem_st32(t_o + c * 32, o);
-            }
-          }
-          m = mnew;
-          tmem_st32(t_s, pa);
-          tmem_st32(t_s + 32, pb);
-          tmem_wait_st();
-        }
+        if (!warp_all(!*abort_flag && mbar_wait(&B.s_full[half], tile_no & 1))) { ok = false; break; }
+        tc_fence_after();
         if (half == 0 && !clean) {
           // V rows of hidden keys become zeros before any product reads the tile (the second
           // half's P V is issued after the first half's)
-          if (!mbar_wait(&B.full[v_slot], v_use & 1)) { ok = false; break; }
+          if (!warp_all(mbar_wait(&B.full[v_slot], v_use & 1))) { ok = false; break; }
           const int key = key0 + r;
           if (!(key < len && (mask == nullptr || mask[key] != 0))) {
             uint8_t* vr = sb + Lay::kRing + v_slot * Lay::kTile + r * 128;
@@ -627,19 +625,127 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
           }
           fence_proxy_async_smem();
         }
+        if (warp_live) {
+          // Hidden scores become -inf in place, in a loop of its own: the code below stays one, small and
+          // without spills.
+          if (part) {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              const int key = key0 + 32 * c + lane, n = min(max(lim - key0 - 32 * c, 0), 32);
+              uint32_t vis = __ballot_sync(0xffffffffu, key < len && (mask == nullptr || mask[key] != 0));
+              vis &= n == 32 ? ~0u : (1u << n) - 1u;
+              uint32_t v[32];
+              tmem_ld32(t_s + c * 32, v);
+              tmem_wait_ld32(v);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = (vis >> i) & 1u ? v[i] : 0xff800000u;
+              tmem_st32(t_s + c * 32, v);
+            }
+            tmem_wait_st();
+          }
+          // Scores come in chunks of 32 columns, and the first two are read again once the maximum is known:
+          // all 128 do not fit beside the rest of a thread's 168 registers, and a spill is slow (224 KB of
+          // shared memory leave local memory no L1). A chunk is in flight while the one before is used. One in
+          // four exponentials runs on the FMA pipe: the special-function unit alone (16 a clock) needs 2048
+          // clocks for the two halves' tile, as long as the products.
+          uint32_t v0[32], v1[32], v2[32], v3[32];
+          float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
+          auto maxes = [&](uint32_t (&v)[32]) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              a0 = max3_nan(a0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+              a1 = max3_nan(a1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+              a2 = max3_nan(a2, __uint_as_float(v[i + 4]), __uint_as_float(v[i + 5]));
+              a3 = max3_nan(a3, __uint_as_float(v[i + 6]), __uint_as_float(v[i + 7]));
+            }
+          };
+          tmem_ld32(t_s, v0);
+          tmem_wait_ld32(v0);
+          tmem_ld32(t_s + 32, v1);
+          maxes(v0);
+          tmem_wait_ld32(v1);
+          tmem_ld32(t_s + 64, v2);
+          maxes(v1);
+          tmem_wait_ld32(v2);
+          tmem_ld32(t_s + 96, v3);
+          maxes(v2);
+          tmem_wait_ld32(v3);
+          maxes(v3);
+          a0 = max3_nan(max3_nan(a0, a1, a2), a3, a3);
+          const float bmax = a0 == -INFINITY ? a0 : a0 * sl;
+          const float mnew = bmax <= m + kFwLazy ? m : bmax;  // a NaN moves in and stays
+          const float mu = mnew == -INFINITY ? 0.f : mnew;
+          const float corr = ex2(m - mu);  // 1 when m stays, 0 before the first key
+          // s_full of this tile implies the previous P V has completed: O may be rescaled
+          if (j > g.k0 && __any_sync(0xffffffffu, mnew != m)) {
+#pragma unroll 1
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(t_o + c * 16, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_st16(t_o + c * 16, o);
+            }
+          }
+          m = mnew;
+          uint64_t sum_a = pack2(l * corr, 0.f), sum_b = pack2(0.f, 0.f);
+          const uint64_t sl2 = pack2(sl, sl), mu2 = pack2(-mu, -mu);
+          uint32_t pk[32];
+          auto probs = [&](uint32_t (&v)[32], uint32_t* out) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const uint64_t x = fma2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sl2, mu2);
+              float e0, e1;
+              if (i % 8 == 6) {
+                exp2_poly2(x, e0, e1);
+              } else {
+                unpack2(x, e0, e1);
+                e0 = ex2(e0);
+                e1 = ex2(e1);
+              }
+              if (i & 2) sum_b = add2(sum_b, pack2(e0, e1));
+              else sum_a = add2(sum_a, pack2(e0, e1));
+              out[i / 2] = pack_bf16(e0, e1);
+            }
+          };
+          // P of the last 64 keys goes over their scores first, so that its product starts half a tile early
+          probs(v2, pk);
+          tmem_ld32(t_s, v0);
+          probs(v3, pk + 16);
+          tmem_st32(t_s + 64, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&B.p_half[half]);
+          tmem_wait_ld32(v0);
+          tmem_ld32(t_s + 32, v1);
+          probs(v0, pk);
+          tmem_wait_ld32(v1);
+          probs(v1, pk + 16);
+          tmem_st32(t_s, pk);
+          float s0, s1, s2, s3;
+          unpack2(sum_a, s0, s1);
+          unpack2(sum_b, s2, s3);
+          l = (s0 + s1) + (s2 + s3);
+          tmem_wait_st();
+        } else {
+          mbar_arrive(&B.p_half[half]);
+        }
         tc_fence_before();
         mbar_arrive(&B.p_full[half]);
         skip(1);
       }
       if (!ok) break;
       // every score product of this item has run: the next item's Q may take the tile
-      if (more && active(gn)) load_q(gn);
-      if (!mbar_wait(&B.o_done[half], seg_no & 1) || *abort_flag) { ok = false; break; }
+      if (!next_seg(gn)) { ok = false; break; }
+      if (active(gn)) load_q(gn);
+      if (!warp_all(mbar_wait(&B.o_done[half], seg_no & 1) && !*abort_flag)) { ok = false; break; }
       ++seg_no;
       tc_fence_after();
       if (warp_live) {
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        const float ls = l == 0.f ? -INFINITY : m + log2f(l);
+        const float inv = m == -INFINITY ? 0.f : 1.f / l;  // no key: zero
+        const float ls = m == -INFINITY ? -INFINITY : m + log2f(l);
+        const XRow x = fw_row(sd, live ? row : 0);
         const bool all = g.k0 == 0 && g.k1 == g.n;
         const bool to_slot = !all || A.sides > 1;
         float* po = nullptr;
@@ -692,7 +798,6 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
         }
       }
       tc_fence_before();  // O is read before the next item's first P V (ordered by p_full)
-      have = more;
       g = gn;
     }
     if (!ok) atomicExch(&B.abort_flag, 1);
@@ -850,6 +955,8 @@ int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, c
     S.s = s[i];
     S.row_tiles = static_cast<int>((side_rows(s[i]) + kFwRows - 1) / kFwRows);
     S.items = S.row_tiles * s[i].nb * s[i].hkv;
+    S.by_T = fast_div(s[i].T);
+    S.by_G = fast_div(s[i].G);
     rc = make_xmap(&m[2 * i], s[i].k, D, s[i].klen, s[i].hkv, s[i].nb, s[i].k_t, s[i].k_h, s[i].k_b, 128);
     if (rc) return rc;
     rc = make_xmap(&m[2 * i + 1], s[i].v, D, s[i].klen, s[i].hkv, s[i].nb, s[i].v_t, s[i].v_h, s[i].v_b, 128);

@@ -55,6 +55,32 @@ inline int make_xmap(XMap* m, const void* base, int64_t D, int64_t len, int64_t 
   return TRNSPARSE_OK;
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// The MMA warp stays converged: all lanes wait and vote, one elected lane issues. The addresses of its MMAs are
+// then uniform values, which the compiler keeps in uniform registers; one lane walking the loop alone moves them
+// there for every MMA (2340 clocks against 2080 for 32 MMAs of 64 clocks with their waits).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n.reg .pred P;\nelect.sync _|P, 0xffffffff;\nselp.u32 %0, 1, 0, P;\n}\n" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ bool warp_all(bool b) { return __all_sync(0xffffffffu, b) != 0; }
+// A shared-memory descriptor's low word holds the address (16-byte units), which moves; the high word stays.
+__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t lo) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(d) : "r"(lo), "r"(static_cast<uint32_t>(desc >> 32)));
+  return d;
+}
+
 // tcgen05.wait::ld that also orders the loaded registers: nothing that uses them moves above it.
 __device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;\n"
@@ -71,6 +97,55 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Pairs of floats in one 64-bit register: the packed fp32 instructions of sm_100 do two elements an issue slot.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// The larger of three, NaN if any is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x of two elements on the FMA pipe, x <= 120 or so: x = n + f with n the nearest integer (adding 1.5 2^23
+// leaves it in the low mantissa bits), 2^f on [-1/2, 1/2] by a degree-4 minimax polynomial (relative error
+// 2.6e-6, fitted by weighted least squares for this file; P is rounded to bf16 at 2^-9 afterwards), and n added
+// to the exponent. x below -126 gives 0.
+__device__ __forceinline__ void exp2_poly2(uint64_t x2, float& a, float& b) {
+  float xa, xb;
+  unpack2(x2, xa, xb);
+  x2 = pack2(fmaxf(xa, -126.f), fmaxf(xb, -126.f));
+  const float magic = 12582912.f;
+  const uint64_t t = add2(x2, pack2(magic, magic));
+  const uint64_t n = add2(t, pack2(-magic, -magic));
+  const uint64_t f = fma2(n, pack2(-1.f, -1.f), x2);
+  uint64_t p = fma2(f, pack2(0x1.3997d6p-7f, 0x1.3997d6p-7f), pack2(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+  p = fma2(f, p, pack2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+  p = fma2(f, p, pack2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+  p = fma2(f, p, pack2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  float ta, tb, pa, pb;
+  unpack2(t, ta, tb);
+  unpack2(p, pa, pb);
+  a = xa < -126.f ? 0.f : __uint_as_float((__float_as_uint(ta) << 23) + __float_as_uint(pa));
+  b = xb < -126.f ? 0.f : __uint_as_float((__float_as_uint(tb) << 23) + __float_as_uint(pb));
 }
 
 // Strides (batch, head, token) the tensor maps and 16-byte accesses take: multiples of 8 elements, not
