@@ -23,21 +23,13 @@ from .ops import _back, _dev_of
 _DTYPES = (torch.float32, torch.bfloat16)
 
 
-class _on_device:
-    """``torch.cuda.device`` that costs nothing when the device is already current."""
-
-    __slots__ = ("ctx",)
-
-    def __init__(self, dev: torch.device):
-        self.ctx = None if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+def _on_device(dev: torch.device, run) -> None:
+    """``run(stream handle)`` with ``dev`` as the current device."""
+    if dev.index == torch.cuda.current_device():
+        run(torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            run(torch._C._cuda_getCurrentRawStream(dev.index))
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -48,17 +40,18 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _tiles(t: torch.Tensor) -> torch.Tensor:
     """``t`` as the attention kernels load it fastest: unit last stride, and where head_dim allows it rows that
     start on 16 bytes (an operand that does not have them is copied once, which costs less than narrow loads)."""
-    if t.stride(-1) != 1:
-        return t.contiguous()
+    *outer, last = t.stride()
     n = 16 // t.element_size()
-    if t.shape[-1] % n:
-        return t
-    for size, stride in zip(t.shape[:-1], t.stride()):
-        if size > 1 and (stride % n or stride < 0):
-            return t.contiguous()
-    if t.shape[-2] > 1 and t.stride(-2) == 0:
-        return t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    if last == 1:
+        if t.shape[-1] % n:
+            return t
+        bits = 0
+        for size, stride in zip(t.shape, outer):
+            if size > 1:
+                bits |= stride
+        if bits % n == 0 and bits >= 0 and (outer[-1] or t.shape[-2] <= 1):
+            return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    return t.contiguous()
 
 
 def _to(t: torch.Tensor | None, dev: torch.device, dtype: torch.dtype | None = None) -> torch.Tensor | None:
@@ -116,10 +109,9 @@ def _qk_args(xs, outs, dys, weights, dws, positions, inv_freq, eps, interleaved)
 
 
 def _qk_forward(q, k, positions, inv_freq, qw, kw, eps, interleaved):
-    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    outs = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k)]
     a = _qk_args((q, k), outs, None, (qw, kw), None, positions, inv_freq, eps, interleaved)
-    with _on_device(q.device):
-        _lib.call("trnsparse_qk_norm_rope", C.byref(a), _lib.stream_handle(q.device))
+    _on_device(q.device, lambda stream: _lib.call("trnsparse_qk_norm_rope", C.byref(a), stream))
     return outs
 
 
@@ -140,11 +132,13 @@ class _QkNormRopeFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         dws = [torch.empty_like(w) if w is not None and need[2 + i] else None for i, w in enumerate((qw, kw))]
         a = _qk_args((q, k), dxs, dys, (qw, kw), dws, positions, inv_freq, ctx.eps, ctx.interleaved)
-        with _on_device(q.device):
+
+        def run(stream):
             n = _lib.raw("trnsparse_qk_norm_rope_workspace_size")(C.byref(a))
             ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
-            _lib.call("trnsparse_qk_norm_rope_backward", C.byref(a), ws.data_ptr(), ws.numel(),
-                      _lib.stream_handle(q.device))
+            _lib.call("trnsparse_qk_norm_rope_backward", C.byref(a), ws.data_ptr(), ws.numel(), stream)
+
+        _on_device(q.device, run)
         return dxs[0], dxs[1], dws[0], dws[1], None, None, None, None
 
 
@@ -241,10 +235,12 @@ def _like(t: torch.Tensor) -> torch.Tensor:
 
 
 def _run_attention(name, a, dev):
-    with _on_device(dev):
+    def run(stream):
         n = _lib.raw(name + "_workspace_size")(C.byref(a))
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        _lib.call(name, C.byref(a), _lib.ptr(ws), n, _lib.stream_handle(dev))
+        _lib.call(name, C.byref(a), _lib.ptr(ws), n, stream)
+
+    _on_device(dev, run)
 
 
 def _cross_forward(q, k, v, lengths, mask, scale, want_lse):

@@ -597,10 +597,11 @@ template <int HD, bool COL>
 int bw_launch(const BwArgs& A, const XMap (&m)[4], int units, cudaStream_t st) {
   using Lay = BwLayout<HD>;
   auto kern = xattn_bwd_tc_kernel<HD, COL>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kSmem);
-  if (e != cudaSuccess) return cuda_status(e, "cross_attention backward: set smem");
+  static unsigned long long done = 0;  // a bit per device; setting the attribute again is harmless
+  int rc = allow_smem(kern, Lay::kSmem, &done, "cross_attention backward: set smem");
+  if (rc) return rc;
   const int sms = sm_count();
-  e = launch_pdl(kern, dim3(units < sms ? units : sms), dim3(kBwThreads), Lay::kSmem, st, m[0].map, m[1].map,
+  cudaError_t e = launch_pdl(kern, dim3(units < sms ? units : sms), dim3(kBwThreads), Lay::kSmem, st, m[0].map, m[1].map,
                  m[2].map, m[3].map, A, units);
   if (e != cudaSuccess) return cuda_status(e, "cross_attention backward launch");
   return debug_sync(st, COL ? "cross_attention backward: dK, dV" : "cross_attention backward: dQ");

@@ -49,7 +49,7 @@ constexpr int kFwThreads = 352;
 constexpr int kFwRows = 256;  // rows of an item, two halves of 128
 constexpr int kFwKeys = 128;
 constexpr float kFwLazy = 8.f;
-constexpr int kFwItemCost = 1;  // in key tiles; see fw_cost
+constexpr int kFwItemCost = 2;  // in key tiles; see fw_cost
 
 template <int HD>
 struct FwLayout {
@@ -139,7 +139,8 @@ __device__ __forceinline__ void quad_transpose(uint4 (&q)[4], int i) {
 }
 
 __device__ __forceinline__ int fw_tiles(const FwSide& sd, int bi) { return (side_len(sd.s, bi) + kFwKeys - 1) / kFwKeys; }
-// Cost of an item in key tiles: its tiles and, unless it has none, kFwItemCost for its Q, drain and output.
+// Cost of an item in key tiles: its tiles and, unless it has none, kFwItemCost for its Q, drain and output (1, 2, 3
+// measured: 45.4, 43.5, 42.9 us in a decode over 8 ragged sequences, 170, 167, 175 us in prompts of 777 tokens).
 __device__ __forceinline__ int fw_cost(int tiles) { return tiles > 0 ? tiles + kFwItemCost : 0; }
 
 __device__ __forceinline__ XRow fw_row(const FwSide& sd, int64_t r) {
@@ -532,8 +533,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
       v_use = static_cast<int>(p / Lay::kStages);
       v_slot = static_cast<int>(p - static_cast<int64_t>(v_use) * Lay::kStages);
     };
-    // Q rows of an item into the swizzled tile: a warp loads its own 32 rows, HD / 8 lanes a row, eight loads
-    // in flight
+    // Q rows of an item into the swizzled tile, asynchronously: a warp copies its own 32 rows, HD / 8 lanes a row
     auto load_q = [&](const FwSeg& g) {
       const FwSide& sd = A.side[g.side];
       const XSide& s = sd.s;
@@ -541,21 +541,26 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
       const int64_t mine = row < R ? q_offset(s, g.bi, g.h, fw_row(sd, row)) : -1;
       constexpr int kLanes = HD / 8, kPer = 32 / kLanes;
       const int c = lane % kLanes;
-      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(s.q) + c * 8;
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(s.q);
 #pragma unroll
-      for (int i0 = 0; i0 < 32 / kPer; i0 += 8) {
-        uint4 v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int64_t off = __shfl_sync(0xffffffffu, mine, (i0 + i) * kPer + lane / kLanes);
-          v[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (off >= 0 && c * 8 < A.D) v[i] = __ldg(reinterpret_cast<const uint4*>(q + off));
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int tr = (warp & 3) * 32 + (i0 + i) * kPer + lane / kLanes;
-          *reinterpret_cast<uint4*>(q_tile + (c >> 3) * 16384 + tr * 128 + (((c & 7) ^ (tr & 7)) << 4)) =
-              make_uint4(v[i].x ^ A.q_flip, v[i].y ^ A.q_flip, v[i].z ^ A.q_flip, v[i].w ^ A.q_flip);
+      for (int i = 0; i < 32 / kPer; ++i) {
+        const int tr = (warp & 3) * 32 + i * kPer + lane / kLanes;
+        const int64_t off = __shfl_sync(0xffffffffu, mine, i * kPer + lane / kLanes);
+        const bool in = off >= 0 && c * 8 < A.D;
+        cp_async16(q_tile + (c >> 3) * 16384 + tr * 128 + (((c & 7) ^ (tr & 7)) << 4), in ? q + off + c * 8 : q, in);
+      }
+    };
+    auto finish_q = [&] {
+      cp_async_wait_all();
+      if (A.q_flip) {  // a negative scale: flip Q's signs, and scale by its magnitude
+        __syncwarp();
+        constexpr int kLanes = HD / 8, kPer = 32 / kLanes;
+        const int c = lane % kLanes;
+        for (int i = 0; i < 32 / kPer; ++i) {
+          const int tr = (warp & 3) * 32 + i * kPer + lane / kLanes;
+          uint4* p = reinterpret_cast<uint4*>(q_tile + (c >> 3) * 16384 + tr * 128 + (((c & 7) ^ (tr & 7)) << 4));
+          const uint4 v = *p;
+          *p = make_uint4(v.x ^ A.q_flip, v.y ^ A.q_flip, v.z ^ A.q_flip, v.w ^ A.q_flip);
         }
       }
       fence_proxy_async_smem();
@@ -575,7 +580,10 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
 
     FwSeg g, gn;
     bool ok = warp_all(!*abort_flag) && next_seg(g);
-    if (ok && active(g)) load_q(g);
+    if (ok && active(g)) {
+      load_q(g);
+      finish_q();
+    }
     while (ok && g.side >= 0) {
       if (!active(g)) {
         if (g.k0 == g.k1) {  // a whole item without keys: zeros
@@ -590,7 +598,10 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
         }
         skip(g.k1 - g.k0);
         if (!next_seg(gn)) { ok = false; break; }
-        if (active(gn)) load_q(gn);
+        if (active(gn)) {
+          load_q(gn);
+          finish_q();
+        }
         g = gn;
         continue;
       }
@@ -611,6 +622,11 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
         const bool part = !clean || __any_sync(0xffffffffu, live && key0 + kFwKeys > lim);
         if (!warp_all(!*abort_flag && mbar_wait(&B.s_full[half], tile_no & 1))) { ok = false; break; }
         tc_fence_after();
+        if (j + 1 == g.k1) {
+          // every score product of this item has run: the next item's Q takes the tile while the last P is formed
+          if (!next_seg(gn)) { ok = false; break; }
+          if (active(gn)) load_q(gn);
+        }
         if (half == 0 && !clean) {
           // V rows of hidden keys become zeros before any product reads the tile (the second
           // half's P V is issued after the first half's)
@@ -736,9 +752,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
         skip(1);
       }
       if (!ok) break;
-      // every score product of this item has run: the next item's Q may take the tile
-      if (!next_seg(gn)) { ok = false; break; }
-      if (active(gn)) load_q(gn);
+      if (active(gn)) finish_q();
       if (!warp_all(mbar_wait(&B.o_done[half], seg_no & 1) && !*abort_flag)) { ok = false; break; }
       ++seg_no;
       tc_fence_after();
@@ -903,8 +917,9 @@ template <int HD>
 int fw_launch(const FwArgs& A, const XMap (&m)[4], int grid, cudaStream_t st) {
   using Lay = FwLayout<HD>;
   auto kern = xattn_fwd_tc_kernel<HD>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kSmem);
-  if (e != cudaSuccess) return cuda_status(e, "attention (tensor cores): set smem");
+  static unsigned long long done = 0;  // a bit per device; setting the attribute again is harmless
+  int rc = allow_smem(kern, Lay::kSmem, &done, "attention (tensor cores): set smem");
+  if (rc) return rc;
   kern<<<grid, kFwThreads, Lay::kSmem, st>>>(m[0].map, m[1].map, m[2].map, m[3].map, A);
   TSB_CHECK_LAUNCH("attention (tensor cores) launch");
   return debug_sync(st, "attention (tensor cores)");

@@ -148,6 +148,27 @@ __device__ __forceinline__ void exp2_poly2(uint64_t x2, float& a, float& b) {
   b = xb < -126.f ? 0.f : __uint_as_float((__float_as_uint(tb) << 23) + __float_as_uint(pb));
 }
 
+// Asynchronous 16-byte copy global -> shared, zeros when !in (then nothing is read).
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;\n" ::: "memory"); }
+
+// Dynamic shared memory above the default, asked for once per device (`done`: a bit each).
+template <typename K>
+int allow_smem(K kern, int bytes, unsigned long long* done, const char* what) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e, what);
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (__atomic_load_n(done, __ATOMIC_ACQUIRE) & bit) return TRNSPARSE_OK;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return cuda_status(e, what);
+  __atomic_fetch_or(done, bit, __ATOMIC_RELEASE);
+  return TRNSPARSE_OK;
+}
+
 // Strides (batch, head, token) the tensor maps and 16-byte accesses take: multiples of 8 elements, not
 // negative, below 2^39 elements; a dimension of one entry has no stride to look at.
 inline bool strides_ok(const int64_t* s, int64_t nb, int64_t nh, int64_t nt, bool keys) {
