@@ -45,29 +45,27 @@ struct QkArgs {
   const double* freq;
   int64_t tokens, pos_stride;  // tokens = B * S; pos_stride: 0 (one row for the batch) or S's stride
   int S, D, R, pos64, w_bf16, head_chunk;
-  float eps;
+  float eps, inv_d;
 };
 
-__device__ __forceinline__ float cvt_in(float v) { return v; }
-__device__ __forceinline__ float cvt_in(__nv_bfloat16 v) { return __bfloat162float(v); }
-
+// VEC elements as they lie in memory, and as floats.
 template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    v[0] = cvt_in(p[0]);
-  } else if constexpr (sizeof(T) == 4) {
-    static_assert(VEC == 4, "fp32 vectors are 16 bytes");
-    const float4 q = *reinterpret_cast<const float4*>(p);
-    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-  } else {
-    uint32_t w[VEC / 2];
-    if constexpr (VEC == 8) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
-    else *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+struct Raw {
+  uint32_t w[VEC == 1 ? 1 : VEC * sizeof(T) / 4];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void load_raw(const T* p, Raw<T, VEC>& v) {
+  if constexpr (VEC == 1 && sizeof(T) == 2) v.w[0] = static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p)) << 16;
+  else if constexpr (VEC == 1) v.w[0] = __float_as_uint(*reinterpret_cast<const float*>(p));
+  else if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(v.w) = *reinterpret_cast<const uint4*>(p);
+  else *reinterpret_cast<uint2*>(v.w) = *reinterpret_cast<const uint2*>(p);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void to_floats(const Raw<T, VEC>& r, float (&v)[VEC]) {
 #pragma unroll
-    for (int i = 0; i < VEC / 2; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+  for (int i = 0; i < VEC; ++i) {
+    if constexpr (VEC == 1 || sizeof(T) == 4) v[i] = __uint_as_float(r.w[i]);
+    else v[i] = __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
   }
 }
 
@@ -85,8 +83,7 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
       __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
       w[i] = *reinterpret_cast<uint32_t*>(&h);
     }
-    if constexpr (VEC == 8) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(w);
-    else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(w);
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(w);
   }
 }
 
@@ -127,7 +124,7 @@ __device__ __forceinline__ void from_pairs(float (&a)[VEC], float (&b)[VEC]) {
 
 // KU units per lane (VEC == 1 only: up to 128 units on 32 lanes), LPR lanes per token.
 template <typename T, int VEC, int KU, bool INTER, bool BWD>
-__global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs A, int lpr) {
+__global__ void __launch_bounds__(kQkThreads, VEC == 1 ? 1 : BWD ? 3 : 4) qk_norm_rope_kernel(const QkArgs A, int lpr) {
   extern __shared__ float sm_dw[];
   const int which = static_cast<int>(blockIdx.y) < A.t[0].chunks ? 0 : 1;
   const QkTensor& t = A.t[which];
@@ -190,26 +187,46 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs A
         }
       }
     }
-    const T* xt = static_cast<const T*>(t.x) + bi * t.xs[0] + si * t.xs[2];
-    const T* dyt = BWD ? static_cast<const T*>(t.dy) + bi * t.dys[0] + si * t.dys[2] : nullptr;
-    T* ot = static_cast<T*>(t.out) + bi * t.os[0] + si * t.os[2];
-#pragma unroll 2
+    const T* xt = static_cast<const T*>(t.x) + bi * t.xs[0] + h0 * t.xs[1] + si * t.xs[2];
+    const T* dyt = BWD ? static_cast<const T*>(t.dy) + bi * t.dys[0] + h0 * t.dys[1] + si * t.dys[2] : nullptr;
+    T* ot = static_cast<T*>(t.out) + bi * t.os[0] + h0 * t.os[1] + si * t.os[2];
+    // the next head's vectors are in flight while this head's are used
+    Raw<T, VEC> rx[KU][2], rd[BWD ? KU : 1][2];
+    auto fetch = [&] {
+#pragma unroll
+      for (int u = 0; u < KU; ++u)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int o = e ? o2[u] : o1[u];
+          if (live && o >= 0) {
+            load_raw<T, VEC>(xt + o, rx[u][e]);
+            if constexpr (BWD) load_raw<T, VEC>(dyt + o, rd[u][e]);
+          }
+        }
+      xt += t.xs[1];
+      if constexpr (BWD) dyt += t.dys[1];
+    };
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        rx[u][e] = Raw<T, VEC>{};
+        if constexpr (BWD) rd[u][e] = Raw<T, VEC>{};
+      }
+    if (h0 < h1) fetch();
     for (int h = h0; h < h1; ++h) {
       float a[KU][VEC], b[KU][VEC], ga[KU][VEC], gb[KU][VEC];
       float ss = 0.f, gx = 0.f;
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) a[u][i] = b[u][i] = ga[u][i] = gb[u][i] = 0.f;
-        const T* xr = xt + h * t.xs[1];
-        if (live && o1[u] >= 0) load_vec<T, VEC>(xr + o1[u], a[u]);
-        if (live && o2[u] >= 0) load_vec<T, VEC>(xr + o2[u], b[u]);
+        to_floats<T, VEC>(rx[u][0], a[u]);
+        to_floats<T, VEC>(rx[u][1], b[u]);
         if constexpr (BWD) {
-          const T* dr = dyt + h * t.dys[1];
-          if (live && o1[u] >= 0) load_vec<T, VEC>(dr + o1[u], ga[u]);
-          if (live && o2[u] >= 0) load_vec<T, VEC>(dr + o2[u], gb[u]);
+          to_floats<T, VEC>(rd[u][0], ga[u]);
+          to_floats<T, VEC>(rd[u][1], gb[u]);
         }
       }
+      if (h + 1 < h1) fetch();
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
         to_pairs<VEC, INTER>(a[u], b[u]);
@@ -229,9 +246,8 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs A
         ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if constexpr (BWD) gx += __shfl_xor_sync(0xffffffffu, gx, o);
       }
-      const float r = 1.f / sqrtf(ss / static_cast<float>(D) + A.eps);
-      const float mean_gu = BWD ? gx * r / static_cast<float>(D) : 0.f;
-      T* orow = ot + h * t.os[1];
+      const float r = rsqrtf(fmaf(ss, A.inv_d, A.eps));
+      const float mean_gu = BWD ? gx * r * A.inv_d : 0.f;
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
 #pragma unroll
@@ -249,9 +265,10 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs A
           }
         }
         from_pairs<VEC, INTER>(a[u], b[u]);
-        if (live && o1[u] >= 0) store_vec<T, VEC>(orow + o1[u], a[u]);
-        if (live && o2[u] >= 0) store_vec<T, VEC>(orow + o2[u], b[u]);
+        if (live && o1[u] >= 0) store_vec<T, VEC>(ot + o1[u], a[u]);
+        if (live && o2[u] >= 0) store_vec<T, VEC>(ot + o2[u], b[u]);
       }
+      ot += t.os[1];
     }
   }
 
@@ -321,7 +338,9 @@ QkPlan qk_plan(const trnsparse_qk_norm_rope_args* a, bool bwd) {
     }
     return true;
   };
-  p.vec = es == 4 ? (fits(4) ? 4 : 1) : (fits(8) ? 8 : fits(4) ? 4 : 1);
+  // four elements a piece for both types: bf16 pieces of eight need twice the registers (148 in the backward pass,
+  // one CTA an SM: 246 us against 128 at 16384 tokens of 2 x 16 heads of 128)
+  p.vec = fits(4) ? 4 : 1;
   const int units = static_cast<int>((a->head_dim + 2 * p.vec - 1) / (2 * p.vec));
   p.lpr = 1;
   while (p.lpr < units && p.lpr < 32) p.lpr *= 2;
@@ -336,8 +355,13 @@ QkPlan qk_plan(const trnsparse_qk_norm_rope_args* a, bool bwd) {
   };
   while (p.head_chunk > 1 && blocks(p.head_chunk) < 8 * sms) p.head_chunk /= 2;
   for (int i = 0; i < 2; ++i) p.chunks[i] = static_cast<int>((a->heads[i] + p.head_chunk - 1) / p.head_chunk);
-  const int64_t cap = 8ll * sms;
-  p.grid_x = static_cast<int>(tgroups < cap ? tgroups : cap);
+  // Forward: a token group a CTA (up to a bound). Backward: as few CTAs as fill the GPU once, each with the same
+  // number of groups, because every CTA leaves a partial row of dw to be added.
+  const int chunks = p.chunks[0] + p.chunks[1];
+  int64_t cap = bwd ? 3ll * sms / (chunks > 0 ? chunks : 1) : 64ll * sms;
+  if (cap < 1) cap = 1;
+  const int64_t each = (tgroups + cap - 1) / cap;
+  p.grid_x = static_cast<int>((tgroups + each - 1) / each);
   return p;
 }
 
@@ -360,7 +384,6 @@ int qk_dispatch(const QkArgs& A, const QkPlan& p, bool f32, cudaStream_t st) {
     if (p.vec == 4) return qk_launch<float, 4, 1, INTER, BWD>(A, p, st);
     return qk_launch<float, 1, 4, INTER, BWD>(A, p, st);
   }
-  if (p.vec == 8) return qk_launch<__nv_bfloat16, 8, 1, INTER, BWD>(A, p, st);
   if (p.vec == 4) return qk_launch<__nv_bfloat16, 4, 1, INTER, BWD>(A, p, st);
   return qk_launch<__nv_bfloat16, 1, 4, INTER, BWD>(A, p, st);
 }
@@ -428,6 +451,7 @@ int qk_run(const trnsparse_qk_norm_rope_args* a, bool bwd, void* ws, size_t ws_b
   A.w_bf16 = a->weight_dtype == TRNSPARSE_BF16;
   A.head_chunk = p.head_chunk;
   A.eps = static_cast<float>(a->eps);
+  A.inv_d = 1.f / static_cast<float>(a->head_dim);
   const bool f32 = a->dtype == TRNSPARSE_F32;
   if (bwd) rc = a->interleaved ? qk_dispatch<true, true>(A, p, f32, st) : qk_dispatch<false, true>(A, p, f32, st);
   else rc = a->interleaved ? qk_dispatch<true, false>(A, p, f32, st) : qk_dispatch<false, false>(A, p, f32, st);
