@@ -38,16 +38,16 @@ struct BwLayout {
   static constexpr int kChunks = HD / 64;
   static constexpr int kTile = 128 * HD * 2;
   static constexpr int kX1Stages = 3, kX2Stages = 2;
-  static constexpr int kX2Stage = kTile + 1024;  // with the walked rows' log-sum-exp and D
   static constexpr int kF1 = 0, kF2 = kTile, kX1 = 2 * kTile;
   static constexpr int kX2 = kX1 + kX1Stages * kTile;
-  static constexpr int kBar = kX2 + kX2Stages * kX2Stage;
+  static constexpr int kStat = kX2 + kX2Stages * kTile;  // two stages: the walked rows' -log-sum-exp and -D
+  static constexpr int kBar = kStat + 2 * 1024;
   static constexpr int kSmem = kBar + 256;
   static constexpr uint32_t kTmemS = 0, kTmemDP = 128, kTmemAcc0 = 256, kTmemAcc1 = 384;
 };
 
 struct BwBars {
-  uint64_t f_full, f_empty, x1_full[3], x1_empty[3], x2_full[2], x2_empty[2];
+  uint64_t f_full, f_empty, x1_full[3], x1_empty[3], x2_full[2], x2_empty[2], st_full[2], st_empty[2];
   uint64_t s_full, dp_full, p_full, ds_full, acc_full;
   uint32_t tmem_slot;
   int abort_flag;
@@ -57,7 +57,7 @@ struct BwArgs {
   const int* lengths;
   const uint8_t* mask;
   int64_t mask_stride;
-  const float *lse, *delta;  // [batch, q_heads, padded tokens]
+  const float *nlse, *ndelta;  // -log-sum-exp and -D, [batch, q_heads, padded tokens]
   void *out0, *out1;         // dQ, or dK and dV
   int64_t s0[3], s1[3];      // their strides
   float *part0, *part1;      // fp32 parts [parts][rows][D], or null
@@ -111,6 +111,8 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     for (int i = 0; i < 2; ++i) {
       mbar_init(&B.x2_full[i], 1);
       mbar_init(&B.x2_empty[i], 1);
+      mbar_init(&B.st_full[i], 1);
+      mbar_init(&B.st_empty[i], 1);
     }
     mbar_init(&B.s_full, 1);
     mbar_init(&B.dp_full, 1);
@@ -134,8 +136,9 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
   const int padded = A.q_tiles * 128;
 
   if (warp == 8) {
-    // ---------------- producers: lane 0 the fixed tiles and X1, lane 1 X2
-    if (lane < 2 && !*abort_flag) {
+    // ---------------- producers: lane 0 the fixed tiles and X1, lane 1 X2, in columns lane 2 the statistics (rings
+    // of their own: each is released at another time)
+    if (lane < (COL ? 3 : 2) && !*abort_flag) {
       int n = 0, nu = 0;
       bool ok = true;
       for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
@@ -173,19 +176,22 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
             constexpr int w = COL ? 0 : 2;
             for (int c = 0; c < Lay::kChunks; ++c)
               tma_load_4d(dst + c * 16384, COL ? &tq : &tk, c * 64, row, h * A.mul_h[w], x.b * A.mul_b[w], &B.x1_full[st]);
-          } else {
+          } else if (lane == 1) {
             const int st = n % Lay::kX2Stages, use = n / Lay::kX2Stages;
             if (*abort_flag || (use > 0 && !mbar_wait(&B.x2_empty[st], (use - 1) & 1))) { ok = false; break; }
-            uint8_t* dst = sb + Lay::kX2 + st * Lay::kX2Stage;
-            mbar_arrive_expect_tx(&B.x2_full[st], Lay::kTile + (COL ? 1024 : 0));
+            uint8_t* dst = sb + Lay::kX2 + st * Lay::kTile;
+            mbar_arrive_expect_tx(&B.x2_full[st], Lay::kTile);
             constexpr int w = COL ? 1 : 3;
             for (int c = 0; c < Lay::kChunks; ++c)
               tma_load_4d(dst + c * 16384, COL ? &tg : &tv, c * 64, row, h * A.mul_h[w], x.b * A.mul_b[w], &B.x2_full[st]);
-            if (COL) {
-              const int64_t at = (static_cast<int64_t>(x.b) * A.Hq + h) * padded + row;
-              bulk_g2s(dst + Lay::kTile, A.lse + at, 512, &B.x2_full[st]);
-              bulk_g2s(dst + Lay::kTile + 512, A.delta + at, 512, &B.x2_full[st]);
-            }
+          } else {
+            const int st = n & 1, use = n >> 1;
+            if (*abort_flag || (use > 0 && !mbar_wait(&B.st_empty[st], (use - 1) & 1))) { ok = false; break; }
+            uint8_t* dst = sb + Lay::kStat + st * 1024;
+            const int64_t at = (static_cast<int64_t>(x.b) * A.Hq + h) * padded + row;
+            mbar_arrive_expect_tx(&B.st_full[st], 1024);
+            bulk_g2s(dst, A.nlse + at, 512, &B.st_full[st]);
+            bulk_g2s(dst + 512, A.ndelta + at, 512, &B.st_full[st]);
           }
         }
       }
@@ -196,9 +202,11 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           if (nu > 0) mbar_wait(&B.f_full, (nu - 1) & 1);
           for (int i = max(0, n - Lay::kX1Stages); i < n; ++i)
             mbar_wait(&B.x1_full[i % Lay::kX1Stages], (i / Lay::kX1Stages) & 1);
-        } else {
+        } else if (lane == 1) {
           for (int i = max(0, n - Lay::kX2Stages); i < n; ++i)
             mbar_wait(&B.x2_full[i % Lay::kX2Stages], (i / Lay::kX2Stages) & 1);
+        } else {
+          for (int i = max(0, n - 2); i < n; ++i) mbar_wait(&B.st_full[i & 1], (i >> 1) & 1);
         }
       }
     }
@@ -236,7 +244,7 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         }
       };
       auto x1_at = [&] { return kX1 + s1 * (Lay::kTile >> 4); };
-      auto x2_at = [&] { return kX2 + s2 * (Lay::kX2Stage >> 4); };
+      auto x2_at = [&] { return kX2 + s2 * (Lay::kTile >> 4); };
       auto ensure = [&](bool seen, uint64_t* bar, int parity) { return warp_all(seen || mbar_wait(bar, parity & 1)); };
       constexpr int kK = HD / 16;
       int n = 0, nu = 0;
@@ -279,7 +287,10 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
               if (lead) accumulate(tmem + Lay::kTmemAcc1, tmem + Lay::kTmemS, x2_now, kk, j > 0 || kk > 0);
             if (more) x1_seen = mbar_test_wait(&B.x1_full[s1], u1 & 1);
             else ds_seen = mbar_test_wait(&B.ds_full, n & 1);
-            if (lead) accumulate(tmem + Lay::kTmemAcc1, tmem + Lay::kTmemS, x2_now, 7, true);
+            if (lead) {
+              accumulate(tmem + Lay::kTmemAcc1, tmem + Lay::kTmemS, x2_now, 7, true);
+              umma_commit(&B.x2_empty[e2]);
+            }
           }
           if (more) {
             if (!ensure(x1_seen, &B.x1_full[s1], u1)) { ok = false; break; }
@@ -301,8 +312,7 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           if (lead) {
             accumulate(tmem + Lay::kTmemAcc0, tmem + Lay::kTmemDP, x1_now, 7, true);
             umma_commit(&B.x1_empty[e1]);
-            // not before ds_full: the pointwise warps read D from the stage until then
-            if (COL) umma_commit(&B.x2_empty[e2]);
+            if (COL) umma_commit(&B.st_empty[n & 1]);  // ds_full: the pointwise warps are through with them
           }
           if (more) {
             if (!ensure(x2_seen, &B.x2_full[s2], u2)) { ok = false; break; }
@@ -328,7 +338,7 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     const int half = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + Lay::kTmemS + lane_base + half * 64, t_dp = tmem + Lay::kTmemDP + lane_base + half * 64;
-    const float sl = A.scale_log2;
+    const uint64_t sl2 = pack2(A.scale_log2, A.scale_log2);
     int n = 0, nu = 0;
     bool ok = warp_all(!*abort_flag);
     for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
@@ -336,15 +346,16 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       const int len = bw_len(A, x.b);
       const uint8_t* mask = A.mask ? A.mask + x.b * A.mask_stride : nullptr;
       const int fixed = x.tile * 128 + r;
-      float row_lse = 0.f, row_delta = 0.f;
+      uint64_t row_nlse = 0, row_ndelta = 0;
       bool dead = false;  // columns: this key is hidden
       if (COL) {
         dead = fixed >= len || (mask && !mask[fixed]);
       } else {
         const int64_t at = (static_cast<int64_t>(x.b) * A.Hq + x.h) * padded + fixed;
-        row_lse = A.lse[at];
-        row_delta = A.delta[at];
+        row_nlse = pack2(A.nlse[at], A.nlse[at]);
+        row_ndelta = pack2(A.ndelta[at], A.ndelta[at]);
       }
+      const bool any_dead = COL && __any_sync(0xffffffffu, dead);
       for (int s = x.beg; s < x.end; ++s, ++n) {
         uint32_t kept[2] = {~0u, ~0u};
         bool part = false;
@@ -358,91 +369,115 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
             }
           }
         }
-        const float* st = reinterpret_cast<const float*>(sb + Lay::kX2 + (n % Lay::kX2Stages) * Lay::kX2Stage + Lay::kTile) + half * 64;
+        const float* st = reinterpret_cast<const float*>(sb + Lay::kStat + (n & 1) * 1024) + half * 64;
         if (!warp_all(!*abort_flag && mbar_wait(&B.s_full, n & 1))) { ok = false; break; }
-        if (COL && !warp_all(mbar_wait(&B.x2_full[n % Lay::kX2Stages], (n / Lay::kX2Stages) & 1))) { ok = false; break; }
+        if (COL && !warp_all(mbar_wait(&B.st_full[n & 1], (n >> 1) & 1))) { ok = false; break; }
         tc_fence_after();
-        uint32_t p[2][32];
+        uint32_t p[2][32], pk[32];
         tmem_ld32(t_s, p[0]);
         tmem_ld32(t_s + 32, p[1]);
-        tmem_wait_ld();
+        tmem_wait_ld32(p[0]);
+        tmem_wait_ld32(p[1]);
         if (!COL) {
           tc_fence_before();
           mbar_arrive(&B.p_full);  // the score columns may be written again
         }
+        // Packed fp32 arithmetic; one in four exponentials on the FMA pipe (two warps of a scheduler share a
+        // special-function unit that does four a clock).
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            float4 ls = make_float4(row_lse, row_lse, row_lse, row_lse);
-            if (COL) ls = *reinterpret_cast<const float4*>(st + c * 32 + i);
-            float e[4];
-            e[0] = ex2(fmaf(__uint_as_float(p[c][i]), sl, -ls.x));
-            e[1] = ex2(fmaf(__uint_as_float(p[c][i + 1]), sl, -ls.y));
-            e[2] = ex2(fmaf(__uint_as_float(p[c][i + 2]), sl, -ls.z));
-            e[3] = ex2(fmaf(__uint_as_float(p[c][i + 3]), sl, -ls.w));
-#pragma unroll
-            for (int q = 0; q < 4; ++q) p[c][i + q] = __float_as_uint(COL && dead ? 0.f : e[q]);
-          }
-        if (!COL && part) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) p[c][i] = (kept[c] >> i) & 1u ? p[c][i] : 0u;
-          // hidden keys' K rows become zeros before dS K (their scores are read already)
-          if (half == 0) {
-            const int key = s * 128 + r;
-            if (!(key < len && (mask == nullptr || mask[key] != 0))) {
-              uint8_t* kr = sb + Lay::kX1 + (n % Lay::kX1Stages) * Lay::kTile + r * 128;
-#pragma unroll
-              for (int c = 0; c < Lay::kChunks; ++c)
-#pragma unroll
-                for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(kr + c * 16384 + q * 16) = make_uint4(0u, 0u, 0u, 0u);
+            uint64_t l0 = row_nlse, l1 = row_nlse;
+            if (COL) {
+              const ulonglong2 ls = *reinterpret_cast<const ulonglong2*>(st + c * 32 + i);
+              l0 = ls.x;
+              l1 = ls.y;
             }
-            fence_proxy_async_smem();
+            const uint64_t x0 = fma2(pack2(__uint_as_float(p[c][i]), __uint_as_float(p[c][i + 1])), sl2, l0);
+            const uint64_t x1 = fma2(pack2(__uint_as_float(p[c][i + 2]), __uint_as_float(p[c][i + 3])), sl2, l1);
+            float e0, e1, e2, e3;
+            unpack2(x0, e0, e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
+            if (i % 8 == 4) {
+              exp2_poly2(x1, e2, e3);
+            } else {
+              unpack2(x1, e2, e3);
+              e2 = ex2(e2);
+              e3 = ex2(e3);
+            }
+            p[c][i] = __float_as_uint(e0);
+            p[c][i + 1] = __float_as_uint(e1);
+            p[c][i + 2] = __float_as_uint(e2);
+            p[c][i + 3] = __float_as_uint(e3);
+            if (COL) {
+              pk[c * 16 + i / 2] = pack_bf16(e0, e1);
+              pk[c * 16 + i / 2 + 1] = pack_bf16(e2, e3);
+            }
           }
-        }
+        // hidden keys: the packed P and dS become zeros, whatever was computed
+        auto hide = [&](uint32_t (&w)[32]) {
+          if (COL) {
+            if (any_dead)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) w[i] = dead ? 0u : w[i];
+          } else if (part) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const uint32_t k = kept[i >> 4] >> (2 * (i & 15));
+              w[i] &= (k & 1u ? 0xffffu : 0u) | (k & 2u ? 0xffff0000u : 0u);
+            }
+          }
+        };
         if (COL) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; i += 2)
-              pk[c * 16 + i / 2] = pack_bf16(__uint_as_float(p[c][i]), __uint_as_float(p[c][i + 1]));
+          hide(pk);
           tmem_st32(t_s, pk);
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(&B.p_full);
+        } else if (part && half == 0) {
+          // hidden keys' K rows become zeros before dS K (their scores are read already)
+          const int key = s * 128 + r;
+          if (!(key < len && (mask == nullptr || mask[key] != 0))) {
+            uint8_t* kr = sb + Lay::kX1 + (n % Lay::kX1Stages) * Lay::kTile + r * 128;
+#pragma unroll
+            for (int c = 0; c < Lay::kChunks; ++c)
+#pragma unroll
+              for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(kr + c * 16384 + q * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
         }
         if (!warp_all(mbar_wait(&B.dp_full, n & 1))) { ok = false; break; }
         tc_fence_after();
-        uint32_t ds[32];
+        uint32_t dp[2][32];
+        tmem_ld32(t_dp, dp[0]);
+        tmem_wait_ld32(dp[0]);
+        tmem_ld32(t_dp + 32, dp[1]);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t dp[32];
-          tmem_ld32(t_dp + c * 32, dp);
-          tmem_wait_ld();
+          if (c) tmem_wait_ld32(dp[1]);
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            float4 de = make_float4(row_delta, row_delta, row_delta, row_delta);
-            if (COL) de = *reinterpret_cast<const float4*>(st + 128 + c * 32 + i);
-            float t[4];
-            t[0] = __uint_as_float(p[c][i]) * (__uint_as_float(dp[i]) - de.x);
-            t[1] = __uint_as_float(p[c][i + 1]) * (__uint_as_float(dp[i + 1]) - de.y);
-            t[2] = __uint_as_float(p[c][i + 2]) * (__uint_as_float(dp[i + 2]) - de.z);
-            t[3] = __uint_as_float(p[c][i + 3]) * (__uint_as_float(dp[i + 3]) - de.w);
+            uint64_t d0 = row_ndelta, d1 = row_ndelta;
             if (COL) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) t[q] = dead ? 0.f : t[q];
-            } else if (part) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) t[q] = (kept[c] >> (i + q)) & 1u ? t[q] : 0.f;
+              const ulonglong2 de = *reinterpret_cast<const ulonglong2*>(st + 128 + c * 32 + i);
+              d0 = de.x;
+              d1 = de.y;
             }
-            ds[c * 16 + i / 2] = pack_bf16(t[0], t[1]);
-            ds[c * 16 + i / 2 + 1] = pack_bf16(t[2], t[3]);
+            const uint64_t t0 = mul2(pack2(__uint_as_float(p[c][i]), __uint_as_float(p[c][i + 1])),
+                                     add2(pack2(__uint_as_float(dp[c][i]), __uint_as_float(dp[c][i + 1])), d0));
+            const uint64_t t1 = mul2(pack2(__uint_as_float(p[c][i + 2]), __uint_as_float(p[c][i + 3])),
+                                     add2(pack2(__uint_as_float(dp[c][i + 2]), __uint_as_float(dp[c][i + 3])), d1));
+            float e0, e1, e2, e3;
+            unpack2(t0, e0, e1);
+            unpack2(t1, e2, e3);
+            pk[c * 16 + i / 2] = pack_bf16(e0, e1);
+            pk[c * 16 + i / 2 + 1] = pack_bf16(e2, e3);
           }
         }
-        tmem_st32(t_dp, ds);
+        hide(pk);
+        tmem_st32(t_dp, pk);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&B.ds_full);
@@ -504,13 +539,14 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
   }
 }
 
-// D = rowsum(dO o O) and the log-sum-exp, padded to whole 128-row tiles (lse = +inf there: P = 0). 16 lanes a row.
+// -D = -rowsum(dO o O) and the log-sum-exp negated, padded to whole 128-row tiles (-inf there: P = 0). 16 lanes a
+// row. Negated, they enter the packed multiply-adds as they are.
 __global__ void __launch_bounds__(256) xattn_row_sums_kernel(const __nv_bfloat16* __restrict__ dout,
                                                              const __nv_bfloat16* __restrict__ out,
                                                              const float* __restrict__ lse, int64_t rows, int Hq,
                                                              int Sq, int padded, int D, int64_t g_b, int64_t g_h,
                                                              int64_t g_t, int64_t o_b, int64_t o_h, int64_t o_t,
-                                                             float* lse_pad, float* delta) {
+                                                             float* nlse, float* ndelta) {
   grid_dep_launch();
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
   const int c = threadIdx.x & 15;
@@ -532,8 +568,8 @@ __global__ void __launch_bounds__(256) xattn_row_sums_kernel(const __nv_bfloat16
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (in && c == 0) {
-    delta[row] = s;
-    lse_pad[row] = t < Sq ? lse[bh * Sq + t] : INFINITY;
+    ndelta[row] = -s;
+    nlse[row] = t < Sq ? -lse[bh * Sq + t] : -INFINITY;
   }
 }
 
@@ -658,8 +694,8 @@ int xattn_bwd_tc(const trnsparse_attention_args* a, void* ws, cudaStream_t st) {
   A.lengths = a->key_lengths;
   A.mask = a->key_mask;
   A.mask_stride = a->key_mask_stride;
-  A.lse = lse;
-  A.delta = delta;
+  A.nlse = lse;
+  A.ndelta = delta;
   A.B = (int)B;
   A.Hq = (int)Hq;
   A.Hkv = (int)Hk;

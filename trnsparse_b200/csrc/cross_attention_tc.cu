@@ -825,21 +825,24 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
   }
 }
 
-// Joins the pieces of every row of the split part: a thread per (row, 4 elements), rows fastest, as the slots
-// are laid out. One side: blocks walk its split items (those that one CTA finished are done). Two sides: blocks
-// walk the own side's items, whose rows r of sequence b are rows b G T + r of the prefix's item of that key head.
+// Joins the pieces of every row of the split part, 32 rows of an item a block: a thread per (row, 4 elements),
+// rows fastest, as the slots are laid out; the rows then leave through shared memory as whole lines. One side:
+// blocks walk its split items (those that one CTA finished are done). Two sides: blocks walk the own side's items,
+// whose rows r of sequence b are rows b G T + r of the prefix's item of that key head.
 __global__ void __launch_bounds__(256) xattn_join_kernel(const __grid_constant__ FwArgs A, int G) {
+  __shared__ __align__(16) __nv_bfloat16 tile[32][136];
   grid_dep_wait();
   const FwSide& S = A.side[A.sides - 1];
   const int item = blockIdx.x + A.whole * G, per = S.s.hkv * S.row_tiles;
   const int bi = item / per, rem = item - bi * per, h = rem / S.row_tiles, rt = rem - h * S.row_tiles;
-  const int64_t R = side_rows(S.s), row0 = static_cast<int64_t>(rt) * kFwRows;
-  const int rows = static_cast<int>(min(static_cast<int64_t>(kFwRows), R - row0));
+  const int64_t R = side_rows(S.s), row0 = static_cast<int64_t>(rt) * kFwRows + blockIdx.y * 32;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(32), R - row0));
   const int index = A.sides > 1 ? A.side[0].items + static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x);
   const int n = fw_tiles(S, bi);
   const int2 p = n > 0 ? A.pieces[index] : make_int2(0, -1);
-  if (A.sides == 1 && n > 0 && p.x == p.y) return;
-  for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * (A.D / 4); i += gridDim.y * 256) {
+  if (rows <= 0 || (A.sides == 1 && n > 0 && p.x == p.y)) return;
+  const int q4 = A.D / 4;
+  for (int i = threadIdx.x; i < rows * q4; i += 256) {
     const int c4 = i / rows, r = i - c4 * rows;
     float mx = -INFINITY, den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -864,12 +867,19 @@ __global__ void __launch_bounds__(256) xattn_join_kernel(const __grid_constant__
       const int pi = h * P.row_tiles + static_cast<int>(pr / kFwRows);
       add_item(A.pieces[pi], 0, pi, static_cast<int>(pr % kFwRows));
     }
-    add_item(p, A.sides - 1, item, r);
-    const XRow x = side_row(S.s, row0 + r);
+    add_item(p, A.sides - 1, item, blockIdx.y * 32 + r);
     const float inv = den == 0.f ? 0.f : 1.f / den;
-    __nv_bfloat16* po = A.out + o_offset(S.s, bi, h, x) + c4 * 4;
-    *reinterpret_cast<uint2*>(po) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-    if (A.lse != nullptr && c4 == 0) A.lse[flat_row(S.s, bi, h, x)] = den == 0.f ? -INFINITY : mx + log2f(den);
+    *reinterpret_cast<uint2*>(&tile[r][c4 * 4]) =
+        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    if (A.lse != nullptr && c4 == 0)
+      A.lse[flat_row(S.s, bi, h, side_row(S.s, row0 + r))] = den == 0.f ? -INFINITY : mx + log2f(den);
+  }
+  __syncthreads();
+  const int q8 = A.D / 8;
+  for (int i = threadIdx.x; i < rows * q8; i += 256) {
+    const int r = i / q8, c = i - r * q8;
+    *reinterpret_cast<uint4*>(A.out + o_offset(S.s, bi, h, side_row(S.s, row0 + r)) + c * 8) =
+        *reinterpret_cast<const uint4*>(&tile[r][c * 8]);
   }
 }
 
@@ -889,8 +899,10 @@ FwPlan fw_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n) {
     tiles += it * ((s[i].klen + kFwKeys - 1) / kFwKeys);
   }
   p.grid = static_cast<int>(tiles < sms ? (tiles > 0 ? tiles : 1) : sms);
-  // one side: whole items for all but the last one to two rounds
-  if (n == 1 && items >= 2ll * p.grid) p.whole = static_cast<int>(items / p.grid - 1);
+  // One side: whole items for all but the last round (items of one length), or the last one to two rounds, which
+  // then even out what unequal lengths left.
+  const int last = s[0].lengths != nullptr && s[0].nb > 1 ? 1 : 0;
+  if (n == 1 && items >= (1 + last) * static_cast<int64_t>(p.grid)) p.whole = static_cast<int>(items / p.grid - last);
   p.split_items = static_cast<int>(items - static_cast<int64_t>(p.whole) * p.grid);
   p.slot_rows = static_cast<int>(most < kFwRows ? most : kFwRows);
   // slots and their log-sum-exps, then (two sides) each side's item slots
@@ -1003,7 +1015,8 @@ int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, c
   rc = D <= 64 ? fw_launch<64>(A, m, p.grid, st) : fw_launch<128>(A, m, p.grid, st);
   if (rc) return rc;
   const int64_t last = side_rows(s[n - 1]), rows = last < kFwRows ? last : kFwRows;
-  const dim3 grid(n == 1 ? p.split_items : A.side[1].items, static_cast<unsigned>((rows * (D / 4) + 255) / 256));
+  if (n == 1 && p.split_items == 0) return TRNSPARSE_OK;
+  const dim3 grid(n == 1 ? p.split_items : A.side[1].items, static_cast<unsigned>((rows + 31) / 32));
   cudaError_t e = launch_pdl(xattn_join_kernel, grid, dim3(256), 0, st, A, p.grid);
   if (e != cudaSuccess) return cuda_status(e, "attention (tensor cores): join");
   return debug_sync(st, "attention (tensor cores): join");

@@ -125,27 +125,36 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return r;
 }
 
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // 2^x of two elements on the FMA pipe, x <= 120 or so: x = n + f with n the nearest integer (adding 1.5 2^23
 // leaves it in the low mantissa bits), 2^f on [-1/2, 1/2] by a degree-4 minimax polynomial (relative error
 // 2.6e-6, fitted by weighted least squares for this file; P is rounded to bf16 at 2^-9 afterwards), and n added
-// to the exponent. x below -126 gives 0.
+// to the exponent. x below -126 gives 0, NaN gives NaN.
 __device__ __forceinline__ void exp2_poly2(uint64_t x2, float& a, float& b) {
-  float xa, xb;
+  float xa, xb, la, lb;
   unpack2(x2, xa, xb);
-  x2 = pack2(fmaxf(xa, -126.f), fmaxf(xb, -126.f));
+  asm("max.NaN.f32 %0, %1, 0fC2FE0000;\n" : "=f"(la) : "f"(xa));  // -127
+  asm("max.NaN.f32 %0, %1, 0fC2FE0000;\n" : "=f"(lb) : "f"(xb));
+  const uint64_t x = pack2(la, lb);
   const float magic = 12582912.f;
-  const uint64_t t = add2(x2, pack2(magic, magic));
+  const uint64_t t = add2(x, pack2(magic, magic));
   const uint64_t n = add2(t, pack2(-magic, -magic));
-  const uint64_t f = fma2(n, pack2(-1.f, -1.f), x2);
+  const uint64_t f = fma2(n, pack2(-1.f, -1.f), x);
   uint64_t p = fma2(f, pack2(0x1.3997d6p-7f, 0x1.3997d6p-7f), pack2(0x1.ca1440p-5f, 0x1.ca1440p-5f));
   p = fma2(f, p, pack2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
   p = fma2(f, p, pack2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
   p = fma2(f, p, pack2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-  float ta, tb, pa, pb;
+  float ta, tb, pa, pb, za, zb;
   unpack2(t, ta, tb);
   unpack2(p, pa, pb);
-  a = xa < -126.f ? 0.f : __uint_as_float((__float_as_uint(ta) << 23) + __float_as_uint(pa));
-  b = xb < -126.f ? 0.f : __uint_as_float((__float_as_uint(tb) << 23) + __float_as_uint(pb));
+  unpack2(mul2(x, pack2(0.f, 0.f)), za, zb);
+  a = xa >= -126.f ? __uint_as_float((__float_as_uint(ta) << 23) + __float_as_uint(pa)) : za;
+  b = xb >= -126.f ? __uint_as_float((__float_as_uint(tb) << 23) + __float_as_uint(pb)) : zb;
 }
 
 // Asynchronous 16-byte copy global -> shared, zeros when !in (then nothing is read).
