@@ -202,6 +202,34 @@ def test_cross_attention(dtype, B, Hq, Hkv, Sq, Sk, D, kind):
             assert (got[dead] == 0).all()
 
 
+def test_calls_from_fresh_host_threads():
+    """A host thread that has made no CUDA call yet (autograd's worker is one) runs every operator."""
+    import threading
+
+    g = _gen(26)
+    q, k, v = (_randn(g, 1, 2, s, 64, dtype=BF16) for s in (40, 150, 150))
+    want = ts.cross_attention(q, k, v)
+    qd = q.detach().requires_grad_(True)
+    out = ts.cross_attention(qd, k, v)
+    lens = torch.tensor([40], device="cuda")
+    shared = ts.shared_prefix_attention(q[:, :, :1], k[0], v[0], k[:, :, :40], v[:, :, :40], lens)
+    got = []
+
+    def work():
+        got.append(ts.cross_attention(q, k, v))
+        got.append(ts.shared_prefix_attention(q[:, :, :1], k[0], v[0], k[:, :, :40], v[:, :, :40], lens))
+
+    def back():
+        got.append(torch.autograd.grad(out, qd, torch.ones_like(out), retain_graph=True)[0])
+
+    for f in (work, back):
+        t = threading.Thread(target=f)
+        t.start()
+        t.join()
+    assert torch.equal(got[0], want) and torch.equal(got[1], shared)
+    assert torch.equal(got[2], torch.autograd.grad(out, qd, torch.ones_like(out))[0])
+
+
 def test_cross_attention_repeats_bit_for_bit():
     g = _gen(22)
     for dtype, D in ((BF16, 128), (BF16, 64), (F32, 64)):

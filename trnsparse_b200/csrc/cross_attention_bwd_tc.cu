@@ -14,10 +14,10 @@
 //   S = F1 X1^T, dP = F2 X2^T, acc0 += dS X1, and in columns acc1 += P X2.
 // One CTA per SM, 10 warps: warp 8 TMA producer, warp 9 MMA issuer, warps 0-7
 // the pointwise part (thread = TMEM lane warp % 4, 64 of the 128 columns). P
-// overwrites S and dS overwrites dP in TMEM (A operands of the second
-// products), each half of the columns at the start of its own 64. MMAs run in
-// issue order, so per step: acc1 += P_j X2_j, S_{j+1}, acc0 += dS_j X1_j,
-// dP_{j+1}: the next scores are there when the pointwise warps return.
+// and dS overwrite scores in TMEM (A operands of the second products), each half
+// of the columns at the start of its own 64. MMAs run in issue order. Columns:
+// acc1 += P_j X2_j, S_{j+1}, acc0 += dS_j X1_j, dP_{j+1}; rows, with two S
+// buffers: dP_{j+1}, acc0 += dS_j X1_j, S_{j+2}.
 //
 // What bounds it: the walked tiles, 64 KB a step at head_dim 128 from L2 at
 // 40-50 GB/s per SM (about 1.4 us), against 3 (rows) or 4 (columns) products of
@@ -33,7 +33,7 @@ namespace {
 
 constexpr int kBwThreads = 320;
 
-template <int HD>
+template <int HD, bool COL>
 struct BwLayout {
   static constexpr int kChunks = HD / 64;
   static constexpr int kTile = 128 * HD * 2;
@@ -43,12 +43,13 @@ struct BwLayout {
   static constexpr int kStat = kX2 + kX2Stages * kTile;  // two stages: the walked rows' -log-sum-exp and -D
   static constexpr int kBar = kStat + 2 * 1024;
   static constexpr int kSmem = kBar + 256;
-  static constexpr uint32_t kTmemS = 0, kTmemDP = 128, kTmemAcc0 = 256, kTmemAcc1 = 384;
+  // columns: S / P, dP / dS, dK, dV; rows: two S / dS, dP, dQ
+  static constexpr uint32_t kTmemS = 0, kTmemDP = COL ? 128 : 256, kTmemAcc0 = COL ? 256 : 384, kTmemAcc1 = 384;
 };
 
 struct BwBars {
   uint64_t f_full, f_empty, x1_full[3], x1_empty[3], x2_full[2], x2_empty[2], st_full[2], st_empty[2];
-  uint64_t s_full, dp_full, p_full, ds_full, acc_full;
+  uint64_t s_full[2], dp_full, p_half, p_full, ds_full, acc_full;
   uint32_t tmem_slot;
   int abort_flag;
 };
@@ -74,6 +75,11 @@ __device__ __forceinline__ int bw_len(const BwArgs& A, int b) {
 // Unit u: part p of the walk of a fixed tile; b outermost, so round-robin CTAs see every length alike.
 struct BwUnit {
   int b, h, tile, part, beg, end;  // h: query head (rows) or key head (columns)
+  int rot;                         // the walk starts `rot` steps behind beg and wraps
+  __device__ int step(int i) const {
+    const int s = beg + rot + i;
+    return s < end ? s : s - (end - beg);
+  }
 };
 template <bool COL>
 __device__ __forceinline__ BwUnit bw_unit(const BwArgs& A, int u) {
@@ -89,6 +95,9 @@ __device__ __forceinline__ BwUnit bw_unit(const BwArgs& A, int u) {
   const int steps = COL ? (x.tile * 128 < len ? A.G * A.q_tiles : 0) : (len + 127) / 128;
   x.beg = min(steps, x.part * A.chunk);
   x.end = min(steps, x.beg + A.chunk);
+  // CTAs that run together share a head: each starts elsewhere in the walk, so they do not all read one tile
+  // from the same few L2 slices at a time.
+  x.rot = x.end > x.beg ? (x.tile * 5) % (x.end - x.beg) : 0;
   return x;
 }
 
@@ -97,7 +106,7 @@ __global__ void __launch_bounds__(kBwThreads, 1)
 xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tg,
                     const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                     const __grid_constant__ BwArgs A, int units) {
-  using Lay = BwLayout<HD>;
+  using Lay = BwLayout<HD, COL>;
   extern __shared__ __align__(16) uint8_t sb[];  // no static shared memory: 1024-byte aligned
   BwBars& B = *reinterpret_cast<BwBars*>(sb + Lay::kBar);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -114,8 +123,10 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       mbar_init(&B.st_full[i], 1);
       mbar_init(&B.st_empty[i], 1);
     }
-    mbar_init(&B.s_full, 1);
+    mbar_init(&B.s_full[0], 1);
+    mbar_init(&B.s_full[1], 1);
     mbar_init(&B.dp_full, 1);
+    mbar_init(&B.p_half, 256);
     mbar_init(&B.p_full, 256);
     mbar_init(&B.ds_full, 256);
     mbar_init(&B.acc_full, 1);
@@ -158,7 +169,8 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           }
         }
         ++nu;
-        for (int s = x.beg; s < x.end; ++s, ++n) {
+        for (int i = 0; i < x.end - x.beg; ++i, ++n) {
+          const int s = x.step(i);
           int h, row;
           if (COL) {
             const int g = s / A.q_tiles;
@@ -253,81 +265,163 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         const BwUnit x = bw_unit<COL>(A, u);
         const int steps = x.end - x.beg;
         if (steps <= 0) continue;
-        if (!ensure(false, &B.f_full, nu) || !ensure(false, &B.x1_full[s1], u1)) { ok = false; break; }
+        if (!ensure(false, &B.f_full, nu)) { ok = false; break; }
         ++nu;
-        tc_fence_after();
-        if (lead) {
-#pragma unroll
-          for (int kk = 0; kk < kK; ++kk) product(tmem + Lay::kTmemS, 0, x1_at(), kk);
-          umma_commit(&B.s_full);
-        }
-        if (!ensure(false, &B.x2_full[s2], u2)) { ok = false; break; }
-        if (lead) {
-#pragma unroll
-          for (int kk = 0; kk < kK; ++kk) product(tmem + Lay::kTmemDP, kF2, x2_at(), kk);
-          umma_commit(&B.dp_full);
-          if (!COL) umma_commit(&B.x2_empty[s2]);
-          if (steps == 1) umma_commit(&B.f_empty);
-        }
-        // s1, s2: this step's tiles. Barriers are looked at before the last MMA of a burst and waited for only if
-        // they were not complete then (cross_attention_tc.cu).
-        bool p_seen = false;
-        for (int j = 0; j < steps; ++j, ++n) {
-          const bool more = j + 1 < steps;
-          const uint32_t x1_now = x1_at(), x2_now = x2_at();
-          const int e1 = s1, e2 = s2;
-          next1();
-          next2();
-          if (!ensure(p_seen, &B.p_full, n)) { ok = false; break; }
+        // Barriers are looked at before the last MMA of a burst and waited for only if they were not complete then
+        // (cross_attention_tc.cu).
+        if constexpr (COL) {
+          if (!ensure(false, &B.x1_full[s1], u1)) { ok = false; break; }
           tc_fence_after();
-          bool x1_seen = !more, ds_seen = false, x2_seen = !more;
-          if (COL) {
+          if (lead) {
 #pragma unroll
-            for (int kk = 0; kk < 7; ++kk)
-              if (lead) accumulate(tmem + Lay::kTmemAcc1, tmem + Lay::kTmemS, x2_now, kk, j > 0 || kk > 0);
+            for (int kk = 0; kk < kK; ++kk) product(tmem + Lay::kTmemS, 0, x1_at(), kk);
+            umma_commit(&B.s_full[0]);
+          }
+          if (!ensure(false, &B.x2_full[s2], u2)) { ok = false; break; }
+          if (lead) {
+#pragma unroll
+            for (int kk = 0; kk < kK; ++kk) product(tmem + Lay::kTmemDP, kF2, x2_at(), kk);
+            umma_commit(&B.dp_full);
+            if (steps == 1) umma_commit(&B.f_empty);
+          }
+          // s1, s2: this step's tiles
+          bool p_seen = false;
+          for (int j = 0; j < steps; ++j, ++n) {
+            const bool more = j + 1 < steps;
+            const uint32_t x1_now = x1_at(), x2_now = x2_at();
+            const int e1 = s1, e2 = s2;
+            next1();
+            next2();
+            auto pv = [&](int kk, bool add) { accumulate(tmem + Lay::kTmemAcc1, tmem + Lay::kTmemS, x2_now, kk, add); };
+            // P of the first 32 columns of each warp half (k-steps 0, 1, 4, 5), then the rest
+            if (!ensure(p_seen, &B.p_half, n)) { ok = false; break; }
+            tc_fence_after();
+            if (lead) {
+              pv(0, j > 0);
+              pv(1, true);
+              pv(4, true);
+            }
+            const bool f_seen = mbar_test_wait(&B.p_full, n & 1);
+            if (lead) pv(5, true);
+            if (!ensure(f_seen, &B.p_full, n)) { ok = false; break; }
+            tc_fence_after();
+            bool x1_seen = !more, ds_seen = false, x2_seen = !more;
+            if (lead) {
+              pv(2, true);
+              pv(3, true);
+              pv(6, true);
+            }
             if (more) x1_seen = mbar_test_wait(&B.x1_full[s1], u1 & 1);
             else ds_seen = mbar_test_wait(&B.ds_full, n & 1);
             if (lead) {
-              accumulate(tmem + Lay::kTmemAcc1, tmem + Lay::kTmemS, x2_now, 7, true);
+              pv(7, true);
               umma_commit(&B.x2_empty[e2]);
             }
-          }
-          if (more) {
-            if (!ensure(x1_seen, &B.x1_full[s1], u1)) { ok = false; break; }
+            if (more) {
+              if (!ensure(x1_seen, &B.x1_full[s1], u1)) { ok = false; break; }
 #pragma unroll
-            for (int kk = 0; kk < kK - 1; ++kk)
-              if (lead) product(tmem + Lay::kTmemS, 0, x1_at(), kk);
-            ds_seen = mbar_test_wait(&B.ds_full, n & 1);
+              for (int kk = 0; kk < kK - 1; ++kk)
+                if (lead) product(tmem + Lay::kTmemS, 0, x1_at(), kk);
+              ds_seen = mbar_test_wait(&B.ds_full, n & 1);
+              if (lead) {
+                product(tmem + Lay::kTmemS, 0, x1_at(), kK - 1);
+                umma_commit(&B.s_full[0]);
+              }
+            }
+            if (!ensure(ds_seen, &B.ds_full, n)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < 7; ++kk)
+              if (lead) accumulate(tmem + Lay::kTmemAcc0, tmem + Lay::kTmemDP, x1_now, kk, j > 0 || kk > 0);
+            if (more) x2_seen = mbar_test_wait(&B.x2_full[s2], u2 & 1);
             if (lead) {
-              product(tmem + Lay::kTmemS, 0, x1_at(), kK - 1);
-              umma_commit(&B.s_full);
+              accumulate(tmem + Lay::kTmemAcc0, tmem + Lay::kTmemDP, x1_now, 7, true);
+              umma_commit(&B.x1_empty[e1]);
+              umma_commit(&B.st_empty[n & 1]);  // ds_full: the pointwise warps are through with them
+            }
+            if (more) {
+              if (!ensure(x2_seen, &B.x2_full[s2], u2)) { ok = false; break; }
+#pragma unroll
+              for (int kk = 0; kk < kK - 1; ++kk)
+                if (lead) product(tmem + Lay::kTmemDP, kF2, x2_at(), kk);
+              p_seen = mbar_test_wait(&B.p_half, (n + 1) & 1);
+              if (lead) {
+                product(tmem + Lay::kTmemDP, kF2, x2_at(), kK - 1);
+                umma_commit(&B.dp_full);
+                if (j + 2 == steps) umma_commit(&B.f_empty);  // the last use of the fixed tiles
+              }
+            } else if (lead) {
+              umma_commit(&B.acc_full);
             }
           }
-          if (!ensure(ds_seen, &B.ds_full, n)) { ok = false; break; }
+        } else {
+          // Rows need no P in TMEM, which leaves room for two S: S runs a step ahead of the pointwise warps, dS goes
+          // over the S it came from, and the next dP is issued before dS K: no product waits for a pointwise step
+          // but the one that needs its result.
+          if (!ensure(false, &B.x1_full[s1], u1)) { ok = false; break; }
           tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < 7; ++kk)
-            if (lead) accumulate(tmem + Lay::kTmemAcc0, tmem + Lay::kTmemDP, x1_now, kk, j > 0 || kk > 0);
-          if (more) x2_seen = mbar_test_wait(&B.x2_full[s2], u2 & 1);
-          if (lead) {
-            accumulate(tmem + Lay::kTmemAcc0, tmem + Lay::kTmemDP, x1_now, 7, true);
-            umma_commit(&B.x1_empty[e1]);
-            if (COL) umma_commit(&B.st_empty[n & 1]);  // ds_full: the pointwise warps are through with them
-          }
-          if (more) {
-            if (!ensure(x2_seen, &B.x2_full[s2], u2)) { ok = false; break; }
-#pragma unroll
-            for (int kk = 0; kk < kK - 1; ++kk)
-              if (lead) product(tmem + Lay::kTmemDP, kF2, x2_at(), kk);
-            p_seen = mbar_test_wait(&B.p_full, (n + 1) & 1);
+          int c1 = s1;  // this step's K; s1 runs ahead to the next S
+          auto next_s = [&](int m) {
             if (lead) {
-              product(tmem + Lay::kTmemDP, kF2, x2_at(), kK - 1);
-              umma_commit(&B.dp_full);
-              if (!COL) umma_commit(&B.x2_empty[s2]);
-              if (j + 2 == steps) umma_commit(&B.f_empty);  // the last use of the fixed tiles
+#pragma unroll
+              for (int kk = 0; kk < kK; ++kk) product(tmem + Lay::kTmemS + (m & 1) * 128, 0, x1_at(), kk);
+              umma_commit(&B.s_full[m & 1]);
             }
-          } else if (lead) {
-            umma_commit(&B.acc_full);
+            next1();
+          };
+          next_s(n);
+          if (!ensure(false, &B.x2_full[s2], u2)) { ok = false; break; }
+          if (lead) {
+#pragma unroll
+            for (int kk = 0; kk < kK; ++kk) product(tmem + Lay::kTmemDP, kF2, x2_at(), kk);
+            umma_commit(&B.dp_full);
+            umma_commit(&B.x2_empty[s2]);
+            if (steps == 1) umma_commit(&B.f_empty);
+          }
+          next2();
+          if (steps > 1) {
+            if (!ensure(false, &B.x1_full[s1], u1)) { ok = false; break; }
+            next_s(n + 1);
+          }
+          bool ds_seen = false;
+          for (int j = 0; j < steps; ++j, ++n) {
+            const bool more = j + 1 < steps;
+            bool x2_seen = more && mbar_test_wait(&B.x2_full[s2], u2 & 1);
+            if (!ensure(ds_seen, &B.ds_full, n)) { ok = false; break; }
+            ds_seen = false;
+            tc_fence_after();
+            if (more) {
+              if (!ensure(x2_seen, &B.x2_full[s2], u2)) { ok = false; break; }
+              if (lead) {
+#pragma unroll
+                for (int kk = 0; kk < kK; ++kk) product(tmem + Lay::kTmemDP, kF2, x2_at(), kk);
+                umma_commit(&B.dp_full);
+                umma_commit(&B.x2_empty[s2]);
+                if (j + 2 == steps) umma_commit(&B.f_empty);  // the last use of the fixed tiles
+              }
+              next2();
+            }
+            const uint32_t x1_now = kX1 + c1 * (Lay::kTile >> 4);
+#pragma unroll
+            for (int kk = 0; kk < 7; ++kk)
+              if (lead) accumulate(tmem + Lay::kTmemAcc0, tmem + Lay::kTmemS + (n & 1) * 128, x1_now, kk, j > 0 || kk > 0);
+            const bool x1_seen = j + 2 < steps && mbar_test_wait(&B.x1_full[s1], u1 & 1);
+            if (lead) {
+              accumulate(tmem + Lay::kTmemAcc0, tmem + Lay::kTmemS + (n & 1) * 128, x1_now, 7, true);
+              umma_commit(&B.x1_empty[c1]);
+              if (!more) umma_commit(&B.acc_full);
+            }
+            c1 = c1 + 1 == Lay::kX1Stages ? 0 : c1 + 1;
+            if (j + 2 < steps) {
+              if (!ensure(x1_seen, &B.x1_full[s1], u1)) { ok = false; break; }
+              if (lead) {
+#pragma unroll
+                for (int kk = 0; kk < kK; ++kk) product(tmem + Lay::kTmemS + (n & 1) * 128, 0, x1_at(), kk);
+                umma_commit(&B.s_full[n & 1]);
+              }
+              next1();
+              ds_seen = mbar_test_wait(&B.ds_full, (n + 1) & 1);
+            }
           }
         }
       }
@@ -356,7 +450,8 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         row_ndelta = pack2(A.ndelta[at], A.ndelta[at]);
       }
       const bool any_dead = COL && __any_sync(0xffffffffu, dead);
-      for (int s = x.beg; s < x.end; ++s, ++n) {
+      for (int step = 0; step < x.end - x.beg; ++step, ++n) {
+        const int s = x.step(step);
         uint32_t kept[2] = {~0u, ~0u};
         bool part = false;
         if (!COL) {
@@ -370,22 +465,33 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           }
         }
         const float* st = reinterpret_cast<const float*>(sb + Lay::kStat + (n & 1) * 1024) + half * 64;
-        if (!warp_all(!*abort_flag && mbar_wait(&B.s_full, n & 1))) { ok = false; break; }
+        if (!warp_all(!*abort_flag && mbar_wait(&B.s_full[COL ? 0 : n & 1], (COL ? n : n >> 1) & 1))) { ok = false; break; }
         if (COL && !warp_all(mbar_wait(&B.st_full[n & 1], (n >> 1) & 1))) { ok = false; break; }
         tc_fence_after();
+        const uint32_t t_sn = t_s + (COL ? 0 : (n & 1) * 128);
         uint32_t p[2][32], pk[32];
-        tmem_ld32(t_s, p[0]);
-        tmem_ld32(t_s + 32, p[1]);
+        tmem_ld32(t_sn, p[0]);
+        tmem_ld32(t_sn + 32, p[1]);
         tmem_wait_ld32(p[0]);
         tmem_wait_ld32(p[1]);
-        if (!COL) {
-          tc_fence_before();
-          mbar_arrive(&B.p_full);  // the score columns may be written again
-        }
+        // hidden keys: the packed P and dS become zeros, whatever was computed
+        auto hide = [&](uint32_t* w, int c) {
+          if (COL) {
+            if (any_dead)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = dead ? 0u : w[i];
+          } else if (part) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const uint32_t k = kept[c] >> (2 * i);
+              w[i] &= (k & 1u ? 0xffffu : 0u) | (k & 2u ? 0xffff0000u : 0u);
+            }
+          }
+        };
         // Packed fp32 arithmetic; one in four exponentials on the FMA pipe (two warps of a scheduler share a
         // special-function unit that does four a clock).
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 2; ++c) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
             uint64_t l0 = row_nlse, l1 = row_nlse;
@@ -416,27 +522,15 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
               pk[c * 16 + i / 2 + 1] = pack_bf16(e2, e3);
             }
           }
-        // hidden keys: the packed P and dS become zeros, whatever was computed
-        auto hide = [&](uint32_t (&w)[32]) {
           if (COL) {
-            if (any_dead)
-#pragma unroll
-              for (int i = 0; i < 32; ++i) w[i] = dead ? 0u : w[i];
-          } else if (part) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const uint32_t k = kept[i >> 4] >> (2 * (i & 15));
-              w[i] &= (k & 1u ? 0xffffu : 0u) | (k & 2u ? 0xffff0000u : 0u);
-            }
+            hide(pk + c * 16, c);
+            tmem_st16(t_s + c * 16, pk + c * 16);
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(c ? &B.p_full : &B.p_half);
           }
-        };
-        if (COL) {
-          hide(pk);
-          tmem_st32(t_s, pk);
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(&B.p_full);
-        } else if (part && half == 0) {
+        }
+        if (!COL && part && half == 0) {
           // hidden keys' K rows become zeros before dS K (their scores are read already)
           const int key = s * 128 + r;
           if (!(key < len && (mask == nullptr || mask[key] != 0))) {
@@ -476,8 +570,9 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
             pk[c * 16 + i / 2 + 1] = pack_bf16(e2, e3);
           }
         }
-        hide(pk);
-        tmem_st32(t_dp, pk);
+        hide(pk, 0);
+        hide(pk + 16, 1);
+        tmem_st32(COL ? t_dp : t_sn, pk);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&B.ds_full);
@@ -490,7 +585,8 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         ++nu;
         tc_fence_after();
       }
-      const bool live = fixed < (COL ? A.Sk : A.Sq);
+      const int limit = COL ? A.Sk : A.Sq;
+      const bool live = fixed < limit;
       const int64_t fr = (static_cast<int64_t>(x.b) * (COL ? A.Hkv : A.Hq) + x.h) * (COL ? A.Sk : A.Sq) + fixed;
 #pragma unroll
       for (int a = 0; a < (COL ? 2 : 1); ++a) {
@@ -516,13 +612,19 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
             for (int i = 0; i < 32; i += 4)
               if (d0 + i < A.D)
                 *reinterpret_cast<float4*>(po + d0 + i) = make_float4(val(i), val(i + 1), val(i + 2), val(i + 3));
-          } else if (live) {
+          } else if (po == nullptr) {
+            // four lanes exchange their four 16-byte pieces, so that a store writes 64 contiguous bytes of a row
+            uint4 q[4];
 #pragma unroll
-            for (int i = 0; i < 32; i += 8)
-              if (d0 + i < A.D)
-                *reinterpret_cast<uint4*>(ob + d0 + i) =
-                    make_uint4(pack_bf16(val(i), val(i + 1)), pack_bf16(val(i + 2), val(i + 3)),
-                               pack_bf16(val(i + 4), val(i + 5)), pack_bf16(val(i + 6), val(i + 7)));
+            for (int i = 0; i < 4; ++i)
+              q[i] = make_uint4(pack_bf16(val(8 * i), val(8 * i + 1)), pack_bf16(val(8 * i + 2), val(8 * i + 3)),
+                                pack_bf16(val(8 * i + 4), val(8 * i + 5)), pack_bf16(val(8 * i + 6), val(8 * i + 7)));
+            quad_transpose(q, lane & 3);
+            const int d = d0 + (lane & 3) * 8;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (fixed - (lane & 3) + k < limit && d < A.D)
+                *reinterpret_cast<uint4*>(ob + (k - (lane & 3)) * os[2] + d) = q[k];
           }
         }
       }
@@ -631,7 +733,7 @@ BwPlan bw_plan(const trnsparse_attention_args* a) {
 
 template <int HD, bool COL>
 int bw_launch(const BwArgs& A, const XMap (&m)[4], int units, cudaStream_t st) {
-  using Lay = BwLayout<HD>;
+  using Lay = BwLayout<HD, COL>;
   auto kern = xattn_bwd_tc_kernel<HD, COL>;
   static unsigned long long done = 0;  // a bit per device; setting the attribute again is harmless
   int rc = allow_smem(kern, Lay::kSmem, &done, "cross_attention backward: set smem");

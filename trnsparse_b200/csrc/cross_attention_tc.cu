@@ -117,27 +117,6 @@ struct FwArgs {
   uint32_t q_flip;             // sign bits of a negative scale, applied to Q
 };
 
-__device__ __forceinline__ uint4 shfl_xor4(uint4 v, int m) {
-  return make_uint4(__shfl_xor_sync(0xffffffffu, v.x, m), __shfl_xor_sync(0xffffffffu, v.y, m),
-                    __shfl_xor_sync(0xffffffffu, v.z, m), __shfl_xor_sync(0xffffffffu, v.w, m));
-}
-// Lane i of four holds q[0..3]; afterwards q[k] is what lane k held as q[i].
-__device__ __forceinline__ void quad_transpose(uint4 (&q)[4], int i) {
-#pragma unroll
-  for (int m = 1; m <= 2; m <<= 1) {
-    const bool up = i & m;
-#pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      if (a & m) continue;
-      // swap q[a | m] of the lower lane with q[a] of the upper lane
-      const uint4 give = up ? q[a] : q[a | m];
-      const uint4 got = shfl_xor4(give, m);
-      if (up) q[a] = got;
-      else q[a | m] = got;
-    }
-  }
-}
-
 __device__ __forceinline__ int fw_tiles(const FwSide& sd, int bi) { return (side_len(sd.s, bi) + kFwKeys - 1) / kFwKeys; }
 // Cost of an item in key tiles: its tiles and, unless it has none, kFwItemCost for its Q, drain and output (1, 2, 3
 // measured: 45.4, 43.5, 42.9 us in a decode over 8 ragged sequences, 170, 167, 175 us in prompts of 777 tokens).

@@ -48,9 +48,20 @@ inline int make_xmap(XMap* m, const void* base, int64_t D, int64_t len, int64_t 
   cuuint64_t strides[3] = {(cuuint64_t)row, m->mul_h ? (cuuint64_t)s_h * 2 : (cuuint64_t)row,
                            m->mul_b ? (cuuint64_t)s_b * 2 : (cuuint64_t)row};
   cuuint32_t box[4] = {64, box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
-  CUresult r = encode(&m->map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
-                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto run = [&] {
+    return encode(&m->map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = run();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // a driver call, and this host thread (autograd's, for one) has made no runtime call yet
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return cuda_status(e, "tensor map: make the device's context current");
+    r = run();
+  }
   if (r != CUDA_SUCCESS) return fail(TRNSPARSE_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return TRNSPARSE_OK;
 }
@@ -155,6 +166,27 @@ __device__ __forceinline__ void exp2_poly2(uint64_t x2, float& a, float& b) {
   unpack2(mul2(x, pack2(0.f, 0.f)), za, zb);
   a = xa >= -126.f ? __uint_as_float((__float_as_uint(ta) << 23) + __float_as_uint(pa)) : za;
   b = xb >= -126.f ? __uint_as_float((__float_as_uint(tb) << 23) + __float_as_uint(pb)) : zb;
+}
+
+__device__ __forceinline__ uint4 shfl_xor4(uint4 v, int m) {
+  return make_uint4(__shfl_xor_sync(0xffffffffu, v.x, m), __shfl_xor_sync(0xffffffffu, v.y, m),
+                    __shfl_xor_sync(0xffffffffu, v.z, m), __shfl_xor_sync(0xffffffffu, v.w, m));
+}
+// Lane i of four holds q[0..3]; afterwards q[k] is what lane k held as q[i].
+__device__ __forceinline__ void quad_transpose(uint4 (&q)[4], int i) {
+#pragma unroll
+  for (int m = 1; m <= 2; m <<= 1) {
+    const bool up = i & m;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      if (a & m) continue;
+      // swap q[a | m] of the lower lane with q[a] of the upper lane
+      const uint4 give = up ? q[a] : q[a | m];
+      const uint4 got = shfl_xor4(give, m);
+      if (up) q[a] = got;
+      else q[a | m] = got;
+    }
+  }
 }
 
 // Asynchronous 16-byte copy global -> shared, zeros when !in (then nothing is read).
