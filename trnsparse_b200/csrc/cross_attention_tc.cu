@@ -40,16 +40,17 @@
 // their V rows are zeroed in shared memory before the product, so NaN or
 // infinity in padding never meets a zero P. Only tiles that hold hidden keys
 // pay for it.
-#include "xattn_tc.cuh"
+#include "xattn_items.cuh"
 
 namespace tsb {
 namespace {
 
 constexpr int kFwThreads = 352;
 constexpr int kFwRows = 256;  // rows of an item, two halves of 128
-constexpr int kFwKeys = 128;
+constexpr int kFwKeys = 128, kFwKeyShift = 7;
 constexpr float kFwLazy = 8.f;
-constexpr int kFwItemCost = 2;  // in key tiles; see fw_cost
+// 1, 2, 3 measured: 45.4, 43.5, 42.9 us in a decode over 8 ragged sequences, 170, 167, 175 us in prompts of 777 tokens
+constexpr int kFwItemCost = 2;
 
 template <int HD>
 struct FwLayout {
@@ -63,13 +64,6 @@ struct FwLayout {
   static constexpr uint32_t kTmemO = 256;  // S / P: [0, 128) and [128, 256); O: [256, +HD) and [384, +HD)
 };
 
-// A run of key tiles of one item; side < 0 ends the list. Made by one warp, read by all roles from a ring in
-// shared memory: the walk's state and divisions stay out of the other warps' registers.
-struct FwSeg {
-  int side, item, bi, h, rt, k0, k1, n, len;
-};
-constexpr int kFwSegs = 4;
-
 struct FwBars {
   uint64_t full[10], empty[10], q_full[2], s_full[2], p_half[2], p_full[2], o_done[2];
   uint64_t seg_full[kFwSegs], seg_empty[kFwSegs];
@@ -78,183 +72,7 @@ struct FwBars {
   int abort_flag;
 };
 
-// Division by a run-time constant: n / d for 0 <= n < 2^31 is the high word of n * mul, shifted by s, with
-// 2^s < d <= 2^(s + 1) and mul = 2^(32 + s) / d rounded up (below 2^32): the rounding adds less than d n to n 2^(32 +
-// s), so less than one part in n to the quotient.
-struct FastDiv {
-  uint32_t d, mul, shift;
-};
-inline FastDiv fast_div(int d) {
-  FastDiv f = {static_cast<uint32_t>(d), 0u, 0u};
-  while ((2u << f.shift) < static_cast<uint32_t>(d)) ++f.shift;
-  if (d > 1) f.mul = static_cast<uint32_t>(((1ull << (32 + f.shift)) + d - 1) / d);
-  return f;
-}
-__device__ __forceinline__ int fdiv(const FastDiv& f, int n) {
-  return f.d == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), f.mul) >> f.shift);
-}
-
 static_assert(sizeof(FwBars) <= 512, "FwLayout::kSmem");
-
-struct FwSide {
-  XSide s;
-  int row_tiles, items;
-  FastDiv by_T, by_G;
-  int mul_kh, mul_kb, mul_vh, mul_vb;
-};
-
-struct FwArgs {
-  FwSide side[2];
-  int sides, D, whole;         // whole: items per CTA taken whole (one side only)
-  // Slots of (O / l, log-sum-exp) as [D / 4][rows][4], so that a warp's 32 rows write whole lines: two per CTA
-  // and, with two sides, one per item that a single CTA finished.
-  float *slots, *slot_lse, *item_slots[2], *item_lse[2];
-  int slot_rows, item_rows[2];  // min(256, rows of an item), the largest and each side's
-  int2* pieces;                // first and last CTA of every item of the split part
-  __nv_bfloat16* out;
-  float* lse;
-  float scale_log2;            // |scale| log2(e)
-  uint32_t q_flip;             // sign bits of a negative scale, applied to Q
-};
-
-__device__ __forceinline__ int fw_tiles(const FwSide& sd, int bi) { return (side_len(sd.s, bi) + kFwKeys - 1) / kFwKeys; }
-// Cost of an item in key tiles: its tiles and, unless it has none, kFwItemCost for its Q, drain and output (1, 2, 3
-// measured: 45.4, 43.5, 42.9 us in a decode over 8 ragged sequences, 170, 167, 175 us in prompts of 777 tokens).
-__device__ __forceinline__ int fw_cost(int tiles) { return tiles > 0 ? tiles + kFwItemCost : 0; }
-
-__device__ __forceinline__ XRow fw_row(const FwSide& sd, int64_t r) {
-  const int n = static_cast<int>(r), u = fdiv(sd.by_T, n), b2 = fdiv(sd.by_G, u);
-  XRow x;
-  x.t = n - u * sd.s.T;
-  x.g = u - b2 * sd.s.G;
-  x.b2 = b2;
-  return x;
-}
-
-// Walks a CTA's items: whole ones first (also those without keys), then its run [begin, begin + left) of the
-// split part's cost.
-struct FwCursor {
-  const FwArgs& A;
-  long long begin, left;
-  long long at;  // where the last item begins
-  int w, side, item, k;
-  __device__ void decode(FwSeg& g) const {
-    const FwSide& sd = A.side[g.side];
-    const int per = sd.s.hkv * sd.row_tiles;
-    g.bi = g.item / per;
-    const int r = g.item - g.bi * per;
-    g.h = r / sd.row_tiles;
-    g.rt = r - g.h * sd.row_tiles;
-    g.len = side_len(sd.s, g.bi);
-    g.n = (g.len + kFwKeys - 1) / kFwKeys;
-  }
-  __device__ bool next(FwSeg& g) {
-    if (w < A.whole) {
-      g.side = 0;
-      g.item = w * gridDim.x + blockIdx.x;
-      ++w;
-      decode(g);
-      g.k0 = 0;
-      g.k1 = g.n;
-      return true;
-    }
-    while (left > 0) {
-      if (item >= A.side[side].items) {
-        ++side;
-        item = 0;
-      }
-      g.side = side;
-      g.item = item++;
-      decode(g);
-      const int k0 = k;
-      k = 0;
-      if (g.n == 0) continue;
-      at = begin - k0;
-      const long long take = min(static_cast<long long>(fw_cost(g.n) - k0), left);
-      g.k0 = k0;
-      g.k1 = static_cast<int>(min(static_cast<long long>(g.n), k0 + take));
-      begin += take;
-      left -= take;
-      if (g.k0 < g.k1) return true;
-    }
-    return false;
-  }
-};
-
-// Sums of the items' costs, and position lookups, by one warp.
-// Lane l holds 8 consecutive entries of every 256.
-struct FwScan {
-  // Cost of the items before item `i`.
-  static __device__ long long before(const FwSide& sd, int i, int lane) {
-    const int per = sd.s.hkv * sd.row_tiles, b0 = i / per;
-    long long t = 0;
-    if (sd.s.lengths == nullptr) {
-      t = static_cast<long long>(b0) * fw_cost(fw_tiles(sd, 0));
-    } else {
-      for (int base = 0; base < b0; base += 256)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int b = base + lane * 8 + e;
-          if (b < b0) t += fw_cost(fw_tiles(sd, b));
-        }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    }
-    t *= per;
-    const int r = i - b0 * per;
-    return r == 0 ? t : t + static_cast<long long>(r) * fw_cost(fw_tiles(sd, b0));
-  }
-  // Item and place within it at position x of the side (x below its total).
-  static __device__ void locate(const FwSide& sd, long long x, int lane, int& item, int& k) {
-    const int per = sd.s.hkv * sd.row_tiles;
-    if (sd.s.lengths == nullptr) {
-      const int n = fw_cost(fw_tiles(sd, 0));
-      item = static_cast<int>(x / n);
-      k = static_cast<int>(x - static_cast<long long>(item) * n);
-      return;
-    }
-    long long done = 0;
-    for (int base = 0; base < sd.s.nb; base += 256) {
-      int n[8];
-      long long s = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int b = base + lane * 8 + e;
-        n[e] = b < sd.s.nb ? fw_cost(fw_tiles(sd, b)) : 0;
-        s += n[e];
-      }
-      long long inc = s;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      const long long all = __shfl_sync(0xffffffffu, inc, 31);
-      if ((done + all) * per > x) {
-        const unsigned hit = __ballot_sync(0xffffffffu, (done + inc) * per > x);
-        const int src = __ffs(hit) - 1;
-        long long at = done + inc - s;
-        int fi = 0, fk = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const long long end = at + n[e];
-          if (at * per <= x && x < end * per) {
-            const long long rel = x - at * per;
-            fi = (base + lane * 8 + e) * per + static_cast<int>(rel / n[e]);
-            fk = static_cast<int>(rel % n[e]);
-          }
-          at = end;
-        }
-        item = __shfl_sync(0xffffffffu, fi, src);
-        k = __shfl_sync(0xffffffffu, fk, src);
-        return;
-      }
-      done += all;
-    }
-    item = sd.items;  // past the end: never reached for x below the total
-    k = 0;
-  }
-};
 
 template <int HD>
 __global__ void __launch_bounds__(kFwThreads, 1)
@@ -307,24 +125,8 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
   if (warp == 10) {
     // ---------------- the list of segments
     if (!*abort_flag) {
-      // this CTA's run: [W c / G, W (c + 1) / G) of the cost W behind the whole items, G the CTAs that get any (a
-      // piece list has no gaps)
-      const int first = A.whole * static_cast<int>(gridDim.x);
-      const long long t0 = FwScan::before(A.side[0], A.side[0].items, lane);
-      const long long t1 = A.sides > 1 ? FwScan::before(A.side[1], A.side[1].items, lane) : 0;
-      const long long s0 = first ? FwScan::before(A.side[0], first, lane) : 0;
-      const long long W = t0 + t1 - s0;
-      const long long G = W < gridDim.x ? W : gridDim.x, c = blockIdx.x;
-      const long long lo = c < G ? W * c / G : W, hi = c < G ? W * (c + 1) / G : W;
-      FwCursor cur{A, lo, hi - lo, 0, 0, 0, 0, 0};
-      if (hi > lo) {
-        long long x = s0 + lo;
-        if (x >= t0) {
-          cur.side = 1;
-          x -= t0;
-        }
-        FwScan::locate(A.side[cur.side], x, lane, cur.item, cur.k);
-      }
+      FwCursor cur{A};
+      const FwRun run = fw_start(A, cur, lane);
       if (lane == 0) {
         FwSeg g;
         for (int i = 0;; ++i) {
@@ -337,9 +139,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
           B.seg[i % kFwSegs] = g;
           mbar_arrive(&B.seg_full[i % kFwSegs]);
           if (!more || *abort_flag) break;
-          if (!whole && g.k0 == 0)  // an item that begins here: which CTAs hold its pieces
-            A.pieces[g.side == 0 ? g.item - first : A.side[0].items + g.item] =
-                make_int2(blockIdx.x, static_cast<int>(((cur.at + g.n) * G - 1) / W));
+          if (!whole && g.k0 == 0) fw_note_pieces(A, cur, run, g);
         }
       }
     }
@@ -740,21 +540,15 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
         const float ls = m == -INFINITY ? -INFINITY : m + log2f(l);
         const XRow x = fw_row(sd, live ? row : 0);
         const bool all = g.k0 == 0 && g.k1 == g.n;
-        const bool to_slot = !all || A.sides > 1;
+        const bool to_slot = !all || A.keep;
         float* po = nullptr;
         __nv_bfloat16* ob = nullptr;
         int slot_stride = 0;
         if (to_slot) {
-          if (all) {
-            slot_stride = A.item_rows[g.side];
-            po = A.item_slots[g.side] + static_cast<int64_t>(g.item) * slot_stride * A.D;
-            if (live) A.item_lse[g.side][static_cast<int64_t>(g.item) * slot_stride + half * 128 + r] = ls;
-          } else {
-            const int64_t slot = 2ll * blockIdx.x + (g.k0 == 0 ? 1 : 0);
-            slot_stride = A.slot_rows;
-            po = A.slots + slot * slot_stride * A.D;
-            if (live) A.slot_lse[slot * slot_stride + half * 128 + r] = ls;
-          }
+          const int64_t slot = all ? g.item : 2ll * blockIdx.x + (g.k0 == 0 ? 1 : 0);
+          slot_stride = all ? sd.item_rows : sd.slot_rows;
+          po = (all ? sd.item_slots : sd.slots) + slot * slot_stride * A.D;
+          if (live) (all ? sd.item_lse : sd.slot_lse)[slot * slot_stride + half * 128 + r] = ls;
           po += (half * 128 + r) * 4;
         } else if (live) {
           ob = A.out + o_offset(s, g.bi, g.h, x);
@@ -808,17 +602,16 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
 // rows fastest, as the slots are laid out; the rows then leave through shared memory as whole lines. One side:
 // blocks walk its split items (those that one CTA finished are done). Two sides: blocks walk the own side's items,
 // whose rows r of sequence b are rows b G T + r of the prefix's item of that key head.
-__global__ void __launch_bounds__(256) xattn_join_kernel(const __grid_constant__ FwArgs A, int G) {
+__global__ void __launch_bounds__(256) xattn_join_kernel(const __grid_constant__ FwArgs A) {
   __shared__ __align__(16) __nv_bfloat16 tile[32][136];
   grid_dep_wait();
   const FwSide& S = A.side[A.sides - 1];
-  const int item = blockIdx.x + A.whole * G, per = S.s.hkv * S.row_tiles;
+  const int item = blockIdx.x + S.first, per = S.s.hkv * S.row_tiles;
   const int bi = item / per, rem = item - bi * per, h = rem / S.row_tiles, rt = rem - h * S.row_tiles;
-  const int64_t R = side_rows(S.s), row0 = static_cast<int64_t>(rt) * kFwRows + blockIdx.y * 32;
-  const int rows = static_cast<int>(min(static_cast<int64_t>(32), R - row0));
-  const int index = A.sides > 1 ? A.side[0].items + static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x);
+  const int64_t R = side_rows(S.s), row0 = static_cast<int64_t>(rt) * S.tile_rows + blockIdx.y * 32;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(32), min(R, static_cast<int64_t>(rt + 1) * S.tile_rows) - row0));
   const int n = fw_tiles(S, bi);
-  const int2 p = n > 0 ? A.pieces[index] : make_int2(0, -1);
+  const int2 p = n > 0 ? S.pieces[blockIdx.x] : make_int2(0, -1);
   if (rows <= 0 || (A.sides == 1 && n > 0 && p.x == p.y)) return;
   const int q4 = A.D / 4;
   for (int i = threadIdx.x; i < rows * q4; i += 256) {
@@ -835,18 +628,18 @@ __global__ void __launch_bounds__(256) xattn_join_kernel(const __grid_constant__
       acc = make_float4(acc.x * c + w * o.x, acc.y * c + w * o.y, acc.z * c + w * o.z, acc.w * c + w * o.w);
       mx = mn;
     };
-    auto add_item = [&](int2 q, int side, int it, int at) {
-      if (A.sides > 1 && q.x == q.y) add(A.item_slots[side], A.item_lse[side], A.item_rows[side], it, at);
+    auto add_item = [&](int2 q, const FwSide& sd, int it, int at) {
+      if (A.sides > 1 && q.x == q.y) add(sd.item_slots, sd.item_lse, sd.item_rows, it, at);
       else
-        for (int c = q.x; c <= q.y; ++c) add(A.slots, A.slot_lse, A.slot_rows, 2ll * c + (c == q.x ? 1 : 0), at);
+        for (int c = q.x; c <= q.y; ++c) add(sd.slots, sd.slot_lse, sd.slot_rows, 2ll * c + (c == q.x ? 1 : 0), at);
     };
     if (A.sides > 1) {
       const FwSide& P = A.side[0];
       const int64_t pr = static_cast<int64_t>(bi) * S.s.G * S.s.T + row0 + r;
-      const int pi = h * P.row_tiles + static_cast<int>(pr / kFwRows);
-      add_item(A.pieces[pi], 0, pi, static_cast<int>(pr % kFwRows));
+      const int prt = static_cast<int>(pr / P.tile_rows), pi = h * P.row_tiles + prt;
+      add_item(P.pieces[pi], P, pi, static_cast<int>(pr - static_cast<int64_t>(prt) * P.tile_rows));
     }
-    add_item(p, A.sides - 1, item, blockIdx.y * 32 + r);
+    add_item(p, S, item, blockIdx.y * 32 + r);
     const float inv = den == 0.f ? 0.f : 1.f / den;
     *reinterpret_cast<uint2*>(&tile[r][c4 * 4]) =
         make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
@@ -862,45 +655,64 @@ __global__ void __launch_bounds__(256) xattn_join_kernel(const __grid_constant__
   }
 }
 
+// One launch: the sides it takes (all of the call's, or one of two), in the form their rows ask for.
+struct FwLaunch {
+  bool few;
+  int sides, side[2], grid, whole, split_items, slot_rows;
+  int64_t items[2];
+  size_t o, lse, item_o[2], item_lse[2], pieces[2];  // byte offsets in the workspace
+};
 struct FwPlan {
-  int grid, whole, slot_rows, split_items;
-  size_t o[3], lse[3], pieces, total;  // byte offsets: the CTAs' slots, each side's item slots
+  int launches;
+  FwLaunch l[2];
+  size_t total;
 };
 
 FwPlan fw_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n) {
   FwPlan p = {};
-  const int sms = sm_count();
-  int64_t most = 0, tiles = 0, items = 0;
-  for (int i = 0; i < n; ++i) {
-    const int64_t R = side_rows(s[i]), it = (R + kFwRows - 1) / kFwRows * s[i].nb * s[i].hkv;
-    most = most > R ? most : R;
-    items += it;
-    tiles += it * ((s[i].klen + kFwKeys - 1) / kFwKeys);
-  }
-  p.grid = static_cast<int>(tiles < sms ? (tiles > 0 ? tiles : 1) : sms);
-  // One side: whole items for all but the last round (items of one length), or the last one to two rounds, which
-  // then even out what unequal lengths left.
-  const int last = s[0].lengths != nullptr && s[0].nb > 1 ? 1 : 0;
-  if (n == 1 && items >= (1 + last) * static_cast<int64_t>(p.grid)) p.whole = static_cast<int>(items / p.grid - last);
-  p.split_items = static_cast<int>(items - static_cast<int64_t>(p.whole) * p.grid);
-  p.slot_rows = static_cast<int>(most < kFwRows ? most : kFwRows);
-  // slots and their log-sum-exps, then (two sides) each side's item slots
-  int64_t slots = 2ll * p.grid, at = 0;
-  for (int i = 0; i < 3; ++i) {
-    int64_t rows = p.slot_rows;
-    if (i > 0) {
-      if (n < 2) break;
-      const int64_t R = side_rows(s[i - 1]);
-      rows = R < kFwRows ? R : kFwRows;
-      slots = (R + kFwRows - 1) / kFwRows * s[i - 1].nb * s[i - 1].hkv;
+  bool few[2] = {false, false};
+  for (int i = 0; i < n; ++i) few[i] = side_rows(s[i]) <= kFewRows;
+  p.launches = n > 1 && few[0] != few[1] ? 2 : 1;
+  size_t at = 0;
+  const size_t D = static_cast<size_t>(a->head_dim);
+  for (int i = 0; i < p.launches; ++i) {
+    FwLaunch& l = p.l[i];
+    l.sides = p.launches == 2 ? 1 : n;
+    l.few = few[p.launches == 2 ? i : 0];
+    const int64_t tile_rows = l.few ? kFewRows : kFwRows, shift = l.few ? kFewKeyShift : kFwKeyShift;
+    int64_t most = 0, tiles = 0, items = 0;
+    for (int j = 0; j < l.sides; ++j) {
+      const XSide& x = s[l.side[j] = p.launches == 2 ? i : j];
+      const int64_t R = side_rows(x);
+      l.items[j] = (R + tile_rows - 1) / tile_rows * x.nb * x.hkv;
+      items += l.items[j];
+      tiles += l.items[j] * ((x.klen + (1ll << shift) - 1) >> shift);
+      most = most > R ? most : R;
     }
-    p.o[i] = at;
-    at += align256(sizeof(float) * slots * rows * a->head_dim);
-    p.lse[i] = at;
-    at += align256(sizeof(float) * slots * rows);
+    const int64_t full = l.few ? few_rows_grid() : sm_count();
+    l.grid = static_cast<int>(tiles < full ? (tiles > 0 ? tiles : 1) : full);
+    // One side: whole items for all but the last round (items of one length), or the last one to two rounds, which
+    // then even out what unequal lengths left.
+    const XSide& x0 = s[l.side[0]];
+    const int last = x0.lengths != nullptr && x0.nb > 1 ? 1 : 0;
+    if (n == 1 && items >= (1 + last) * static_cast<int64_t>(l.grid)) l.whole = static_cast<int>(items / l.grid - last);
+    l.split_items = static_cast<int>(items - static_cast<int64_t>(l.whole) * l.grid);
+    l.slot_rows = static_cast<int>(most < tile_rows ? most : tile_rows);
+    auto take = [&](size_t bytes) {
+      const size_t was = at;
+      at += align256(bytes);
+      return was;
+    };
+    l.o = take(sizeof(float) * 2 * l.grid * l.slot_rows * D);
+    l.lse = take(sizeof(float) * 2 * l.grid * l.slot_rows);
+    for (int j = 0; j < l.sides; ++j) {
+      const int64_t R = side_rows(s[l.side[j]]), rows = R < tile_rows ? R : tile_rows;
+      l.item_o[j] = take(n > 1 ? sizeof(float) * l.items[j] * rows * D : 0);
+      l.item_lse[j] = take(n > 1 ? sizeof(float) * l.items[j] * rows : 0);
+      l.pieces[j] = take(sizeof(int2) * (n > 1 ? l.items[j] : l.split_items));
+    }
   }
-  p.pieces = at;
-  p.total = p.pieces + align256(sizeof(int2) * p.split_items);
+  p.total = at;
   return p;
 }
 
@@ -952,51 +764,67 @@ int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, c
   int rc = make_sides(a, prefix, s, &n);
   if (rc) return rc;
   const FwPlan p = fw_plan(a, s, n);
-  FwArgs A = {};
-  XMap m[4];
   char* w = static_cast<char*>(ws);
   const int64_t D = a->head_dim;
-  for (int i = 0; i < n; ++i) {
-    FwSide& S = A.side[i];
-    S.s = s[i];
-    S.row_tiles = static_cast<int>((side_rows(s[i]) + kFwRows - 1) / kFwRows);
-    S.items = S.row_tiles * s[i].nb * s[i].hkv;
-    S.by_T = fast_div(s[i].T);
-    S.by_G = fast_div(s[i].G);
-    rc = make_xmap(&m[2 * i], s[i].k, D, s[i].klen, s[i].hkv, s[i].nb, s[i].k_t, s[i].k_h, s[i].k_b, 128);
-    if (rc) return rc;
-    rc = make_xmap(&m[2 * i + 1], s[i].v, D, s[i].klen, s[i].hkv, s[i].nb, s[i].v_t, s[i].v_h, s[i].v_b, 128);
-    if (rc) return rc;
-    S.mul_kh = m[2 * i].mul_h;
-    S.mul_kb = m[2 * i].mul_b;
-    S.mul_vh = m[2 * i + 1].mul_h;
-    S.mul_vb = m[2 * i + 1].mul_b;
-  }
-  for (int i = 2 * n; i < 4; ++i) m[i] = m[i - 2];
-  A.sides = n;
-  A.D = static_cast<int>(D);
-  A.whole = p.whole;
-  A.slot_rows = p.slot_rows;
-  A.slots = reinterpret_cast<float*>(w + p.o[0]);
-  A.slot_lse = reinterpret_cast<float*>(w + p.lse[0]);
-  for (int i = 0; i < 2; ++i) {
-    A.item_slots[i] = reinterpret_cast<float*>(w + p.o[i + 1]);
-    A.item_lse[i] = reinterpret_cast<float*>(w + p.lse[i + 1]);
-    const int64_t R = i < n ? side_rows(s[i]) : 0;
-    A.item_rows[i] = static_cast<int>(R < kFwRows ? R : kFwRows);
-  }
-  A.pieces = reinterpret_cast<int2*>(w + p.pieces);
-  A.out = static_cast<__nv_bfloat16*>(a->out);
-  A.lse = a->lse;
+  FwArgs J = {};  // the call as a whole, for the join
+  J.sides = n;
+  J.D = static_cast<int>(D);
+  J.out = static_cast<__nv_bfloat16*>(a->out);
+  J.lse = a->lse;
   // a scale of 0 (or too small for fp32) stays above 0, so that a hidden score of -inf stays -inf
-  A.scale_log2 = fmaxf(static_cast<float>(fabs(a->scale) * 1.4426950408889634), 1e-37f);
-  A.q_flip = a->scale < 0 ? 0x80008000u : 0u;
-  rc = D <= 64 ? fw_launch<64>(A, m, p.grid, st) : fw_launch<128>(A, m, p.grid, st);
-  if (rc) return rc;
-  const int64_t last = side_rows(s[n - 1]), rows = last < kFwRows ? last : kFwRows;
-  if (n == 1 && p.split_items == 0) return TRNSPARSE_OK;
-  const dim3 grid(n == 1 ? p.split_items : A.side[1].items, static_cast<unsigned>((rows + 31) / 32));
-  cudaError_t e = launch_pdl(xattn_join_kernel, grid, dim3(256), 0, st, A, p.grid);
+  J.scale_log2 = fmaxf(static_cast<float>(fabs(a->scale) * 1.4426950408889634), 1e-37f);
+  J.q_flip = a->scale < 0 ? 0x80008000u : 0u;
+  J.keep = n > 1;
+  for (int i = 0; i < p.launches; ++i) {
+    const FwLaunch& l = p.l[i];
+    FwArgs A = J;
+    A.sides = l.sides;
+    A.whole = l.whole;
+    for (int j = 0; j < l.sides; ++j) {
+      FwSide& S = A.side[j];
+      S.s = s[l.side[j]];
+      S.tile_rows = l.few ? kFewRows : kFwRows;
+      S.key_shift = l.few ? kFewKeyShift : kFwKeyShift;
+      const int64_t R = side_rows(S.s);
+      S.row_tiles = static_cast<int>((R + S.tile_rows - 1) / S.tile_rows);
+      S.items = static_cast<int>(l.items[j]);
+      S.by_T = fast_div(S.s.T);
+      S.by_G = fast_div(S.s.G);
+      S.slots = reinterpret_cast<float*>(w + l.o);
+      S.slot_lse = reinterpret_cast<float*>(w + l.lse);
+      S.slot_rows = l.slot_rows;
+      S.item_slots = reinterpret_cast<float*>(w + l.item_o[j]);
+      S.item_lse = reinterpret_cast<float*>(w + l.item_lse[j]);
+      S.item_rows = static_cast<int>(R < S.tile_rows ? R : S.tile_rows);
+      S.pieces = reinterpret_cast<int2*>(w + l.pieces[j]);
+      S.first = l.whole * l.grid;
+    }
+    if (l.few) {
+      rc = few_rows_launch(A, l.grid, st);
+    } else {
+      A.item_cost = kFwItemCost;
+      XMap m[4];
+      for (int j = 0; j < l.sides && !rc; ++j) {
+        FwSide& S = A.side[j];
+        const XSide& x = S.s;
+        rc = make_xmap(&m[2 * j], x.k, D, x.klen, x.hkv, x.nb, x.k_t, x.k_h, x.k_b, 128);
+        if (!rc) rc = make_xmap(&m[2 * j + 1], x.v, D, x.klen, x.hkv, x.nb, x.v_t, x.v_h, x.v_b, 128);
+        S.mul_kh = m[2 * j].mul_h;
+        S.mul_kb = m[2 * j].mul_b;
+        S.mul_vh = m[2 * j + 1].mul_h;
+        S.mul_vb = m[2 * j + 1].mul_b;
+      }
+      for (int j = 2 * l.sides; j < 4; ++j) m[j] = m[j - 2];
+      if (!rc) rc = D <= 64 ? fw_launch<64>(A, m, l.grid, st) : fw_launch<128>(A, m, l.grid, st);
+    }
+    if (rc) return rc;
+    for (int j = 0; j < l.sides; ++j) J.side[l.side[j]] = A.side[j];
+  }
+  const FwLaunch& l = p.l[p.launches - 1];
+  const FwSide& S = J.side[n - 1];
+  const int blocks = n == 1 ? l.split_items : S.items;
+  if (blocks == 0) return TRNSPARSE_OK;
+  cudaError_t e = launch_pdl(xattn_join_kernel, dim3(blocks, (S.item_rows + 31) / 32), dim3(256), 0, st, J);
   if (e != cudaSuccess) return cuda_status(e, "attention (tensor cores): join");
   return debug_sync(st, "attention (tensor cores): join");
 }
