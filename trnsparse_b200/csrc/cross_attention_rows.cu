@@ -340,17 +340,24 @@ xattn_rows_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_constant
     }
     if (!ok) atomicExch(&B.abort_flag, 1);
   }
+  // launched beside the launch before it: what follows this kernel needs that one's results too
+  grid_dep_wait();
 }
 
 template <int HD>
-int fr_launch(const FwArgs& A, const XMap (&m)[4], int grid, cudaStream_t st) {
+int fr_launch(const FwArgs& A, const XMap (&m)[4], int grid, bool behind, cudaStream_t st) {
   using Lay = FrLayout<HD>;
   auto kern = xattn_rows_kernel<HD>;
   static unsigned long long done = 0;  // a bit per device; setting the attribute again is harmless
   int rc = allow_smem(kern, Lay::kSmem, &done, "attention (few rows): set smem");
   if (rc) return rc;
-  kern<<<grid, kFrThreads, Lay::kSmem, st>>>(m[0].map, m[1].map, m[2].map, m[3].map, A);
-  TSB_CHECK_LAUNCH("attention (few rows) launch");
+  if (behind) {
+    cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kFrThreads), Lay::kSmem, st, m[0].map, m[1].map, m[2].map, m[3].map, A);
+    if (e != cudaSuccess) return cuda_status(e, "attention (few rows) launch");
+  } else {
+    kern<<<grid, kFrThreads, Lay::kSmem, st>>>(m[0].map, m[1].map, m[2].map, m[3].map, A);
+    TSB_CHECK_LAUNCH("attention (few rows) launch");
+  }
   return debug_sync(st, "attention (few rows)");
 }
 
@@ -358,7 +365,7 @@ int fr_launch(const FwArgs& A, const XMap (&m)[4], int grid, cudaStream_t st) {
 
 int few_rows_grid() { return 2 * sm_count(); }
 
-int few_rows_launch(const FwArgs& args, int grid, cudaStream_t st) {
+int few_rows_launch(const FwArgs& args, int grid, bool behind, cudaStream_t st) {
   FwArgs A = args;
   A.item_cost = kFrItemCost;
   XMap m[4];
@@ -374,7 +381,7 @@ int few_rows_launch(const FwArgs& args, int grid, cudaStream_t st) {
     S.mul_vb = m[2 * j + 1].mul_b;
   }
   for (int j = 2 * A.sides; j < 4; ++j) m[j] = m[j - 2];
-  return A.D <= 64 ? fr_launch<64>(A, m, grid, st) : fr_launch<128>(A, m, grid, st);
+  return A.D <= 64 ? fr_launch<64>(A, m, grid, behind, st) : fr_launch<128>(A, m, grid, behind, st);
 }
 
 }  // namespace tsb

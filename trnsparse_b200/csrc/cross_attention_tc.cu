@@ -51,6 +51,7 @@ constexpr int kFwKeys = 128, kFwKeyShift = 7;
 constexpr float kFwLazy = 8.f;
 // 1, 2, 3 measured: 45.4, 43.5, 42.9 us in a decode over 8 ragged sequences, 170, 167, 175 us in prompts of 777 tokens
 constexpr int kFwItemCost = 2;
+constexpr int kFwLeast = 8;
 
 template <int HD>
 struct FwLayout {
@@ -121,6 +122,8 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
     g = B.seg[i % kFwSegs];
     return true;
   };
+
+  grid_dep_launch();  // the own keys' launch of a two-sided call may take SMs as they come free
 
   if (warp == 10) {
     // ---------------- the list of segments
@@ -616,30 +619,37 @@ __global__ void __launch_bounds__(256) xattn_join_kernel(const __grid_constant__
   const int q4 = A.D / 4;
   for (int i = threadIdx.x; i < rows * q4; i += 256) {
     const int c4 = i / rows, r = i - c4 * rows;
+    // Twice over the pieces, first their log-sum-exps for the maximum, then the sums: no load waits for another.
     float mx = -INFINITY, den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](const float* slots, const float* lse, int stride, int64_t slot, int at) {
-      const float ls = lse[slot * stride + at];
+    auto pieces = [&](int2 q, const FwSide& sd, int it, int at, auto&& f) {
+      if (A.sides > 1 && q.x == q.y) {
+        f(sd.item_slots, sd.item_lse, sd.item_rows, static_cast<int64_t>(it), at);
+      } else {
+#pragma unroll 4
+        for (int c = q.x; c <= q.y; ++c) f(sd.slots, sd.slot_lse, sd.slot_rows, 2ll * c + (c == q.x ? 1 : 0), at);
+      }
+    };
+    auto all_pieces = [&](auto&& f) {
+      if (A.sides > 1) {
+        const FwSide& P = A.side[0];
+        const int64_t pr = static_cast<int64_t>(bi) * S.s.G * S.s.T + row0 + r;
+        const int prt = static_cast<int>(pr / P.tile_rows), pi = h * P.row_tiles + prt;
+        pieces(P.pieces[pi], P, pi, static_cast<int>(pr - static_cast<int64_t>(prt) * P.tile_rows), f);
+      }
+      pieces(p, S, item, blockIdx.y * 32 + r, f);
+    };
+    all_pieces([&](const float*, const float* lse, int stride, int64_t slot, int at) {
+      mx = max3_nan(mx, mx, lse[slot * stride + at]);
+    });
+    const float base = mx == -INFINITY ? 0.f : mx;
+    all_pieces([&](const float* slots, const float* lse, int stride, int64_t slot, int at) {
+      const float w = exp2f(lse[slot * stride + at] - base);
       const float4 o = *reinterpret_cast<const float4*>(slots + slot * stride * A.D +
                                                         (static_cast<int64_t>(c4) * stride + at) * 4);
-      if (ls == -INFINITY) return;
-      const float mn = fmaxf(mx, ls), c = exp2f(mx - mn), w = exp2f(ls - mn);
-      den = den * c + w;
-      acc = make_float4(acc.x * c + w * o.x, acc.y * c + w * o.y, acc.z * c + w * o.z, acc.w * c + w * o.w);
-      mx = mn;
-    };
-    auto add_item = [&](int2 q, const FwSide& sd, int it, int at) {
-      if (A.sides > 1 && q.x == q.y) add(sd.item_slots, sd.item_lse, sd.item_rows, it, at);
-      else
-        for (int c = q.x; c <= q.y; ++c) add(sd.slots, sd.slot_lse, sd.slot_rows, 2ll * c + (c == q.x ? 1 : 0), at);
-    };
-    if (A.sides > 1) {
-      const FwSide& P = A.side[0];
-      const int64_t pr = static_cast<int64_t>(bi) * S.s.G * S.s.T + row0 + r;
-      const int prt = static_cast<int>(pr / P.tile_rows), pi = h * P.row_tiles + prt;
-      add_item(P.pieces[pi], P, pi, static_cast<int>(pr - static_cast<int64_t>(prt) * P.tile_rows));
-    }
-    add_item(p, S, item, blockIdx.y * 32 + r);
+      den += w;
+      acc = make_float4(fmaf(w, o.x, acc.x), fmaf(w, o.y, acc.y), fmaf(w, o.z, acc.z), fmaf(w, o.w, acc.w));
+    });
     const float inv = den == 0.f ? 0.f : 1.f / den;
     *reinterpret_cast<uint2*>(&tile[r][c4 * 4]) =
         make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
@@ -689,7 +699,10 @@ FwPlan fw_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n) {
       tiles += l.items[j] * ((x.klen + (1ll << shift) - 1) >> shift);
       most = most > R ? most : R;
     }
-    const int64_t full = l.few ? few_rows_grid() : sm_count();
+    // Beside the own keys' launch the prefix's takes as many SMs as give a CTA kFwLeast tiles: each of its pieces is
+    // written and joined (256 rows in fp32), and the other launch has work for the rest of the SMs.
+    const int64_t least = tiles / kFwLeast > 0 ? tiles / kFwLeast : 1, sms = sm_count();
+    const int64_t full = l.few ? few_rows_grid() : p.launches == 2 && least < sms ? least : sms;
     l.grid = static_cast<int>(tiles < full ? (tiles > 0 ? tiles : 1) : full);
     // One side: whole items for all but the last round (items of one length), or the last one to two rounds, which
     // then even out what unequal lengths left.
@@ -800,7 +813,7 @@ int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, c
       S.first = l.whole * l.grid;
     }
     if (l.few) {
-      rc = few_rows_launch(A, l.grid, st);
+      rc = few_rows_launch(A, l.grid, i > 0, st);
     } else {
       A.item_cost = kFwItemCost;
       XMap m[4];

@@ -232,10 +232,11 @@ __device__ __forceinline__ void fw_note_pieces(const FwArgs& A, const FwCursor& 
 
 }  // namespace
 
-// The few-rows form (cross_attention_rows.cu): all sides of `A` have items of at most kFewRows rows.
+// The few-rows form (cross_attention_rows.cu): all sides of `A` have items of at most kFewRows rows. `behind`: it
+// may run beside the launch before it in the stream, whose results it does not need, and ends after it.
 constexpr int kFewRows = 16;
 constexpr int kFewKeyShift = 6;
 int few_rows_grid();
-int few_rows_launch(const FwArgs& A, int grid, cudaStream_t st);
+int few_rows_launch(const FwArgs& A, int grid, bool behind, cudaStream_t st);
 
 }  // namespace tsb
