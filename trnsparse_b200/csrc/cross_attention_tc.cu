@@ -601,67 +601,84 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
   }
 }
 
-// Joins the pieces of every row of the split part, 32 rows of an item a block: a thread per (row, 4 elements),
-// rows fastest, as the slots are laid out; the rows then leave through shared memory as whole lines. One side:
-// blocks walk its split items (those that one CTA finished are done). Two sides: blocks walk the own side's items,
-// whose rows r of sequence b are rows b G T + r of the prefix's item of that key head.
-__global__ void __launch_bounds__(256) xattn_join_kernel(const __grid_constant__ FwArgs A) {
-  __shared__ __align__(16) __nv_bfloat16 tile[32][136];
-  grid_dep_wait();
+// Joins the pieces of every row of the split part. A thread has 4 elements of a row, rows fastest, as the slots are
+// laid out (whole lines for 32 rows); a block has up to 32 rows and 8 groups of 4 elements. One side: rows of a split item (items that one CTA finished are done). Two sides:
+// 32 packed rows of the prefix's items of a key head, which are rows of one or more sequences' own items.
+__global__ void __launch_bounds__(256, 2) xattn_join_kernel(const __grid_constant__ FwArgs A) {
+  const FwSide& L = A.side[0];  // whose rows the blocks walk
   const FwSide& S = A.side[A.sides - 1];
-  const int item = blockIdx.x + S.first, per = S.s.hkv * S.row_tiles;
-  const int bi = item / per, rem = item - bi * per, h = rem / S.row_tiles, rt = rem - h * S.row_tiles;
-  const int64_t R = side_rows(S.s), row0 = static_cast<int64_t>(rt) * S.tile_rows + blockIdx.y * 32;
-  const int rows = static_cast<int>(min(static_cast<int64_t>(32), min(R, static_cast<int64_t>(rt + 1) * S.tile_rows) - row0));
-  const int n = fw_tiles(S, bi);
-  const int2 p = n > 0 ? S.pieces[blockIdx.x] : make_int2(0, -1);
-  if (rows <= 0 || (A.sides == 1 && n > 0 && p.x == p.y)) return;
-  const int q4 = A.D / 4;
-  for (int i = threadIdx.x; i < rows * q4; i += 256) {
-    const int c4 = i / rows, r = i - c4 * rows;
-    // Twice over the pieces, first their log-sum-exps for the maximum, then the sums: no load waits for another.
+  const int item = A.sides == 1 ? blockIdx.x + L.first : blockIdx.x;
+  const int per = L.s.hkv * L.row_tiles, bi = item / per, rem = item - bi * per, h = rem / L.row_tiles;
+  const int rt = rem - h * L.row_tiles;
+  const int64_t R = side_rows(L.s), row0 = static_cast<int64_t>(rt) * L.tile_rows + blockIdx.y * 32;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(32), min(R, static_cast<int64_t>(rt + 1) * L.tile_rows) - row0));
+  if (rows <= 0) return;
+  const int c0 = blockIdx.z * 8, cw = min(8, A.D / 4 - c0);
+  grid_dep_wait();
+  const int n = fw_tiles(L, bi);
+  const int2 p = n > 0 ? L.pieces[item - L.first] : make_int2(0, -1);
+  if (A.sides == 1 && n > 0 && p.x == p.y) return;
+  for (int i = threadIdx.x; i < rows * cw; i += blockDim.x) {
+    const int c = i / rows, r = i - c * rows, c4 = c0 + c;
+    const int64_t row = row0 + r;
     float mx = -INFINITY, den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto pieces = [&](int2 q, const FwSide& sd, int it, int at, auto&& f) {
-      if (A.sides > 1 && q.x == q.y) {
-        f(sd.item_slots, sd.item_lse, sd.item_rows, static_cast<int64_t>(it), at);
-      } else {
-#pragma unroll 4
-        for (int c = q.x; c <= q.y; ++c) f(sd.slots, sd.slot_lse, sd.slot_rows, 2ll * c + (c == q.x ? 1 : 0), at);
+    // Eight pieces at a time, their log-sum-exps and values in flight together: a load takes about a microsecond
+    // here, so what counts is how many follow one another.
+    auto add = [&](const float* slots, const float* lse, int stride, int at, int count, auto&& slot_of) {
+      for (int k0 = 0; k0 < count; k0 += 8) {
+        float ls[8];
+        float4 o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          ls[k] = -INFINITY;
+          o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (k0 + k < count) {
+            const int64_t slot = slot_of(k0 + k);
+            ls[k] = lse[slot * stride + at];
+            o[k] = *reinterpret_cast<const float4*>(slots + slot * stride * A.D +
+                                                    (static_cast<int64_t>(c4) * stride + at) * 4);
+          }
+        }
+        float mn = mx;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mn = max3_nan(mn, mn, ls[k]);
+        const float base = mn == -INFINITY ? 0.f : mn, c = exp2f(mx - base);
+        den *= c;
+        acc = make_float4(acc.x * c, acc.y * c, acc.z * c, acc.w * c);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float w = exp2f(ls[k] - base);
+          den += w;
+          acc = make_float4(fmaf(w, o[k].x, acc.x), fmaf(w, o[k].y, acc.y), fmaf(w, o[k].z, acc.z), fmaf(w, o[k].w, acc.w));
+        }
+        mx = mn;
       }
     };
-    auto all_pieces = [&](auto&& f) {
-      if (A.sides > 1) {
-        const FwSide& P = A.side[0];
-        const int64_t pr = static_cast<int64_t>(bi) * S.s.G * S.s.T + row0 + r;
-        const int prt = static_cast<int>(pr / P.tile_rows), pi = h * P.row_tiles + prt;
-        pieces(P.pieces[pi], P, pi, static_cast<int>(pr - static_cast<int64_t>(prt) * P.tile_rows), f);
-      }
-      pieces(p, S, item, blockIdx.y * 32 + r, f);
+    auto pieces = [&](int2 q, const FwSide& sd, int it, int at) {
+      const bool single = A.sides > 1 && q.x == q.y;
+      add(single ? sd.item_slots : sd.slots, single ? sd.item_lse : sd.slot_lse, single ? sd.item_rows : sd.slot_rows, at,
+          q.y - q.x + 1, [&](int k) { return single ? static_cast<int64_t>(it) : 2ll * (q.x + k) + (k == 0 ? 1 : 0); });
     };
-    all_pieces([&](const float*, const float* lse, int stride, int64_t slot, int at) {
-      mx = max3_nan(mx, mx, lse[slot * stride + at]);
-    });
-    const float base = mx == -INFINITY ? 0.f : mx;
-    all_pieces([&](const float* slots, const float* lse, int stride, int64_t slot, int at) {
-      const float w = exp2f(lse[slot * stride + at] - base);
-      const float4 o = *reinterpret_cast<const float4*>(slots + slot * stride * A.D +
-                                                        (static_cast<int64_t>(c4) * stride + at) * 4);
-      den += w;
-      acc = make_float4(fmaf(w, o.x, acc.x), fmaf(w, o.y, acc.y), fmaf(w, o.z, acc.z), fmaf(w, o.w, acc.w));
-    });
+    int own_item = 0, own_at = 0;
+    int2 own = make_int2(0, -1);
+    XRow x = fw_row(L, row);
+    int ob = bi;
+    if (A.sides > 1) {
+      // packed row (b, g, t) of the prefix is row (g, t) of sequence b
+      const int orow = x.g * S.s.T + x.t, ort = orow / S.tile_rows;
+      ob = x.b2;
+      x.b2 = 0;
+      own_item = (ob * S.s.hkv + h) * S.row_tiles + ort;
+      own_at = orow - ort * S.tile_rows;
+      if (side_len(S.s, ob) > 0) own = S.pieces[own_item];
+    }
+    pieces(p, L, item, blockIdx.y * 32 + r);
+    if (A.sides > 1) pieces(own, S, own_item, own_at);
     const float inv = den == 0.f ? 0.f : 1.f / den;
-    *reinterpret_cast<uint2*>(&tile[r][c4 * 4]) =
-        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-    if (A.lse != nullptr && c4 == 0)
-      A.lse[flat_row(S.s, bi, h, side_row(S.s, row0 + r))] = den == 0.f ? -INFINITY : mx + log2f(den);
-  }
-  __syncthreads();
-  const int q8 = A.D / 8;
-  for (int i = threadIdx.x; i < rows * q8; i += 256) {
-    const int r = i / q8, c = i - r * q8;
-    *reinterpret_cast<uint4*>(A.out + o_offset(S.s, bi, h, side_row(S.s, row0 + r)) + c * 8) =
-        *reinterpret_cast<const uint4*>(&tile[r][c * 8]);
+    const uint2 v = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<uint2*>(A.out + o_offset(S.s, ob, h, x) + c4 * 4) = v;
+    if (A.lse != nullptr && c4 == 0) A.lse[flat_row(S.s, ob, h, x)] = den == 0.f ? -INFINITY : mx + log2f(den);
   }
 }
 
@@ -834,10 +851,12 @@ int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, c
     for (int j = 0; j < l.sides; ++j) J.side[l.side[j]] = A.side[j];
   }
   const FwLaunch& l = p.l[p.launches - 1];
-  const FwSide& S = J.side[n - 1];
-  const int blocks = n == 1 ? l.split_items : S.items;
+  const FwSide& W = J.side[0];
+  const int blocks = n == 1 ? l.split_items : W.items;
   if (blocks == 0) return TRNSPARSE_OK;
-  cudaError_t e = launch_pdl(xattn_join_kernel, dim3(blocks, (S.item_rows + 31) / 32), dim3(256), 0, st, J);
+  const int threads = W.item_rows >= 32 ? 256 : (W.item_rows * 8 + 31) & ~31;
+  cudaError_t e = launch_pdl(xattn_join_kernel, dim3(blocks, (W.item_rows + 31) / 32, (a->head_dim / 4 + 7) / 8),
+                             dim3(threads), 0, st, J);
   if (e != cudaSuccess) return cuda_status(e, "attention (tensor cores): join");
   return debug_sync(st, "attention (tensor cores): join");
 }
