@@ -246,15 +246,24 @@ __global__ void __launch_bounds__(256) combine_pieces_kernel(const float* __rest
   float acc[8], den = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-  for (int p = 0; p < pieces; ++p) {
-    const float lp = part_lse[p * rows + row];
-    if (lp == -INFINITY) continue;
-    const float w = exp2f(lp - mu);
-    den += w;
-    const float* po = part_o + (p * rows + row) * D;
+  // four pieces' loads in flight together
+  for (int p0 = 0; p0 < pieces; p0 += 4) {
+    float lp[4], v[4][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < D) acc[i] = fmaf(w, po[lane + 32 * i], acc[i]);
+    for (int k = 0; k < 4; ++k) {
+      const bool in = p0 + k < pieces;
+      lp[k] = in ? part_lse[(p0 + k) * rows + row] : -INFINITY;
+      const float* po = part_o + ((p0 + k) * rows + row) * D;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[k][i] = in && lane + 32 * i < D ? po[lane + 32 * i] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float w = exp2f(lp[k] - mu);  // an empty piece holds zeros and weighs 0
+      den += w;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, v[k][i], acc[i]);
+    }
   }
   const int t = static_cast<int>(row % Tq);
   const int64_t bh = row / Tq, b = bh / Hq, h = bh - b * Hq;
@@ -279,12 +288,12 @@ SimtPlan simt_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n
   for (int i = 0; i < n; ++i) most = most > side_rows(s[i]) ? most : side_rows(s[i]);
   // 16-row CTAs where a 64-row tile would be mostly padding
   p.bm = most <= 32 ? 16 : 64;
-  const int64_t want = 2ll * sm_count();
+  const int64_t want = 3ll * sm_count();
   for (int i = 0; i < n; ++i) {
     p.row_tiles[i] = static_cast<int>((side_rows(s[i]) + p.bm - 1) / p.bm);
     const int64_t ctas = static_cast<int64_t>(p.row_tiles[i]) * s[i].nb * s[i].hkv;
     const int64_t tiles = (s[i].klen + kXKeys - 1) / kXKeys;
-    // ranges of at least two tiles, as many as fill the GPU twice
+    // ranges of at least two tiles, as many as fill the GPU with two CTAs an SM
     int64_t splits = ctas > 0 ? (want + ctas - 1) / ctas : 1;
     const int64_t cap = tiles / 2;
     splits = splits < cap ? splits : cap;
