@@ -604,7 +604,12 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
 // Joins the pieces of every row of the split part. A thread has 4 elements of a row, rows fastest, as the slots are
 // laid out (whole lines for 32 rows); a block has up to 32 rows and 8 groups of 4 elements. One side: rows of a split item (items that one CTA finished are done). Two sides:
 // 32 packed rows of the prefix's items of a key head, which are rows of one or more sequences' own items.
-__global__ void __launch_bounds__(256, 2) xattn_join_kernel(const __grid_constant__ FwArgs A) {
+// BATCH pieces of a thread are in flight together (a load takes about a microsecond here, so what counts is how many
+// follow one another): 8 where an item has few rows and many pieces, or a prefix's; 2 where large items were cut
+// once, so that more threads fit on an SM.
+template <int BATCH>
+__global__ void __launch_bounds__(256, BATCH > 2 ? 2 : 5) xattn_join_kernel(const __grid_constant__ FwArgs A) {
+  __shared__ __align__(16) uint2 tile[32][8];
   const FwSide& L = A.side[0];  // whose rows the blocks walk
   const FwSide& S = A.side[A.sides - 1];
   const int item = A.sides == 1 ? blockIdx.x + L.first : blockIdx.x;
@@ -623,14 +628,12 @@ __global__ void __launch_bounds__(256, 2) xattn_join_kernel(const __grid_constan
     const int64_t row = row0 + r;
     float mx = -INFINITY, den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    // Eight pieces at a time, their log-sum-exps and values in flight together: a load takes about a microsecond
-    // here, so what counts is how many follow one another.
     auto add = [&](const float* slots, const float* lse, int stride, int at, int count, auto&& slot_of) {
-      for (int k0 = 0; k0 < count; k0 += 8) {
-        float ls[8];
-        float4 o[8];
+      for (int k0 = 0; k0 < count; k0 += BATCH) {
+        float ls[BATCH];
+        float4 o[BATCH];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < BATCH; ++k) {
           ls[k] = -INFINITY;
           o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (k0 + k < count) {
@@ -642,12 +645,12 @@ __global__ void __launch_bounds__(256, 2) xattn_join_kernel(const __grid_constan
         }
         float mn = mx;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) mn = max3_nan(mn, mn, ls[k]);
+        for (int k = 0; k < BATCH; ++k) mn = max3_nan(mn, mn, ls[k]);
         const float base = mn == -INFINITY ? 0.f : mn, c = exp2f(mx - base);
         den *= c;
         acc = make_float4(acc.x * c, acc.y * c, acc.z * c, acc.w * c);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < BATCH; ++k) {
           const float w = exp2f(ls[k] - base);
           den += w;
           acc = make_float4(fmaf(w, o[k].x, acc.x), fmaf(w, o[k].y, acc.y), fmaf(w, o[k].z, acc.z), fmaf(w, o[k].w, acc.w));
@@ -677,8 +680,22 @@ __global__ void __launch_bounds__(256, 2) xattn_join_kernel(const __grid_constan
     if (A.sides > 1) pieces(own, S, own_item, own_at);
     const float inv = den == 0.f ? 0.f : 1.f / den;
     const uint2 v = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-    *reinterpret_cast<uint2*>(A.out + o_offset(S.s, ob, h, x) + c4 * 4) = v;
+    if (rows == 32) tile[r][c] = v;
+    else *reinterpret_cast<uint2*>(A.out + o_offset(S.s, ob, h, x) + c4 * 4) = v;
     if (A.lse != nullptr && c4 == 0) A.lse[flat_row(S.s, ob, h, x)] = den == 0.f ? -INFINITY : mx + log2f(den);
+  }
+  if (rows < 32) return;
+  __syncthreads();
+  // 32 rows leave in 64 contiguous bytes each
+  for (int i = threadIdx.x; i < 32 * (cw / 2); i += blockDim.x) {
+    const int r = i / (cw / 2), u = i - r * (cw / 2);
+    XRow x = fw_row(L, row0 + r);
+    int ob = bi;
+    if (A.sides > 1) {
+      ob = x.b2;
+      x.b2 = 0;
+    }
+    *reinterpret_cast<uint4*>(A.out + o_offset(S.s, ob, h, x) + c0 * 4 + u * 8) = *reinterpret_cast<const uint4*>(&tile[r][u * 2]);
   }
 }
 
@@ -855,8 +872,8 @@ int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, c
   const int blocks = n == 1 ? l.split_items : W.items;
   if (blocks == 0) return TRNSPARSE_OK;
   const int threads = W.item_rows >= 32 ? 256 : (W.item_rows * 8 + 31) & ~31;
-  cudaError_t e = launch_pdl(xattn_join_kernel, dim3(blocks, (W.item_rows + 31) / 32, (a->head_dim / 4 + 7) / 8),
-                             dim3(threads), 0, st, J);
+  auto kern = n == 1 && W.item_rows >= 32 ? xattn_join_kernel<2> : xattn_join_kernel<8>;
+  cudaError_t e = launch_pdl(kern, dim3(blocks, (W.item_rows + 31) / 32, (a->head_dim / 4 + 7) / 8), dim3(threads), 0, st, J);
   if (e != cudaSuccess) return cuda_status(e, "attention (tensor cores): join");
   return debug_sync(st, "attention (tensor cores): join");
 }
