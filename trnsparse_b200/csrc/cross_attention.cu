@@ -17,6 +17,7 @@
 // head_dim 128 and one loads while the other computes. BM = 16 serves few rows
 // (decoding), 64 the rest. When there are fewer CTAs than SMs the keys are cut
 // into ranges, each writing (O, log-sum-exp) of its part, joined afterwards.
+#include "tc_common.cuh"
 #include "xattn.cuh"
 
 namespace tsb {
@@ -87,6 +88,7 @@ __global__ void __launch_bounds__(NT) xattn_simt_kernel(const XKernel A) {
   const T* vp = static_cast<const T*>(s.v) + bi * s.v_b + h * s.v_h;
   const uint8_t* mask = s.mask ? s.mask + bi * s.mask_stride : nullptr;
   const bool vec = A.vec;
+  grid_dep_launch();  // the other side's launch, which needs none of this one's results, may run beside it
 
   for (int i = tid; i < BM * DC * 16; i += NT) {
     const int row = i / (DC * 16), d = (i - row * (DC * 16)) * 4;
@@ -227,6 +229,7 @@ __global__ void __launch_bounds__(NT) xattn_simt_kernel(const XKernel A) {
       if (A.lse != nullptr && tx == 0) A.lse[fr] = lse;
     }
   }
+  grid_dep_wait();  // ends after the launch it ran beside: what follows needs both
 }
 
 // One warp per row.
@@ -293,10 +296,9 @@ SimtPlan simt_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n
     p.row_tiles[i] = static_cast<int>((side_rows(s[i]) + p.bm - 1) / p.bm);
     const int64_t ctas = static_cast<int64_t>(p.row_tiles[i]) * s[i].nb * s[i].hkv;
     const int64_t tiles = (s[i].klen + kXKeys - 1) / kXKeys;
-    // ranges of at least two tiles, as many as fill the GPU with two CTAs an SM
+    // as many ranges as fill the GPU with two CTAs an SM
     int64_t splits = ctas > 0 ? (want + ctas - 1) / ctas : 1;
-    const int64_t cap = tiles / 2;
-    splits = splits < cap ? splits : cap;
+    splits = splits < tiles ? splits : tiles;
     if (splits > 128) splits = 128;
     if (splits < 1) splits = 1;
     const int64_t per = tiles > 0 ? (tiles + splits - 1) / splits : 1;
@@ -308,27 +310,31 @@ SimtPlan simt_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n
 }
 
 template <typename T, int BM, int NT, int DC>
-int simt_launch(const XKernel& A, int splits, cudaStream_t st) {
+int simt_launch(const XKernel& A, int splits, bool behind, cudaStream_t st) {
   constexpr size_t smem = sizeof(float) * (static_cast<size_t>(BM + kXKeys) * (DC * 64 + 4) + BM * (kXKeys + 4));
   auto kern = xattn_simt_kernel<T, BM, NT, DC>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return cuda_status(e, "attention: set smem");
   const dim3 grid(static_cast<unsigned>(A.row_tiles) * A.s.nb * A.s.hkv, splits);
+  if (behind) {
+    e = launch_pdl(kern, grid, dim3(NT), smem, st, A);
+    return e == cudaSuccess ? TRNSPARSE_OK : cuda_status(e, "attention (CUDA cores) launch");
+  }
   kern<<<grid, NT, smem, st>>>(A);
   TSB_CHECK_LAUNCH("attention (CUDA cores) launch");
   return TRNSPARSE_OK;
 }
 
 template <typename T>
-int simt_dispatch(const XKernel& A, int bm, int dc, int splits, cudaStream_t st) {
+int simt_dispatch(const XKernel& A, int bm, int dc, int splits, bool behind, cudaStream_t st) {
   if (bm == 16) {
-    if (dc == 1) return simt_launch<T, 16, 128, 1>(A, splits, st);
-    if (dc == 2) return simt_launch<T, 16, 128, 2>(A, splits, st);
-    return simt_launch<T, 16, 128, 4>(A, splits, st);
+    if (dc == 1) return simt_launch<T, 16, 128, 1>(A, splits, behind, st);
+    if (dc == 2) return simt_launch<T, 16, 128, 2>(A, splits, behind, st);
+    return simt_launch<T, 16, 128, 4>(A, splits, behind, st);
   }
-  if (dc == 1) return simt_launch<T, 64, 256, 1>(A, splits, st);
-  if (dc == 2) return simt_launch<T, 64, 256, 2>(A, splits, st);
-  return simt_launch<T, 64, 256, 4>(A, splits, st);
+  if (dc == 1) return simt_launch<T, 64, 256, 1>(A, splits, behind, st);
+  if (dc == 2) return simt_launch<T, 64, 256, 2>(A, splits, behind, st);
+  return simt_launch<T, 64, 256, 4>(A, splits, behind, st);
 }
 
 // Every base and stride of the call's operands is a multiple of four elements.
@@ -369,8 +375,8 @@ int simt_forward(const trnsparse_attention_args* a, bool prefix, void* ws, cudaS
     A.vec = four_aligned(a);
     A.scale = static_cast<float>(a->scale);
     A.scale_log2 = static_cast<float>(a->scale * 1.4426950408889634);
-    rc = a->dtype == TRNSPARSE_F32 ? simt_dispatch<float>(A, p.bm, p.dc, p.splits[i], st)
-                                   : simt_dispatch<__nv_bfloat16>(A, p.bm, p.dc, p.splits[i], st);
+    rc = a->dtype == TRNSPARSE_F32 ? simt_dispatch<float>(A, p.bm, p.dc, p.splits[i], i > 0, st)
+                                   : simt_dispatch<__nv_bfloat16>(A, p.bm, p.dc, p.splits[i], i > 0, st);
     if (rc) return rc;
     piece += p.splits[i];
   }
