@@ -13,12 +13,10 @@
 // What bounds it: fp32 FMA. A CTA takes BM packed rows and walks the keys in
 // tiles of 64; a thread forms an RM x 4 tile of scores and an RM x 4 DC tile of
 // the output from float4 reads of shared memory (about four FMA per 16 bytes
-// read). K and V take turns in one buffer, so two CTAs fit on an SM up to
-// head_dim 128 and one loads while the other computes. BM = 16 serves few rows
+// read), while the next tile is copied asynchronously. BM = 16 serves few rows
 // (decoding), 64 the rest. When there are fewer CTAs than SMs the keys are cut
 // into ranges, each writing (O, log-sum-exp) of its part, joined afterwards.
-#include "tc_common.cuh"
-#include "xattn.cuh"
+#include "xattn_tc.cuh"
 
 namespace tsb {
 namespace {
@@ -75,8 +73,9 @@ __global__ void __launch_bounds__(NT) xattn_simt_kernel(const XKernel A) {
   constexpr int TY = NT / 16, RM = BM / TY, DP = DC * 64 + 4, PP = kXKeys + 4;
   extern __shared__ __align__(16) float smx[];
   float* Qs = smx;
-  float* KV = Qs + BM * DP;
-  float* Ps = KV + kXKeys * DP;
+  float* Ks = Qs + BM * DP;
+  float* Vs = Ks + kXKeys * DP;
+  float* Ps = Vs + kXKeys * DP;
   const XSide& s = A.s;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int item = blockIdx.x / A.row_tiles, rt = blockIdx.x - item * A.row_tiles;
@@ -111,19 +110,28 @@ __global__ void __launch_bounds__(NT) xattn_simt_kernel(const XKernel A) {
 #pragma unroll
     for (int c = 0; c < DC; ++c) acc[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  auto load_tile = [&](const T* base, int64_t stride, int k0) {
+  // fp32 rows that start on 16 bytes are copied asynchronously, the others through registers
+  const bool async = sizeof(T) == 4 && vec && D % 4 == 0;
+  auto load_tile = [&](float* dst, const T* base, int64_t stride, int k0) {
     for (int i = tid; i < kXKeys * DC * 16; i += NT) {
       const int row = i / (DC * 16), d = (i - row * (DC * 16)) * 4;
       const int key = k0 + row;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (key < kend && (!mask || mask[key])) v = load4(base + key * stride, d, D, vec);
-      *reinterpret_cast<float4*>(KV + row * DP + d) = v;
+      const bool in = key < kend && (!mask || mask[key]);
+      if (async) {
+        cp_async16(dst + row * DP + d, in && d < D ? base + key * stride + d : base, in && d < D);
+      } else {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (in) v = load4(base + key * stride, d, D, vec);
+        *reinterpret_cast<float4*>(dst + row * DP + d) = v;
+      }
     }
   };
+  // K of the next tile arrives while P V runs, V while the scores are formed
+  if (kbeg < kend) load_tile(Ks, kp, s.k_t, kbeg);
   for (int k0 = kbeg; k0 < kend; k0 += kXKeys) {
+    cp_async_wait_all();
     __syncthreads();
-    load_tile(kp, s.k_t, k0);
-    __syncthreads();
+    load_tile(Vs, vp, s.v_t, k0);
     float sc[RM][4];
 #pragma unroll
     for (int i = 0; i < RM; ++i)
@@ -133,7 +141,7 @@ __global__ void __launch_bounds__(NT) xattn_simt_kernel(const XKernel A) {
     for (int d = 0; d < DC * 64; d += 4) {
       float4 kv[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(KV + (tx + 16 * j) * DP + d);
+      for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * j) * DP + d);
 #pragma unroll
       for (int i = 0; i < RM; ++i) {
         const float4 q = *reinterpret_cast<const float4*>(Qs + (ty * RM + i) * DP + d);
@@ -180,9 +188,9 @@ __global__ void __launch_bounds__(NT) xattn_simt_kernel(const XKernel A) {
         acc[i][c].w *= corr;
       }
     }
+    cp_async_wait_all();
     __syncthreads();
-    load_tile(vp, s.v_t, k0);
-    __syncthreads();
+    if (k0 + kXKeys < kend) load_tile(Ks, kp, s.k_t, k0 + kXKeys);
 #pragma unroll 2
     for (int k = 0; k < kXKeys; k += 4) {
       float4 p[RM];
@@ -192,7 +200,7 @@ __global__ void __launch_bounds__(NT) xattn_simt_kernel(const XKernel A) {
       for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
-          const float4 v = *reinterpret_cast<const float4*>(KV + (k + kk) * DP + tx * 4 + 64 * c);
+          const float4 v = *reinterpret_cast<const float4*>(Vs + (k + kk) * DP + tx * 4 + 64 * c);
 #pragma unroll
           for (int i = 0; i < RM; ++i)
             fma4(acc[i][c], kk == 0 ? p[i].x : kk == 1 ? p[i].y : kk == 2 ? p[i].z : p[i].w, v);
@@ -311,7 +319,7 @@ SimtPlan simt_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n
 
 template <typename T, int BM, int NT, int DC>
 int simt_launch(const XKernel& A, int splits, bool behind, cudaStream_t st) {
-  constexpr size_t smem = sizeof(float) * (static_cast<size_t>(BM + kXKeys) * (DC * 64 + 4) + BM * (kXKeys + 4));
+  constexpr size_t smem = sizeof(float) * (static_cast<size_t>(BM + 2 * kXKeys) * (DC * 64 + 4) + BM * (kXKeys + 4));
   auto kern = xattn_simt_kernel<T, BM, NT, DC>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return cuda_status(e, "attention: set smem");
