@@ -16,7 +16,7 @@
 // read), while the next tile is copied asynchronously. BM = 16 serves few rows
 // (decoding), 64 the rest. When there are fewer CTAs than SMs the keys are cut
 // into ranges, each writing (O, log-sum-exp) of its part, joined afterwards.
-#include "xattn_tc.cuh"
+#include "xattn_tf32.cuh"
 
 namespace tsb {
 namespace {
@@ -240,6 +240,143 @@ __global__ void __launch_bounds__(NT) xattn_simt_kernel(const XKernel A) {
   grid_dep_wait();  // ends after the launch it ran beside: what follows needs both
 }
 
+// 64 rows a CTA, 16 a warp: scores and probabilities stay in registers as product tiles.
+template <typename T, int DC>
+__global__ void __launch_bounds__(128, DC == 1 ? 4 : DC == 2 ? 2 : 1) xattn_mma_kernel(const XKernel A) {
+  constexpr int BM = 64, NT = 128, DP = DC * 64 + 4, NK = kXKeys / 8, NO = DC * 8;
+  extern __shared__ __align__(16) float smx[];
+  float* Qs = smx;
+  float* Ks = Qs + BM * DP;
+  float* Vs = Ks + kXKeys * DP;
+  const XSide& s = A.s;
+  const int tid = threadIdx.x, w = tid >> 5, g = (tid & 31) >> 2, t = tid & 3;
+  const int item = blockIdx.x / A.row_tiles, rt = blockIdx.x - item * A.row_tiles;
+  const int bi = item / s.hkv, h = item - bi * s.hkv;
+  const int64_t R = side_rows(s), r0 = static_cast<int64_t>(rt) * BM;
+  const int D = A.D, len = side_len(s, bi);
+  const int kbeg = blockIdx.y * A.chunk, kend = min(len, kbeg + A.chunk);
+  const T* kp = static_cast<const T*>(s.k) + bi * s.k_b + h * s.k_h;
+  const T* vp = static_cast<const T*>(s.v) + bi * s.v_b + h * s.v_h;
+  const uint8_t* mask = s.mask ? s.mask + bi * s.mask_stride : nullptr;
+  grid_dep_launch();  // the other side's launch, which needs none of this one's results, may run beside it
+
+  for (int i = tid; i < BM * DC * 16; i += NT) {
+    const int row = i / (DC * 16), d = (i - row * (DC * 16)) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r0 + row < R) v = load4(static_cast<const T*>(s.q) + q_offset(s, bi, h, side_row(s, r0 + row)), d, D, A.vec);
+    *reinterpret_cast<float4*>(Qs + row * DP + d) = v;
+  }
+  int lim[2];
+  float m[2], l[2], acc[NO][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t r = r0 + w * 16 + g + 8 * i;
+    lim[i] = r < R ? min(kend, row_limit(s, side_row(s, r), len)) : 0;
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+  }
+#pragma unroll
+  for (int n = 0; n < NO; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[n][j] = 0.f;
+  // fp32 rows that start on 16 bytes are copied asynchronously, the others through registers
+  const bool async = sizeof(T) == 4 && A.vec && D % 4 == 0;
+  auto load_tile = [&](float* dst, const T* base, int64_t stride, int k0) {
+    for (int i = tid; i < kXKeys * DC * 16; i += NT) {
+      const int row = i / (DC * 16), d = (i - row * (DC * 16)) * 4;
+      const int key = k0 + row;
+      const bool in = key < kend && (!mask || mask[key]);
+      if (async) {
+        cp_async16(dst + row * DP + d, in && d < D ? base + key * stride + d : base, in && d < D);
+      } else {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (in) v = load4(base + key * stride, d, D, A.vec);
+        *reinterpret_cast<float4*>(dst + row * DP + d) = v;
+      }
+    }
+  };
+  // K of the next tile arrives while P V runs, V while the scores are formed
+  if (kbeg < kend) load_tile(Ks, kp, s.k_t, kbeg);
+  for (int k0 = kbeg; k0 < kend; k0 += kXKeys) {
+    cp_async_wait_all();
+    __syncthreads();
+    load_tile(Vs, vp, s.v_t, k0);
+    float sc[NK][4];
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sc[n][j] = 0.f;
+    scores_tf32<NK, DP>(sc, Qs + w * 16 * DP, Ks, D, g, t);
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = k0 + n * 8 + 2 * t + (j & 1);
+        const bool hide = key >= lim[j >> 1] || (mask && !mask[key]);
+        sc[n][j] = hide ? -INFINITY : sc[n][j] * A.scale_log2;
+        mx[j >> 1] = fmaxf(mx[j >> 1], sc[n][j]);
+      }
+    float corr[2], mu[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+      const float mn = fmaxf(m[i], mx[i]);
+      mu[i] = mn == -INFINITY ? 0.f : mn;  // no key so far: every term is exactly 0
+      corr[i] = exp2f(m[i] - mu[i]);
+      m[i] = mn;
+      l[i] *= corr[i];  // this lane's columns; the four lanes' sums are joined at the end
+    }
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sc[n][j] = exp2f(sc[n][j] - mu[j >> 1]);
+        l[j >> 1] += sc[n][j];
+      }
+#pragma unroll
+    for (int n = 0; n < NO; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[n][j] *= corr[j >> 1];
+    cp_async_wait_all();
+    __syncthreads();
+    if (k0 + kXKeys < kend) load_tile(Ks, kp, s.k_t, k0 + kXKeys);
+    weigh_tf32<NK, NO, DP>(acc, sc, Vs, g, t);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    const int64_t r = r0 + w * 16 + g + 8 * i;
+    if (r >= R) continue;
+    const XRow x = side_row(s, r);
+    const int64_t fr = flat_row(s, bi, h, x);
+    const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
+    const float lse = l[i] == 0.f ? -INFINITY : m[i] + log2f(l[i]);
+    const bool piece = A.part_o != nullptr;
+    const int64_t pr = static_cast<int64_t>(blockIdx.y) * A.rows_all + fr;
+    float* pp = piece ? A.part_o + pr * D : nullptr;
+    T* po = piece ? nullptr : static_cast<T*>(A.out) + o_offset(s, bi, h, x);
+#pragma unroll
+    for (int n = 0; n < NO; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int d = n * 8 + 2 * t + j;
+        const float v = acc[n][2 * i + j] * inv;
+        if (d < D) {
+          if (piece) pp[d] = v;
+          else store1(po + d, v);
+        }
+      }
+    if (t == 0) {
+      if (piece) A.part_lse[pr] = lse;
+      else if (A.lse != nullptr) A.lse[fr] = lse;
+    }
+  }
+  grid_dep_wait();  // ends after the launch it ran beside: what follows needs both
+}
+
 // One warp per row.
 template <typename T>
 __global__ void __launch_bounds__(256) combine_pieces_kernel(const float* __restrict__ part_o,
@@ -299,17 +436,20 @@ SimtPlan simt_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n
   for (int i = 0; i < n; ++i) most = most > side_rows(s[i]) ? most : side_rows(s[i]);
   // 16-row CTAs where a 64-row tile would be mostly padding
   p.bm = most <= 32 ? 16 : 64;
-  const int64_t want = 3ll * sm_count();
+  // resident CTAs of the 64-row form: by registers and shared memory
+  const int64_t slots = (p.dc == 1 ? 4ll : p.dc == 2 ? 2ll : 1ll) * sm_count();
   for (int i = 0; i < n; ++i) {
     p.row_tiles[i] = static_cast<int>((side_rows(s[i]) + p.bm - 1) / p.bm);
     const int64_t ctas = static_cast<int64_t>(p.row_tiles[i]) * s[i].nb * s[i].hkv;
     const int64_t tiles = (s[i].klen + kXKeys - 1) / kXKeys;
-    // as many ranges as fill the GPU with two CTAs an SM
-    int64_t splits = ctas > 0 ? (want + ctas - 1) / ctas : 1;
-    splits = splits < tiles ? splits : tiles;
-    if (splits > 128) splits = 128;
-    if (splits < 1) splits = 1;
-    const int64_t per = tiles > 0 ? (tiles + splits - 1) / splits : 1;
+    int64_t per;
+    if (p.bm == 16) {  // bound by the reads of K and V: three CTAs an SM (walk_steps' fewer: 46 us against 31 at 4096 keys)
+      int64_t splits = ctas > 0 ? (3ll * sm_count() + ctas - 1) / ctas : 1;
+      splits = splits < 128 ? splits : 128;
+      per = tiles > splits ? (tiles + splits - 1) / splits : 1;
+    } else {
+      per = walk_steps(ctas, tiles, slots, 128);
+    }
     p.chunk[i] = static_cast<int>(per * kXKeys);
     p.splits[i] = static_cast<int>(tiles > 0 ? (tiles + per - 1) / per : 1);
     p.pieces += p.splits[i];
@@ -317,32 +457,33 @@ SimtPlan simt_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n
   return p;
 }
 
-template <typename T, int BM, int NT, int DC>
-int simt_launch(const XKernel& A, int splits, bool behind, cudaStream_t st) {
-  constexpr size_t smem = sizeof(float) * (static_cast<size_t>(BM + 2 * kXKeys) * (DC * 64 + 4) + BM * (kXKeys + 4));
-  auto kern = xattn_simt_kernel<T, BM, NT, DC>;
+int attention_launch(void (*kern)(XKernel), int threads, size_t smem, const XKernel& A, int splits, bool behind,
+                     cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return cuda_status(e, "attention: set smem");
   const dim3 grid(static_cast<unsigned>(A.row_tiles) * A.s.nb * A.s.hkv, splits);
   if (behind) {
-    e = launch_pdl(kern, grid, dim3(NT), smem, st, A);
-    return e == cudaSuccess ? TRNSPARSE_OK : cuda_status(e, "attention (CUDA cores) launch");
+    e = launch_pdl(kern, grid, dim3(threads), smem, st, A);
+    return e == cudaSuccess ? TRNSPARSE_OK : cuda_status(e, "attention launch");
   }
-  kern<<<grid, NT, smem, st>>>(A);
-  TSB_CHECK_LAUNCH("attention (CUDA cores) launch");
+  kern<<<grid, threads, smem, st>>>(A);
+  TSB_CHECK_LAUNCH("attention launch");
   return TRNSPARSE_OK;
+}
+
+template <typename T, int DC>
+int attention_dispatch(const XKernel& A, int bm, int splits, bool behind, cudaStream_t st) {
+  const size_t smem = sizeof(float) * static_cast<size_t>(bm + 2 * kXKeys) * (DC * 64 + 4);
+  if (bm == 64) return attention_launch(xattn_mma_kernel<T, DC>, 128, smem, A, splits, behind, st);
+  return attention_launch(xattn_simt_kernel<T, 16, 128, DC>, 128, smem + sizeof(float) * 16 * (kXKeys + 4), A, splits,
+                          behind, st);
 }
 
 template <typename T>
 int simt_dispatch(const XKernel& A, int bm, int dc, int splits, bool behind, cudaStream_t st) {
-  if (bm == 16) {
-    if (dc == 1) return simt_launch<T, 16, 128, 1>(A, splits, behind, st);
-    if (dc == 2) return simt_launch<T, 16, 128, 2>(A, splits, behind, st);
-    return simt_launch<T, 16, 128, 4>(A, splits, behind, st);
-  }
-  if (dc == 1) return simt_launch<T, 64, 256, 1>(A, splits, behind, st);
-  if (dc == 2) return simt_launch<T, 64, 256, 2>(A, splits, behind, st);
-  return simt_launch<T, 64, 256, 4>(A, splits, behind, st);
+  if (dc == 1) return attention_dispatch<T, 1>(A, bm, splits, behind, st);
+  if (dc == 2) return attention_dispatch<T, 2>(A, bm, splits, behind, st);
+  return attention_dispatch<T, 4>(A, bm, splits, behind, st);
 }
 
 // Every base and stride of the call's operands is a multiple of four elements.

@@ -16,7 +16,7 @@
 // 128, where four 64-row tiles would not fit in shared memory) with RM x RM
 // scores a thread. Where tiles are fewer than SMs the walk is cut into parts
 // whose fp32 sums a last kernel adds in order.
-#include "xattn.cuh"
+#include "xattn_tf32.cuh"
 
 namespace tsb {
 namespace {
@@ -43,15 +43,7 @@ __device__ __forceinline__ float4 bload4(const T* row, int d, int D, bool vec) {
   if (d + 3 < D) r.w = bcvt(row[d + 3]);
   return r;
 }
-__device__ __forceinline__ float bdot4(float4 a, float4 b, float c) {
-  return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, c))));
-}
-__device__ __forceinline__ void bfma4(float4& c, float a, float4 b) {
-  c.x = fmaf(a, b.x, c.x);
-  c.y = fmaf(a, b.y, c.y);
-  c.z = fmaf(a, b.z, c.z);
-  c.w = fmaf(a, b.w, c.w);
-}
+constexpr int kBwdWalk = 32;  // walked rows a step
 
 struct BKernel {
   XSide s;  // o_*: strides of dq here
@@ -84,211 +76,154 @@ __global__ void __launch_bounds__(256) xattn_delta_kernel(const T* __restrict__ 
   if (lane == 0) delta[row] = s;
 }
 
-template <typename T, int BT, int DC, bool COLS>
-__global__ void __launch_bounds__(256) xattn_bwd_simt_kernel(const BKernel A) {
-  constexpr int RM = BT / 16, DP = DC * 64 + 4, PP = BT + 4;
+// 64 fixed rows (queries, or keys with COLS) a CTA, 16 a warp; WT walked rows a step. Above head_dim 128 the sums of
+// dK and of dV have 128 registers a thread each: eight warps, the second four hold dV.
+template <typename T, int DC, bool COLS>
+__global__ void __launch_bounds__(COLS && DC == 4 ? 256 : 128, DC == 1 ? 4 : DC == 2 ? 2 : 1)
+    xattn_bwd_mma_kernel(const BKernel A) {
+  constexpr int BT = 64, WT = kBwdWalk, NT = COLS && DC == 4 ? 256 : 128;
+  constexpr int DP = DC * 64 + 4, NW = WT / 8, NO = DC * 8, CH = DC * 16;
+  constexpr bool BOTH = COLS && DC != 4;
   extern __shared__ __align__(16) float smb[];
   float* F1 = smb;             // fixed: Q (rows) or K (columns)
   float* F2 = F1 + BT * DP;    // fixed: dO or V
   float* X1 = F2 + BT * DP;    // walked: K or Q
-  float* X2 = X1 + BT * DP;    // walked: V or dO
-  float* S1 = X2 + BT * DP;    // dS [query][key]
-  float* S2 = S1 + BT * PP;    // P [query][key] (columns only)
-  float* st_lse = COLS ? S2 + BT * PP : S1 + BT * PP;
-  float* st_delta = st_lse + BT;
+  float* X2 = X1 + WT * DP;    // walked: V or dO
+  float* st_lse = X2 + WT * DP;  // of the walked queries (columns)
+  float* st_delta = st_lse + WT;
   const XSide& s = A.s;
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int tid = threadIdx.x, g = (tid & 31) >> 2, t = tid & 3;
+  const int f0 = (tid >> 5 & 3) * 16;                // this warp's fixed rows
+  const bool second = COLS && DC == 4 && tid >= 128;  // holds dV
   const int item = blockIdx.x / A.tiles, tile = blockIdx.x - item * A.tiles;
   const int bi = item / s.hkv, h = item - bi * s.hkv;
   const int64_t R = side_rows(s);
   const int D = A.D, len = side_len(s, bi);
+  const T* qp = static_cast<const T*>(s.q) + bi * s.q_bi + static_cast<int64_t>(h) * s.G * s.q_h;
+  const T* gp = static_cast<const T*>(A.dout) + bi * A.g_b + static_cast<int64_t>(h) * s.G * A.g_h;
   const T* kp = static_cast<const T*>(s.k) + bi * s.k_b + h * s.k_h;
   const T* vp = static_cast<const T*>(s.v) + bi * s.v_b + h * s.v_h;
+  const int64_t stat0 = (static_cast<int64_t>(bi) * s.hkv + h) * s.G * s.T;  // flat row of packed row 0
   const uint8_t* mask = s.mask ? s.mask + bi * s.mask_stride : nullptr;
-  const bool vec = A.vec;
-  auto load_q = [&](float* q, float* g, int64_t r0) {
-    for (int i = tid; i < BT * DC * 16; i += 256) {
-      const int row = i / (DC * 16), d = (i - row * (DC * 16)) * 4;
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-      if (r0 + row < R) {
-        const XRow x = side_row(s, r0 + row);
-        a = bload4(static_cast<const T*>(s.q) + q_offset(s, bi, h, x), d, D, vec);
-        b = bload4(static_cast<const T*>(A.dout) + bi * A.g_b + (static_cast<int64_t>(h) * s.G + x.g) * A.g_h +
-                       x.t * A.g_t, d, D, vec);
-      }
-      *reinterpret_cast<float4*>(q + row * DP + d) = a;
-      *reinterpret_cast<float4*>(g + row * DP + d) = b;
-    }
-    for (int i = tid; i < BT; i += 256) {
-      float ls = INFINITY, de = 0.f;  // rows past the last: P = 0
-      if (r0 + i < R) {
-        const int64_t fr = flat_row(s, bi, h, side_row(s, r0 + i));
-        ls = A.lse[fr];
-        de = A.delta[fr];
-      }
-      st_lse[i] = ls;
-      st_delta[i] = de;
+  // fp32 rows that start on 16 bytes are copied asynchronously, the others through registers
+  const bool async = sizeof(T) == 4 && A.vec && D % 4 == 0;
+  auto copy4 = [&](float* dst, const T* row, int d, bool in) {
+    if (async) {
+      cp_async16(dst, in && d < D ? row + d : static_cast<const T*>(s.q), in && d < D);
+    } else {
+      *reinterpret_cast<float4*>(dst) = in ? bload4(row, d, D, A.vec) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   };
-  auto load_kv = [&](float* k, float* v, int k0) {
-    for (int i = tid; i < BT * DC * 16; i += 256) {
-      const int row = i / (DC * 16), d = (i - row * (DC * 16)) * 4;
-      const int key = k0 + row;
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-      if (key < len && (!mask || mask[key])) {
-        a = bload4(kp + key * s.k_t, d, D, vec);
-        b = bload4(vp + key * s.v_t, d, D, vec);
-      }
-      *reinterpret_cast<float4*>(k + row * DP + d) = a;
-      *reinterpret_cast<float4*>(v + row * DP + d) = b;
+  auto load_q = [&](float* q, float* go, int64_t r0, int n) {
+    for (int i = tid; i < n * CH; i += NT) {
+      const int row = i / CH, d = (i - row * CH) * 4;
+      const bool in = r0 + row < R;
+      const unsigned r = in ? static_cast<unsigned>(r0 + row) : 0u, hg = r / s.T, tt = r - hg * s.T;
+      copy4(q + row * DP + d, qp + hg * s.q_h + tt * s.q_t, d, in);
+      copy4(go + row * DP + d, gp + hg * A.g_h + tt * A.g_t, d, in);
     }
   };
-  if (COLS) load_kv(F1, F2, tile * BT);
-  else load_q(F1, F2, static_cast<int64_t>(tile) * BT);
-  float4 acc0[RM][DC], acc1[COLS ? RM : 1][COLS ? DC : 1];
+  auto load_kv = [&](float* k, float* v, int k0, int n) {
+    for (int i = tid; i < n * CH; i += NT) {
+      const int row = i / CH, d = (i - row * CH) * 4, key = k0 + row;
+      const bool in = key < len && (!mask || mask[key]);
+      copy4(k + row * DP + d, kp + key * s.k_t, d, in);
+      copy4(v + row * DP + d, vp + key * s.v_t, d, in);
+    }
+  };
+  if (COLS) load_kv(F1, F2, tile * BT, BT);
+  else load_q(F1, F2, static_cast<int64_t>(tile) * BT, BT);
+  float row_lse[2], row_delta[2];  // rows: of this lane's queries
+  bool hide_row[2];                // columns: this lane's keys
 #pragma unroll
-  for (int i = 0; i < RM; ++i)
+  for (int i = 0; i < 2; ++i) {
+    const int64_t r = static_cast<int64_t>(tile) * BT + f0 + g + 8 * i;
+    row_lse[i] = INFINITY;  // rows past the last: P = 0
+    row_delta[i] = 0.f;
+    hide_row[i] = false;
+    if (COLS) {
+      hide_row[i] = r >= len || (mask && !mask[r]);
+    } else if (r < R) {
+      row_lse[i] = A.lse[stat0 + r];
+      row_delta[i] = A.delta[stat0 + r];
+    }
+  }
+  float acc0[NO][4], acc1[BOTH ? NO : 1][4];
 #pragma unroll
-    for (int c = 0; c < DC; ++c) {
-      acc0[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if constexpr (COLS) acc1[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int n = 0; n < NO; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      acc0[n][j] = 0.f;
+      if constexpr (BOTH) acc1[n][j] = 0.f;
     }
   // a walk over keys stops at the kept length; a key tile with no kept key walks nothing
   const int64_t wend = COLS ? (tile * BT < len ? R : 0) : len;
   const int64_t w0 = static_cast<int64_t>(blockIdx.y) * A.chunk;
   const int64_t w1 = wend < w0 + A.chunk ? wend : w0 + A.chunk;
-  for (int64_t w = w0; w < w1; w += BT) {
+  for (int64_t w = w0; w < w1; w += WT) {
     __syncthreads();
-    if (COLS) load_q(X1, X2, w);
-    else load_kv(X1, X2, static_cast<int>(w));
-    __syncthreads();
-    const float* Qs = COLS ? X1 : F1;
-    const float* Gs = COLS ? X2 : F2;
-    const float* Ks = COLS ? F1 : X1;
-    const float* Vs = COLS ? F2 : X2;
-    // queries ty RM + i, keys tx + 16 j
-    float sc[RM][RM], dp[RM][RM];
-#pragma unroll
-    for (int i = 0; i < RM; ++i)
-#pragma unroll
-      for (int j = 0; j < RM; ++j) sc[i][j] = dp[i][j] = 0.f;
-#pragma unroll 2
-    for (int d = 0; d < DC * 64; d += 4) {
-      float4 kv[RM], vv[RM];
-#pragma unroll
-      for (int j = 0; j < RM; ++j) {
-        kv[j] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * j) * DP + d);
-        vv[j] = *reinterpret_cast<const float4*>(Vs + (tx + 16 * j) * DP + d);
-      }
-#pragma unroll
-      for (int i = 0; i < RM; ++i) {
-        const float4 q = *reinterpret_cast<const float4*>(Qs + (ty * RM + i) * DP + d);
-        const float4 g = *reinterpret_cast<const float4*>(Gs + (ty * RM + i) * DP + d);
-#pragma unroll
-        for (int j = 0; j < RM; ++j) {
-          sc[i][j] = bdot4(q, kv[j], sc[i][j]);
-          dp[i][j] = bdot4(g, vv[j], dp[i][j]);
-        }
-      }
-    }
-    const int k0 = COLS ? tile * BT : static_cast<int>(w);
-#pragma unroll
-    for (int j = 0; j < RM; ++j) {
-      const int key = k0 + tx + 16 * j;
-      const bool hide = key >= len || (mask && !mask[key]);
-#pragma unroll
-      for (int i = 0; i < RM; ++i) {
-        const int row = ty * RM + i;
-        const float p = hide ? 0.f : exp2f(fmaf(sc[i][j], A.scale_log2, -st_lse[row]));
-        const float ds = hide ? 0.f : p * (dp[i][j] - st_delta[row]);
-        S1[row * PP + tx + 16 * j] = ds;
-        if constexpr (COLS) S2[row * PP + tx + 16 * j] = p;
-      }
-    }
-    __syncthreads();
-    // Second products; P and dS are read as vectors (a scalar a step made shared memory the bound: 99 against 50 us
-    // for dQ at 2 x 8/2 heads, 333 x 517 x 64).
-    if constexpr (COLS) {
-#pragma unroll 2
-      for (int q = 0; q < BT; ++q) {
-        float p[RM], ds[RM];
-        if constexpr (RM == 4) {
-          *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(S2 + q * PP + ty * RM);
-          *reinterpret_cast<float4*>(ds) = *reinterpret_cast<const float4*>(S1 + q * PP + ty * RM);
-        } else {
-          *reinterpret_cast<float2*>(p) = *reinterpret_cast<const float2*>(S2 + q * PP + ty * RM);
-          *reinterpret_cast<float2*>(ds) = *reinterpret_cast<const float2*>(S1 + q * PP + ty * RM);
-        }
-#pragma unroll
-        for (int c = 0; c < DC; ++c) {
-          const float4 qv = *reinterpret_cast<const float4*>(X1 + q * DP + tx * 4 + 64 * c);
-          const float4 gv = *reinterpret_cast<const float4*>(X2 + q * DP + tx * 4 + 64 * c);
-#pragma unroll
-          for (int i = 0; i < RM; ++i) {
-            bfma4(acc0[i][c], ds[i], qv);
-            bfma4(acc1[i][c], p[i], gv);
-          }
-        }
+    if (COLS) {
+      load_q(X1, X2, w, WT);
+      if (tid < WT) {
+        const bool in = w + tid < R;
+        st_lse[tid] = in ? A.lse[stat0 + w + tid] : INFINITY;
+        st_delta[tid] = in ? A.delta[stat0 + w + tid] : 0.f;
       }
     } else {
-#pragma unroll 2
-      for (int k = 0; k < BT; k += 4) {
-        float4 ds[RM];
-#pragma unroll
-        for (int i = 0; i < RM; ++i) ds[i] = *reinterpret_cast<const float4*>(S1 + (ty * RM + i) * PP + k);
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-          for (int c = 0; c < DC; ++c) {
-            const float4 kv = *reinterpret_cast<const float4*>(X1 + (k + kk) * DP + tx * 4 + 64 * c);
-#pragma unroll
-            for (int i = 0; i < RM; ++i)
-              bfma4(acc0[i][c], kk == 0 ? ds[i].x : kk == 1 ? ds[i].y : kk == 2 ? ds[i].z : ds[i].w, kv);
-          }
-      }
+      load_kv(X1, X2, static_cast<int>(w), WT);
     }
+    cp_async_wait_all();
+    __syncthreads();
+    float sc[NW][4], dp[NW][4];  // scores, then P; dP, then dS: fixed rows by walked rows
+#pragma unroll
+    for (int n = 0; n < NW; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sc[n][j] = dp[n][j] = 0.f;
+    scores_tf32<NW, DP>(sc, F1 + f0 * DP, X1, D, g, t);
+    if (!second) scores_tf32<NW, DP>(dp, F2 + f0 * DP, X2, D, g, t);
+#pragma unroll
+    for (int n = 0; n < NW; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = j >> 1, x = n * 8 + 2 * t + (j & 1);
+        bool hide = hide_row[i];
+        if (!COLS) hide = w + x >= len || (mask && !mask[w + x]);
+        const float p = hide ? 0.f : exp2f(fmaf(sc[n][j], A.scale_log2, -(COLS ? st_lse[x] : row_lse[i])));
+        dp[n][j] = hide ? 0.f : p * (dp[n][j] - (COLS ? st_delta[x] : row_delta[i]));
+        sc[n][j] = p;
+      }
+    if constexpr (BOTH) weigh_tf32<NW, NO, DP>(acc1, sc, X2, g, t);
+    if (second) weigh_tf32<NW, NO, DP>(acc0, sc, X2, g, t);
+    else weigh_tf32<NW, NO, DP>(acc0, dp, X1, g, t);
   }
 #pragma unroll
-  for (int i = 0; i < RM; ++i) {
-    const int64_t r = static_cast<int64_t>(tile) * BT + ty * RM + i;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t r = static_cast<int64_t>(tile) * BT + f0 + g + 8 * i;
     if (r >= (COLS ? static_cast<int64_t>(s.klen) : R)) continue;
-    int64_t fr;
-    T *o0 = nullptr, *o1 = nullptr;
-    if constexpr (COLS) {
-      fr = (static_cast<int64_t>(bi) * s.hkv + h) * s.klen + r;
-      if (A.part0 == nullptr) {
-        o0 = static_cast<T*>(A.dk) + bi * A.dk_s[0] + h * A.dk_s[1] + r * A.dk_s[2];
-        o1 = static_cast<T*>(A.dv) + bi * A.dv_s[0] + h * A.dv_s[1] + r * A.dv_s[2];
-      }
-    } else {
-      const XRow x = side_row(s, r);
-      fr = flat_row(s, bi, h, x);
-      if (A.part0 == nullptr) o0 = static_cast<T*>(A.dq) + o_offset(s, bi, h, x);
-    }
+    const int64_t fr = COLS ? (static_cast<int64_t>(bi) * s.hkv + h) * s.klen + r : stat0 + r;
     const int64_t at = (static_cast<int64_t>(blockIdx.y) * A.rows_all + fr) * D;
-#pragma unroll
-    for (int c = 0; c < DC; ++c) {
-      const int d = tx * 4 + 64 * c;
-      const float e0[4] = {acc0[i][c].x, acc0[i][c].y, acc0[i][c].z, acc0[i][c].w};
-      float e1[4] = {0.f, 0.f, 0.f, 0.f};
-      if constexpr (COLS) {
-        e1[0] = acc1[i][c].x;
-        e1[1] = acc1[i][c].y;
-        e1[2] = acc1[i][c].z;
-        e1[3] = acc1[i][c].w;
-      }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (d + q >= D) continue;
-        if (A.part0 != nullptr) {
-          A.part0[at + d + q] = e0[q] * A.scale;
-          if constexpr (COLS) A.part1[at + d + q] = e1[q];
-        } else {
-          bstore(o0 + d + q, e0[q] * A.scale);
-          if constexpr (COLS) bstore(o1 + d + q, e1[q]);
-        }
-      }
+    const bool piece = A.part0 != nullptr;
+    T *o0 = nullptr, *o1 = nullptr;
+    if (!piece && COLS) {
+      o0 = static_cast<T*>(A.dk) + bi * A.dk_s[0] + h * A.dk_s[1] + r * A.dk_s[2];
+      o1 = static_cast<T*>(A.dv) + bi * A.dv_s[0] + h * A.dv_s[1] + r * A.dv_s[2];
+    } else if (!piece) {
+      o0 = static_cast<T*>(A.dq) + o_offset(s, bi, h, side_row(s, r));
     }
+    auto put = [&](float* part, T* o, int d, float v) {
+      if (piece) part[at + d] = v;
+      else bstore(o + d, v);
+    };
+#pragma unroll
+    for (int n = 0; n < NO; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int d = n * 8 + 2 * t + j;
+        if (d >= D) continue;
+        if (second) put(A.part1, o1, d, acc0[n][2 * i + j]);
+        else put(A.part0, o0, d, acc0[n][2 * i + j] * A.scale);
+        if constexpr (BOTH) put(A.part1, o1, d, acc1[n][2 * i + j]);
+      }
   }
 }
 
@@ -310,30 +245,24 @@ __global__ void __launch_bounds__(256) xattn_sum_parts_kernel(const float* __res
 // ---------------------------------------------------------------- host side
 
 struct BPlan {
-  int bt, dc, parts[2], chunk[2], tiles[2];  // [0] rows (dQ), [1] columns (dK, dV)
+  int dc, parts[2], chunk[2], tiles[2];  // [0] rows (dQ), [1] columns (dK, dV)
   size_t ws;
 };
 
 BPlan bwd_plan(const trnsparse_attention_args* a, const XSide& s) {
   BPlan p = {};
   p.dc = a->head_dim <= 64 ? 1 : a->head_dim <= 128 ? 2 : 4;
-  p.bt = p.dc == 4 ? 32 : 64;
   const int64_t R = side_rows(s);
   const int64_t fixed[2] = {R, s.klen}, walk[2] = {s.klen, R};
-  const int64_t want = 2ll * sm_count();  // two CTAs an SM up to head_dim 64, and no SM without one
+  const int64_t slots = (p.dc == 1 ? 4ll : p.dc == 2 ? 2ll : 1ll) * sm_count();  // resident CTAs
   const int64_t rows = a->batch * a->q_heads * a->q_len, keys = a->batch * a->kv_heads * a->k_len;
   p.ws = sizeof(float) * static_cast<size_t>(rows);
   size_t parts_ws = 0;
   for (int i = 0; i < 2; ++i) {
-    p.tiles[i] = static_cast<int>((fixed[i] + p.bt - 1) / p.bt);
-    const int64_t ctas = static_cast<int64_t>(p.tiles[i]) * s.nb * s.hkv, steps = (walk[i] + p.bt - 1) / p.bt;
-    // each part at least two steps
-    int64_t parts = ctas > 0 ? want / ctas : 1;
-    if (parts > steps / 2) parts = steps / 2;
-    if (parts > 32) parts = 32;
-    if (parts < 1) parts = 1;
-    const int64_t per = steps > 0 ? (steps + parts - 1) / parts : 1;
-    p.chunk[i] = static_cast<int>(per * p.bt);
+    p.tiles[i] = static_cast<int>((fixed[i] + 63) / 64);
+    const int64_t ctas = static_cast<int64_t>(p.tiles[i]) * s.nb * s.hkv, steps = (walk[i] + kBwdWalk - 1) / kBwdWalk;
+    const int64_t per = walk_steps(ctas, steps, slots, 32);
+    p.chunk[i] = static_cast<int>(per * kBwdWalk);
     p.parts[i] = static_cast<int>(steps > 0 ? (steps + per - 1) / per : 1);
     if (p.parts[i] > 1) {
       const size_t b = sizeof(float) * static_cast<size_t>(p.parts[i]) * a->head_dim * (i ? 2 * keys : rows);
@@ -344,24 +273,24 @@ BPlan bwd_plan(const trnsparse_attention_args* a, const XSide& s) {
   return p;
 }
 
-template <typename T, int BT, int DC, bool COLS>
+template <typename T, int DC, bool COLS>
 int bwd_launch(const BKernel& A, int parts, cudaStream_t st) {
-  constexpr size_t smem =
-      sizeof(float) * (4ull * BT * (DC * 64 + 4) + (COLS ? 2 : 1) * BT * (BT + 4) + 2 * BT);
-  auto kern = xattn_bwd_simt_kernel<T, BT, DC, COLS>;
+  constexpr size_t smem = sizeof(float) * (2ull * (64 + kBwdWalk) * (DC * 64 + 4) + 2 * kBwdWalk);
+  auto kern = xattn_bwd_mma_kernel<T, DC, COLS>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return cuda_status(e, "cross_attention backward: set smem");
+  const int threads = COLS && DC == 4 ? 256 : 128;
   if (A.tiles > 0)
-    kern<<<dim3(static_cast<unsigned>(A.tiles) * A.s.nb * A.s.hkv, parts), 256, smem, st>>>(A);
+    kern<<<dim3(static_cast<unsigned>(A.tiles) * A.s.nb * A.s.hkv, parts), threads, smem, st>>>(A);
   TSB_CHECK_LAUNCH("cross_attention backward launch");
   return TRNSPARSE_OK;
 }
 
 template <typename T, bool COLS>
 int bwd_dispatch(const BKernel& A, int dc, int parts, cudaStream_t st) {
-  if (dc == 1) return bwd_launch<T, 64, 1, COLS>(A, parts, st);
-  if (dc == 2) return bwd_launch<T, 64, 2, COLS>(A, parts, st);
-  return bwd_launch<T, 32, 4, COLS>(A, parts, st);
+  if (dc == 1) return bwd_launch<T, 1, COLS>(A, parts, st);
+  if (dc == 2) return bwd_launch<T, 2, COLS>(A, parts, st);
+  return bwd_launch<T, 4, COLS>(A, parts, st);
 }
 
 template <typename T>

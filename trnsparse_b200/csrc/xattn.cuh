@@ -73,6 +73,23 @@ int check_attention(const trnsparse_attention_args* a, const char* what);
 int combine_pieces(const float* part_o, const float* part_lse, int pieces, const trnsparse_attention_args* a,
                    cudaStream_t st);
 
+// Steps of a walk that one of `ctas` CTAs takes when the walks are cut to fill the GPU's `slots` resident CTAs: the
+// fewest waves times (steps + 2 for the start and end of a CTA), and half a step for each part that is joined afterwards.
+inline int64_t walk_steps(int64_t ctas, int64_t steps, int64_t slots, int64_t most) {
+  int64_t best = steps > 0 ? steps : 1;
+  double least = 1e300;
+  for (int64_t n = 1; n <= most && n <= steps; ++n) {
+    const int64_t per = (steps + n - 1) / n, parts = (steps + per - 1) / per;
+    const double cost = static_cast<double>((ctas * parts + slots - 1) / slots) * static_cast<double>(per + 2) +
+                        (parts > 1 ? 2.0 + 0.5 * static_cast<double>(parts) : 0.0);
+    if (cost < least) {
+      least = cost;
+      best = per;
+    }
+  }
+  return best;
+}
+
 // Tensor-core forms (bf16, head_dim a multiple of 8 up to 128, 16-byte rows).
 bool xattn_tc_ok(const trnsparse_attention_args* a, bool prefix);
 size_t xattn_tc_workspace(const trnsparse_attention_args* a, bool prefix);
