@@ -1,8 +1,8 @@
-// Dense attention on CUDA cores: cross attention (query rows against another
+// Dense attention in fp32: cross attention (query rows against another
 // sequence's keys, shared key heads, ragged or masked keys) and shared-prefix
 // attention (decoding over one prefix for the whole batch plus each sequence's
-// own keys). fp32 at any head_dim up to 256, and the bf16 shapes the
-// tensor-core kernels do not take.
+// own keys), at any head_dim up to 256; and the bf16 shapes the tcgen05 kernels
+// do not take.
 //
 //   s = scale q.k over the kept keys,  P = softmax(s),  O = P V
 // in one pass over the keys with the running row maximum m and sum l; a row
@@ -10,18 +10,23 @@
 // rows are loaded as zeros and their scores are set to -inf, so what the
 // padding holds (infinities, NaN) does not matter.
 //
-// What bounds it: fp32 FMA. A CTA takes BM packed rows and walks the keys in
-// tiles of 64; a thread forms an RM x 4 tile of scores and an RM x 4 DC tile of
-// the output from float4 reads of shared memory (about four FMA per 16 bytes
-// read), while the next tile is copied asynchronously. BM = 16 serves few rows
-// (decoding), 64 the rest. When there are fewer CTAs than SMs the keys are cut
-// into ranges, each writing (O, log-sum-exp) of its part, joined afterwards.
+// Two forms. Up to 32 packed rows (decoding) are bound by the reads of K and V:
+// 16 rows a CTA on the CUDA cores, a thread forming a 2 x 4 tile of scores and a
+// 2 x 4 DC tile of the output from float4 reads of shared memory. More rows are
+// bound by arithmetic: 128 rows a CTA on the tensor cores (3xTF32, xattn_tf32.cuh),
+// 48 TFLOP/s at 2 x 16/16 heads, 1024 x 1024 x 64 (179 us; 308 on the CUDA cores)
+// and 52 with 16/4 heads at head_dim 128 (334 us; 615). The tensor pipe is then half
+// busy: two warps a scheduler, a third of whose instructions are the products.
+// In both the next tile is copied asynchronously. When there are fewer CTAs than
+// fill the GPU the keys are cut into ranges, each writing (O, log-sum-exp) of its
+// part, joined afterwards.
 #include "xattn_tf32.cuh"
 
 namespace tsb {
 namespace {
 
-constexpr int kXKeys = 64;
+constexpr int kXKeys = 64;    // keys a tile: 16-row form
+constexpr int kMmaKeys = 32;  // and 128-row form
 
 __device__ __forceinline__ float xcvt(float v) { return v; }
 __device__ __forceinline__ float xcvt(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -69,7 +74,7 @@ struct XKernel {
 };
 
 template <typename T, int BM, int NT, int DC>
-__global__ void __launch_bounds__(NT) xattn_simt_kernel(const XKernel A) {
+__global__ void __launch_bounds__(NT) xattn_few_kernel(const XKernel A) {
   constexpr int TY = NT / 16, RM = BM / TY, DP = DC * 64 + 4, PP = kXKeys + 4;
   extern __shared__ __align__(16) float smx[];
   float* Qs = smx;
@@ -240,16 +245,18 @@ __global__ void __launch_bounds__(NT) xattn_simt_kernel(const XKernel A) {
   grid_dep_wait();  // ends after the launch it ran beside: what follows needs both
 }
 
-// 64 rows a CTA, 16 a warp: scores and probabilities stay in registers as product tiles.
+// 128 rows a CTA: four warps of 32, so that each split of a K or V element feeds two products, or (above head_dim 128,
+// where 32 rows' sums would not fit in registers) eight of 16. Scores and probabilities stay in registers.
 template <typename T, int DC>
-__global__ void __launch_bounds__(128, DC == 1 ? 4 : DC == 2 ? 2 : 1) xattn_mma_kernel(const XKernel A) {
-  constexpr int BM = 64, NT = 128, DP = DC * 64 + 4, NK = kXKeys / 8, NO = DC * 8;
+__global__ void __launch_bounds__(DC == 4 ? 256 : 128, DC <= 2 ? 2 : 1) xattn_mma_kernel(const XKernel A) {
+  constexpr int BM = 128, MT = DC == 4 ? 1 : 2, NT = DC == 4 ? 256 : 128, KT = kMmaKeys;
+  constexpr int DP = DC * 64 + 4, NK = KT / 8, NO = DC * 8, CH = DC * 16;
   extern __shared__ __align__(16) float smx[];
   float* Qs = smx;
   float* Ks = Qs + BM * DP;
-  float* Vs = Ks + kXKeys * DP;
+  float* Vs = Ks + KT * DP;
   const XSide& s = A.s;
-  const int tid = threadIdx.x, w = tid >> 5, g = (tid & 31) >> 2, t = tid & 3;
+  const int tid = threadIdx.x, wr = (tid >> 5) * 16 * MT, g = (tid & 31) >> 2, t = tid & 3;
   const int item = blockIdx.x / A.row_tiles, rt = blockIdx.x - item * A.row_tiles;
   const int bi = item / s.hkv, h = item - bi * s.hkv;
   const int64_t R = side_rows(s), r0 = static_cast<int64_t>(rt) * BM;
@@ -258,122 +265,155 @@ __global__ void __launch_bounds__(128, DC == 1 ? 4 : DC == 2 ? 2 : 1) xattn_mma_
   const T* kp = static_cast<const T*>(s.k) + bi * s.k_b + h * s.k_h;
   const T* vp = static_cast<const T*>(s.v) + bi * s.v_b + h * s.v_h;
   const uint8_t* mask = s.mask ? s.mask + bi * s.mask_stride : nullptr;
+  const bool busy = r0 + wr < R;  // a warp without rows only copies
   grid_dep_launch();  // the other side's launch, which needs none of this one's results, may run beside it
 
-  for (int i = tid; i < BM * DC * 16; i += NT) {
-    const int row = i / (DC * 16), d = (i - row * (DC * 16)) * 4;
+  for (int i = tid; i < BM * CH; i += NT) {
+    const int row = i / CH, d = (i - row * CH) * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r0 + row < R) v = load4(static_cast<const T*>(s.q) + q_offset(s, bi, h, side_row(s, r0 + row)), d, D, A.vec);
     *reinterpret_cast<float4*>(Qs + row * DP + d) = v;
   }
-  int lim[2];
-  float m[2], l[2], acc[NO][4];
+  int lim[MT][2], least = kend;
+  float m[MT][2], l[MT][2], acc[MT][NO][4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t r = r0 + w * 16 + g + 8 * i;
-    lim[i] = r < R ? min(kend, row_limit(s, side_row(s, r), len)) : 0;
-    m[i] = -INFINITY;
-    l[i] = 0.f;
+  for (int a = 0; a < MT; ++a) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t r = r0 + wr + a * 16 + g + 8 * i;
+      lim[a][i] = r < R ? min(kend, row_limit(s, side_row(s, r), len)) : kend;
+      least = min(least, lim[a][i]);
+      m[a][i] = -INFINITY;
+      l[a][i] = 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < NO; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[a][n][j] = 0.f;
   }
-#pragma unroll
-  for (int n = 0; n < NO; ++n)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[n][j] = 0.f;
   // fp32 rows that start on 16 bytes are copied asynchronously, the others through registers
   const bool async = sizeof(T) == 4 && A.vec && D % 4 == 0;
+  const int c_row = tid / CH, c_d = (tid % CH) * 4;  // this thread's first row and its columns
   auto load_tile = [&](float* dst, const T* base, int64_t stride, int k0) {
-    for (int i = tid; i < kXKeys * DC * 16; i += NT) {
-      const int row = i / (DC * 16), d = (i - row * (DC * 16)) * 4;
-      const int key = k0 + row;
-      const bool in = key < kend && (!mask || mask[key]);
-      if (async) {
-        cp_async16(dst + row * DP + d, in && d < D ? base + key * stride + d : base, in && d < D);
-      } else {
+    if (async) {
+      const T* src = base + (k0 + c_row) * stride + c_d;
+      const bool any = c_d < D;
+#pragma unroll 4
+      for (int row = c_row; row < KT; row += NT / CH, src += NT / CH * stride) {
+        const bool in = any && k0 + row < kend && (!mask || mask[k0 + row]);
+        cp_async16(dst + row * DP + c_d, in ? src : base, in);
+      }
+    } else {
+      for (int row = c_row; row < KT; row += NT / CH) {
+        const int key = k0 + row;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (in) v = load4(base + key * stride, d, D, A.vec);
-        *reinterpret_cast<float4*>(dst + row * DP + d) = v;
+        if (key < kend && (!mask || mask[key])) v = load4(base + key * stride, c_d, D, A.vec);
+        *reinterpret_cast<float4*>(dst + row * DP + c_d) = v;
       }
     }
   };
   // K of the next tile arrives while P V runs, V while the scores are formed
   if (kbeg < kend) load_tile(Ks, kp, s.k_t, kbeg);
-  for (int k0 = kbeg; k0 < kend; k0 += kXKeys) {
+  for (int k0 = kbeg; k0 < kend; k0 += KT) {
     cp_async_wait_all();
     __syncthreads();
     load_tile(Vs, vp, s.v_t, k0);
-    float sc[NK][4];
+    float sc[MT][NK][4];
+    if (busy) {
 #pragma unroll
-    for (int n = 0; n < NK; ++n)
+      for (int a = 0; a < MT; ++a)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sc[n][j] = 0.f;
-    scores_tf32<NK, DP>(sc, Qs + w * 16 * DP, Ks, D, g, t);
-    float mx[2] = {-INFINITY, -INFINITY};
+        for (int n = 0; n < NK; ++n)
 #pragma unroll
-    for (int n = 0; n < NK; ++n)
+          for (int j = 0; j < 4; ++j) sc[a][n][j] = 0.f;
+      scores_tf32<MT, NK, DP>(sc, Qs + wr * DP, Ks, D, g, t);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = k0 + n * 8 + 2 * t + (j & 1);
-        const bool hide = key >= lim[j >> 1] || (mask && !mask[key]);
-        sc[n][j] = hide ? -INFINITY : sc[n][j] * A.scale_log2;
-        mx[j >> 1] = fmaxf(mx[j >> 1], sc[n][j]);
+      for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[a][n][j] *= A.scale_log2;
+      if (mask || k0 + KT > least) {
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int key = k0 + n * 8 + 2 * t + j;
+            const bool hid = key >= kend || (mask && !mask[key]);
+#pragma unroll
+            for (int a = 0; a < MT; ++a)
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                if (hid || key >= lim[a][i]) sc[a][n][2 * i + j] = -INFINITY;
+          }
       }
-    float corr[2], mu[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-      const float mn = fmaxf(m[i], mx[i]);
-      mu[i] = mn == -INFINITY ? 0.f : mn;  // no key so far: every term is exactly 0
-      corr[i] = exp2f(m[i] - mu[i]);
-      m[i] = mn;
-      l[i] *= corr[i];  // this lane's columns; the four lanes' sums are joined at the end
+      for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < NK; ++n) mx = fmaxf(mx, fmaxf(sc[a][n][2 * i], sc[a][n][2 * i + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float mn = fmaxf(m[a][i], mx);
+          const float mu = mn == -INFINITY ? 0.f : mn;  // no key so far: every term is exactly 0
+          const float corr = ex2(m[a][i] - mu);
+          m[a][i] = mn;
+          float sum = 0.f;
+#pragma unroll
+          for (int n = 0; n < NK; ++n)
+#pragma unroll
+            for (int j = 2 * i; j < 2 * i + 2; ++j) {
+              sc[a][n][j] = ex2(sc[a][n][j] - mu);
+              sum += sc[a][n][j];
+            }
+          l[a][i] = l[a][i] * corr + sum;  // this lane's columns; the four lanes' sums are joined at the end
+#pragma unroll
+          for (int n = 0; n < NO; ++n) {
+            acc[a][n][2 * i] *= corr;
+            acc[a][n][2 * i + 1] *= corr;
+          }
+        }
     }
-#pragma unroll
-    for (int n = 0; n < NK; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        sc[n][j] = exp2f(sc[n][j] - mu[j >> 1]);
-        l[j >> 1] += sc[n][j];
-      }
-#pragma unroll
-    for (int n = 0; n < NO; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[n][j] *= corr[j >> 1];
     cp_async_wait_all();
     __syncthreads();
-    if (k0 + kXKeys < kend) load_tile(Ks, kp, s.k_t, k0 + kXKeys);
-    weigh_tf32<NK, NO, DP>(acc, sc, Vs, g, t);
+    if (k0 + KT < kend) load_tile(Ks, kp, s.k_t, k0 + KT);
+    if (busy) weigh_tf32<MT, NK, NO, DP>(acc, sc, Vs, g, t);
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    const int64_t r = r0 + w * 16 + g + 8 * i;
-    if (r >= R) continue;
-    const XRow x = side_row(s, r);
-    const int64_t fr = flat_row(s, bi, h, x);
-    const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
-    const float lse = l[i] == 0.f ? -INFINITY : m[i] + log2f(l[i]);
-    const bool piece = A.part_o != nullptr;
-    const int64_t pr = static_cast<int64_t>(blockIdx.y) * A.rows_all + fr;
-    float* pp = piece ? A.part_o + pr * D : nullptr;
-    T* po = piece ? nullptr : static_cast<T*>(A.out) + o_offset(s, bi, h, x);
+  for (int a = 0; a < MT; ++a)
 #pragma unroll
-    for (int n = 0; n < NO; ++n)
+    for (int i = 0; i < 2; ++i) {
+      float ls = l[a][i];
+      ls += __shfl_xor_sync(0xffffffffu, ls, 1);
+      ls += __shfl_xor_sync(0xffffffffu, ls, 2);
+      const int64_t r = r0 + wr + a * 16 + g + 8 * i;
+      if (r >= R) continue;
+      const XRow x = side_row(s, r);
+      const int64_t fr = flat_row(s, bi, h, x);
+      const float inv = ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls);
+      const float lse = ls == 0.f ? -INFINITY : m[a][i] + log2f(ls);
+      const bool piece = A.part_o != nullptr;
+      const int64_t pr = static_cast<int64_t>(blockIdx.y) * A.rows_all + fr;
+      float* pp = piece ? A.part_o + pr * D : nullptr;
+      T* po = piece ? nullptr : static_cast<T*>(A.out) + o_offset(s, bi, h, x);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int d = n * 8 + 2 * t + j;
-        const float v = acc[n][2 * i + j] * inv;
-        if (d < D) {
-          if (piece) pp[d] = v;
-          else store1(po + d, v);
+      for (int n = 0; n < NO; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int d = n * 8 + 2 * t + j;
+          const float v = acc[a][n][2 * i + j] * inv;
+          if (d < D) {
+            if (piece) pp[d] = v;
+            else store1(po + d, v);
+          }
         }
+      if (t == 0) {
+        if (piece) A.part_lse[pr] = lse;
+        else if (A.lse != nullptr) A.lse[fr] = lse;
       }
-    if (t == 0) {
-      if (piece) A.part_lse[pr] = lse;
-      else if (A.lse != nullptr) A.lse[fr] = lse;
     }
-  }
   grid_dep_wait();  // ends after the launch it ran beside: what follows needs both
 }
 
@@ -425,32 +465,32 @@ __global__ void __launch_bounds__(256) combine_pieces_kernel(const float* __rest
 
 // ---------------------------------------------------------------- host side
 
-struct SimtPlan {
+struct GeneralPlan {
   int bm, dc, splits[2], chunk[2], row_tiles[2], pieces;
 };
 
-SimtPlan simt_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n) {
-  SimtPlan p = {};
+GeneralPlan general_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n) {
+  GeneralPlan p = {};
   p.dc = a->head_dim <= 64 ? 1 : a->head_dim <= 128 ? 2 : 4;
   int64_t most = 0;
   for (int i = 0; i < n; ++i) most = most > side_rows(s[i]) ? most : side_rows(s[i]);
-  // 16-row CTAs where a 64-row tile would be mostly padding
-  p.bm = most <= 32 ? 16 : 64;
-  // resident CTAs of the 64-row form: by registers and shared memory
-  const int64_t slots = (p.dc == 1 ? 4ll : p.dc == 2 ? 2ll : 1ll) * sm_count();
+  // 16-row CTAs where a 128-row tile would be mostly padding
+  p.bm = most <= 32 ? 16 : 128;
+  const int resident = p.dc <= 2 ? 2 : 1;  // CTAs an SM: by registers and shared memory
+  const int64_t keys = p.bm == 16 ? kXKeys : kMmaKeys;
   for (int i = 0; i < n; ++i) {
     p.row_tiles[i] = static_cast<int>((side_rows(s[i]) + p.bm - 1) / p.bm);
     const int64_t ctas = static_cast<int64_t>(p.row_tiles[i]) * s[i].nb * s[i].hkv;
-    const int64_t tiles = (s[i].klen + kXKeys - 1) / kXKeys;
+    const int64_t tiles = (s[i].klen + keys - 1) / keys;
     int64_t per;
     if (p.bm == 16) {  // bound by the reads of K and V: three CTAs an SM (walk_steps' fewer: 46 us against 31 at 4096 keys)
       int64_t splits = ctas > 0 ? (3ll * sm_count() + ctas - 1) / ctas : 1;
       splits = splits < 128 ? splits : 128;
       per = tiles > splits ? (tiles + splits - 1) / splits : 1;
     } else {
-      per = walk_steps(ctas, tiles, slots, 128);
+      per = walk_steps(ctas, tiles, sm_count(), resident, 128);
     }
-    p.chunk[i] = static_cast<int>(per * kXKeys);
+    p.chunk[i] = static_cast<int>(per * keys);
     p.splits[i] = static_cast<int>(tiles > 0 ? (tiles + per - 1) / per : 1);
     p.pieces += p.splits[i];
   }
@@ -473,14 +513,16 @@ int attention_launch(void (*kern)(XKernel), int threads, size_t smem, const XKer
 
 template <typename T, int DC>
 int attention_dispatch(const XKernel& A, int bm, int splits, bool behind, cudaStream_t st) {
-  const size_t smem = sizeof(float) * static_cast<size_t>(bm + 2 * kXKeys) * (DC * 64 + 4);
-  if (bm == 64) return attention_launch(xattn_mma_kernel<T, DC>, 128, smem, A, splits, behind, st);
-  return attention_launch(xattn_simt_kernel<T, 16, 128, DC>, 128, smem + sizeof(float) * 16 * (kXKeys + 4), A, splits,
-                          behind, st);
+  const size_t row = sizeof(float) * (DC * 64 + 4);
+  if (bm == 128)
+    return attention_launch(xattn_mma_kernel<T, DC>, DC == 4 ? 256 : 128, row * (128 + 2 * kMmaKeys), A, splits, behind,
+                            st);
+  return attention_launch(xattn_few_kernel<T, 16, 128, DC>, 128,
+                          row * (16 + 2 * kXKeys) + sizeof(float) * 16 * (kXKeys + 4), A, splits, behind, st);
 }
 
 template <typename T>
-int simt_dispatch(const XKernel& A, int bm, int dc, int splits, bool behind, cudaStream_t st) {
+int general_dispatch(const XKernel& A, int bm, int dc, int splits, bool behind, cudaStream_t st) {
   if (dc == 1) return attention_dispatch<T, 1>(A, bm, splits, behind, st);
   if (dc == 2) return attention_dispatch<T, 2>(A, bm, splits, behind, st);
   return attention_dispatch<T, 4>(A, bm, splits, behind, st);
@@ -498,12 +540,12 @@ bool four_aligned(const trnsparse_attention_args* a) {
   return !(p & m) && !(st & 3);
 }
 
-int simt_forward(const trnsparse_attention_args* a, bool prefix, void* ws, cudaStream_t st) {
+int general_forward(const trnsparse_attention_args* a, bool prefix, void* ws, cudaStream_t st) {
   XSide s[2];
   int n = 0;
   int rc = make_sides(a, prefix, s, &n);
   if (rc) return rc;
-  const SimtPlan p = simt_plan(a, s, n);
+  const GeneralPlan p = general_plan(a, s, n);
   const int64_t rows = a->batch * a->q_heads * a->q_len;
   float* part_o = static_cast<float*>(ws);
   float* part_lse = part_o + (p.pieces > 1 ? p.pieces * rows * a->head_dim : 0);
@@ -524,19 +566,19 @@ int simt_forward(const trnsparse_attention_args* a, bool prefix, void* ws, cudaS
     A.vec = four_aligned(a);
     A.scale = static_cast<float>(a->scale);
     A.scale_log2 = static_cast<float>(a->scale * 1.4426950408889634);
-    rc = a->dtype == TRNSPARSE_F32 ? simt_dispatch<float>(A, p.bm, p.dc, p.splits[i], i > 0, st)
-                                   : simt_dispatch<__nv_bfloat16>(A, p.bm, p.dc, p.splits[i], i > 0, st);
+    rc = a->dtype == TRNSPARSE_F32 ? general_dispatch<float>(A, p.bm, p.dc, p.splits[i], i > 0, st)
+                                   : general_dispatch<__nv_bfloat16>(A, p.bm, p.dc, p.splits[i], i > 0, st);
     if (rc) return rc;
     piece += p.splits[i];
   }
   return p.pieces > 1 ? combine_pieces(part_o, part_lse, p.pieces, a, st) : TRNSPARSE_OK;
 }
 
-size_t simt_workspace(const trnsparse_attention_args* a, bool prefix) {
+size_t general_workspace(const trnsparse_attention_args* a, bool prefix) {
   XSide s[2];
   int n = 0;
   if (make_sides(a, prefix, s, &n)) return 0;
-  const SimtPlan p = simt_plan(a, s, n);
+  const GeneralPlan p = general_plan(a, s, n);
   if (p.pieces <= 1) return 0;
   return sizeof(float) * static_cast<size_t>(p.pieces) * a->batch * a->q_heads * a->q_len * (a->head_dim + 1);
 }
@@ -635,7 +677,7 @@ bool nothing(const trnsparse_attention_args* a) { return a->batch * a->q_heads *
 
 size_t attention_workspace(const trnsparse_attention_args* a, bool prefix) {
   if (check_attention(a, "attention") || nothing(a)) return 0;
-  return xattn_tc_ok(a, prefix) ? xattn_tc_workspace(a, prefix) : simt_workspace(a, prefix);
+  return xattn_tc_ok(a, prefix) ? xattn_tc_workspace(a, prefix) : general_workspace(a, prefix);
 }
 
 int attention_run(const trnsparse_attention_args* a, bool prefix, void* ws, size_t ws_bytes, void* stream,
@@ -650,7 +692,7 @@ int attention_run(const trnsparse_attention_args* a, bool prefix, void* ws, size
   TSB_REQUIRE(ws_bytes >= need && (need == 0 || ws), "%s: workspace too small (%zu bytes, needs %zu)", what, ws_bytes,
               need);
   return xattn_tc_ok(a, prefix) ? xattn_tc_forward(a, prefix, ws, as_stream(stream))
-                                : simt_forward(a, prefix, ws, as_stream(stream));
+                                : general_forward(a, prefix, ws, as_stream(stream));
 }
 
 }  // namespace

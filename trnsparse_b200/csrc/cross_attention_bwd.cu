@@ -1,5 +1,5 @@
-// Backward of cross attention on CUDA cores (fp32 at any head_dim up to 256,
-// and the bf16 shapes the tensor-core kernels do not take). With the forward's
+// Backward of cross attention for fp32 at any head_dim up to 256, and for the
+// bf16 shapes the tcgen05 kernels do not take. With the forward's
 // row log-sum-exp (base 2) and D = rowsum(dO o O):
 //   P = 2^(s2 - lse),  dP = dO V^T,  dS = P (dP - D),
 //   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO,
@@ -8,14 +8,18 @@
 // to zero, whatever the padding holds; a row without keys (lse = -inf) has
 // only hidden keys.
 //
-// Two kernels, each owning what it writes, so sums have one fixed order (no
-// atomics): rows (dQ: a tile of packed query rows walks the keys) and columns
-// (dK, dV: a tile of keys walks every query row of its group). Both recompute
-// P: five products of the mathematics cost seven, which buys repeatable results
-// and no traffic for dQ. fp32 FMA bounds both; tiles of 64 (32 above head_dim
-// 128, where four 64-row tiles would not fit in shared memory) with RM x RM
-// scores a thread. Where tiles are fewer than SMs the walk is cut into parts
-// whose fp32 sums a last kernel adds in order.
+// Two walks side by side in one launch, each owning what it writes, so sums have
+// one fixed order (no atomics): rows (dQ: a tile of packed query rows walks the
+// keys) and columns (dK, dV: a tile of keys walks every query row of its group).
+// Both recompute P: five products of the mathematics cost seven, which buys
+// repeatable results and no traffic for dQ. Where tiles are fewer than SMs the
+// walks are cut into parts whose fp32 sums a last kernel adds in order.
+//
+// What bounds it: the tensor cores' tf32 rate (3xTF32 in xattn_tf32.cuh), kept 64%
+// busy with two warps a scheduler; the rest goes to the splits and to waits inside a
+// warp's chain of scores, P and sums. 2 x 16/16 heads, 1024 x 1024 x 64: 656 us,
+// 46 TFLOP/s of the seven products (CUDA cores before: 1171 us; row by row tiles of
+// 16 rows a warp, each walk its own launch: 698); 16/4 heads at head_dim 128: 1237 us.
 #include "xattn_tf32.cuh"
 
 namespace tsb {
@@ -45,6 +49,13 @@ __device__ __forceinline__ float4 bload4(const T* row, int d, int D, bool vec) {
 }
 constexpr int kBwdWalk = 32;  // walked rows a step
 
+// One of the two walks: a CTA each for `tiles` tiles of every item and `parts` ranges of the walked rows.
+struct BWalk {
+  int tiles, chunk, parts;
+  unsigned ctas;       // 0: not wanted
+  float *part0, *part1;  // fp32 parts (null: one part, written to the outputs)
+};
+
 struct BKernel {
   XSide s;  // o_*: strides of dq here
   const void* dout;
@@ -52,9 +63,9 @@ struct BKernel {
   const float *lse, *delta;
   void *dq, *dk, *dv;
   int64_t dk_s[3], dv_s[3];
-  float *part0, *part1;  // fp32 parts (null: one part, written to the outputs)
-  int64_t rows_all;      // rows of one part
-  int D, tiles, chunk, vec;
+  BWalk rows, cols;
+  int64_t all_rows, all_keys;  // rows of one part
+  int D, vec;
   float scale, scale_log2;
 };
 
@@ -76,28 +87,38 @@ __global__ void __launch_bounds__(256) xattn_delta_kernel(const T* __restrict__ 
   if (lane == 0) delta[row] = s;
 }
 
-// 64 fixed rows (queries, or keys with COLS) a CTA, 16 a warp; WT walked rows a step. Above head_dim 128 the sums of
-// dK and of dV have 128 registers a thread each: eight warps, the second four hold dV.
+// Up to head_dim 64 four warps of 32 fixed rows, so that each split of a walked element feeds two products; up to 128
+// eight of 16, as 32 rows' sums would not fit in registers; both with the next walked rows copied behind the arithmetic.
+// Above that, 64 rows (shared memory) and eight warps that share them in pairs: for dQ each takes half the walked keys,
+// the sums are joined at the end; for dK and dV one has each.
+template <int DC>
+struct BShape {
+  static constexpr int kThreads = DC == 1 ? 128 : 256, kTiles16 = DC == 1 ? 2 : 1, kRows = DC == 4 ? 64 : 128;
+  static constexpr int kStages = DC == 4 ? 1 : 2, kResident = DC == 1 ? 2 : 1, kStride = DC * 64 + 4;
+  static constexpr int kSmem = 4 * (2 * kRows * kStride + kStages * 2 * (kBwdWalk * kStride + kBwdWalk));
+};
+
 template <typename T, int DC, bool COLS>
-__global__ void __launch_bounds__(COLS && DC == 4 ? 256 : 128, DC == 1 ? 4 : DC == 2 ? 2 : 1)
-    xattn_bwd_mma_kernel(const BKernel A) {
-  constexpr int BT = 64, WT = kBwdWalk, NT = COLS && DC == 4 ? 256 : 128;
-  constexpr int DP = DC * 64 + 4, NW = WT / 8, NO = DC * 8, CH = DC * 16;
+__device__ __forceinline__ void bwd_walk(const BKernel& A, const BWalk& W, unsigned cta, float* smb) {
+  using S = BShape<DC>;
+  constexpr int MT = S::kTiles16, BT = S::kRows, WT = kBwdWalk, NT = S::kThreads, STAGES = S::kStages;
+  constexpr bool HALF = !COLS && DC == 4;  // a warp takes half the walked rows
+  constexpr int DP = S::kStride, WW = HALF ? WT / 2 : WT, NW = WW / 8, NO = DC * 8, CH = DC * 16;
+  constexpr int XS = 2 * (WT * DP + WT);  // floats of a stage
   constexpr bool BOTH = COLS && DC != 4;
-  extern __shared__ __align__(16) float smb[];
-  float* F1 = smb;             // fixed: Q (rows) or K (columns)
-  float* F2 = F1 + BT * DP;    // fixed: dO or V
-  float* X1 = F2 + BT * DP;    // walked: K or Q
-  float* X2 = X1 + WT * DP;    // walked: V or dO
-  float* st_lse = X2 + WT * DP;  // of the walked queries (columns)
-  float* st_delta = st_lse + WT;
+  float* F1 = smb;           // fixed: Q (rows) or K (columns)
+  float* F2 = F1 + BT * DP;  // fixed: dO or V
+  float* X = F2 + BT * DP;   // walked, a stage: K or Q, V or dO, then (columns) the queries' lse and delta
   const XSide& s = A.s;
   const int tid = threadIdx.x, g = (tid & 31) >> 2, t = tid & 3;
-  const int f0 = (tid >> 5 & 3) * 16;                // this warp's fixed rows
-  const bool second = COLS && DC == 4 && tid >= 128;  // holds dV
-  const int item = blockIdx.x / A.tiles, tile = blockIdx.x - item * A.tiles;
+  const int f0 = (tid >> 5) % (BT / 16 / MT) * 16 * MT;  // this warp's fixed rows
+  const bool upper = DC == 4 && tid >= 128;
+  const bool second = COLS && upper;  // holds dV
+  const int x0 = HALF && upper ? WW : 0;
+  const unsigned line = cta / W.parts, part = cta - line * W.parts;
+  const int item = line / W.tiles, tile = line - item * W.tiles;
   const int bi = item / s.hkv, h = item - bi * s.hkv;
-  const int64_t R = side_rows(s);
+  const int64_t R = side_rows(s), fix0 = static_cast<int64_t>(tile) * BT;
   const int D = A.D, len = side_len(s, bi);
   const T* qp = static_cast<const T*>(s.q) + bi * s.q_bi + static_cast<int64_t>(h) * s.G * s.q_h;
   const T* gp = static_cast<const T*>(A.dout) + bi * A.g_b + static_cast<int64_t>(h) * s.G * A.g_h;
@@ -105,148 +126,227 @@ __global__ void __launch_bounds__(COLS && DC == 4 ? 256 : 128, DC == 1 ? 4 : DC 
   const T* vp = static_cast<const T*>(s.v) + bi * s.v_b + h * s.v_h;
   const int64_t stat0 = (static_cast<int64_t>(bi) * s.hkv + h) * s.G * s.T;  // flat row of packed row 0
   const uint8_t* mask = s.mask ? s.mask + bi * s.mask_stride : nullptr;
+  const bool busy = fix0 + f0 < (COLS ? len : R);  // a warp without rows only copies
   // fp32 rows that start on 16 bytes are copied asynchronously, the others through registers
   const bool async = sizeof(T) == 4 && A.vec && D % 4 == 0;
-  auto copy4 = [&](float* dst, const T* row, int d, bool in) {
+  const int c_row = tid / CH, c_d = (tid % CH) * 4;  // this thread's first row and its columns
+  auto copy4 = [&](float* dst, const T* row, bool in) {
     if (async) {
-      cp_async16(dst, in && d < D ? row + d : static_cast<const T*>(s.q), in && d < D);
+      in = in && c_d < D;
+      cp_async16(dst + c_d, in ? row + c_d : static_cast<const T*>(s.q), in);
     } else {
-      *reinterpret_cast<float4*>(dst) = in ? bload4(row, d, D, A.vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+      *reinterpret_cast<float4*>(dst + c_d) = in ? bload4(row, c_d, D, A.vec) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   };
   auto load_q = [&](float* q, float* go, int64_t r0, int n) {
-    for (int i = tid; i < n * CH; i += NT) {
-      const int row = i / CH, d = (i - row * CH) * 4;
+    for (int row = c_row; row < n; row += NT / CH) {
       const bool in = r0 + row < R;
       const unsigned r = in ? static_cast<unsigned>(r0 + row) : 0u, hg = r / s.T, tt = r - hg * s.T;
-      copy4(q + row * DP + d, qp + hg * s.q_h + tt * s.q_t, d, in);
-      copy4(go + row * DP + d, gp + hg * A.g_h + tt * A.g_t, d, in);
+      copy4(q + row * DP, qp + hg * s.q_h + tt * s.q_t, in);
+      copy4(go + row * DP, gp + hg * A.g_h + tt * A.g_t, in);
     }
   };
   auto load_kv = [&](float* k, float* v, int k0, int n) {
-    for (int i = tid; i < n * CH; i += NT) {
-      const int row = i / CH, d = (i - row * CH) * 4, key = k0 + row;
+    for (int row = c_row; row < n; row += NT / CH) {
+      const int key = k0 + row;
       const bool in = key < len && (!mask || mask[key]);
-      copy4(k + row * DP + d, kp + key * s.k_t, d, in);
-      copy4(v + row * DP + d, vp + key * s.v_t, d, in);
+      copy4(k + row * DP, kp + key * s.k_t, in);
+      copy4(v + row * DP, vp + key * s.v_t, in);
     }
   };
   if (COLS) load_kv(F1, F2, tile * BT, BT);
-  else load_q(F1, F2, static_cast<int64_t>(tile) * BT, BT);
-  float row_lse[2], row_delta[2];  // rows: of this lane's queries
-  bool hide_row[2];                // columns: this lane's keys
+  else load_q(F1, F2, fix0, BT);
+  grid_dep_wait();  // the row sums
+  float row_lse[MT][2], row_delta[MT][2];  // rows: of this lane's queries
+  bool hide_row[MT][2], hide_any = false;  // columns: this lane's keys
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t r = static_cast<int64_t>(tile) * BT + f0 + g + 8 * i;
-    row_lse[i] = INFINITY;  // rows past the last: P = 0
-    row_delta[i] = 0.f;
-    hide_row[i] = false;
-    if (COLS) {
-      hide_row[i] = r >= len || (mask && !mask[r]);
-    } else if (r < R) {
-      row_lse[i] = A.lse[stat0 + r];
-      row_delta[i] = A.delta[stat0 + r];
-    }
-  }
-  float acc0[NO][4], acc1[BOTH ? NO : 1][4];
+  for (int a = 0; a < MT; ++a)
 #pragma unroll
-  for (int n = 0; n < NO; ++n)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      acc0[n][j] = 0.f;
-      if constexpr (BOTH) acc1[n][j] = 0.f;
-    }
-  // a walk over keys stops at the kept length; a key tile with no kept key walks nothing
-  const int64_t wend = COLS ? (tile * BT < len ? R : 0) : len;
-  const int64_t w0 = static_cast<int64_t>(blockIdx.y) * A.chunk;
-  const int64_t w1 = wend < w0 + A.chunk ? wend : w0 + A.chunk;
-  for (int64_t w = w0; w < w1; w += WT) {
-    __syncthreads();
-    if (COLS) {
-      load_q(X1, X2, w, WT);
-      if (tid < WT) {
-        const bool in = w + tid < R;
-        st_lse[tid] = in ? A.lse[stat0 + w + tid] : INFINITY;
-        st_delta[tid] = in ? A.delta[stat0 + w + tid] : 0.f;
+    for (int i = 0; i < 2; ++i) {
+      const int64_t r = fix0 + f0 + a * 16 + g + 8 * i;
+      row_lse[a][i] = INFINITY;  // rows past the last: P = 0
+      row_delta[a][i] = 0.f;
+      hide_row[a][i] = false;
+      if (COLS) {
+        hide_row[a][i] = r >= len || (mask && !mask[r]);
+        hide_any = hide_any || hide_row[a][i];
+      } else if (r < R) {
+        row_lse[a][i] = A.lse[stat0 + r];
+        row_delta[a][i] = A.delta[stat0 + r];
       }
-    } else {
-      load_kv(X1, X2, static_cast<int>(w), WT);
     }
-    cp_async_wait_all();
-    __syncthreads();
-    float sc[NW][4], dp[NW][4];  // scores, then P; dP, then dS: fixed rows by walked rows
+  float acc0[MT][NO][4], acc1[MT][BOTH ? NO : 1][4];
 #pragma unroll
-    for (int n = 0; n < NW; ++n)
+  for (int a = 0; a < MT; ++a)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sc[n][j] = dp[n][j] = 0.f;
-    scores_tf32<NW, DP>(sc, F1 + f0 * DP, X1, D, g, t);
-    if (!second) scores_tf32<NW, DP>(dp, F2 + f0 * DP, X2, D, g, t);
+    for (int n = 0; n < NO; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc0[a][n][j] = 0.f;
+        if constexpr (BOTH) acc1[a][n][j] = 0.f;
+      }
+  auto step = [&](const float* x, int64_t w) {
+    const float *X1 = x + x0 * DP, *X2 = X1 + WT * DP;
+    const float *st_lse = x + 2 * WT * DP, *st_delta = st_lse + WT;
+    w += x0;
+    float sc[MT][NW][4], dp[MT][NW][4];  // scores, then P; dP, then dS: fixed rows by walked rows
+#pragma unroll
+    for (int a = 0; a < MT; ++a)
+#pragma unroll
+      for (int n = 0; n < NW; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[a][n][j] = dp[a][n][j] = 0.f;
+    scores_tf32<MT, NW, DP>(sc, F1 + f0 * DP, X1, D, g, t);
+    if (!second) scores_tf32<MT, NW, DP>(dp, F2 + f0 * DP, X2, D, g, t);
+    const bool some = COLS ? hide_any : mask || w + WW > len;
 #pragma unroll
     for (int n = 0; n < NW; ++n)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = j >> 1, x = n * 8 + 2 * t + (j & 1);
-        bool hide = hide_row[i];
-        if (!COLS) hide = w + x >= len || (mask && !mask[w + x]);
-        const float p = hide ? 0.f : exp2f(fmaf(sc[n][j], A.scale_log2, -(COLS ? st_lse[x] : row_lse[i])));
-        dp[n][j] = hide ? 0.f : p * (dp[n][j] - (COLS ? st_delta[x] : row_delta[i]));
-        sc[n][j] = p;
-      }
-    if constexpr (BOTH) weigh_tf32<NW, NO, DP>(acc1, sc, X2, g, t);
-    if (second) weigh_tf32<NW, NO, DP>(acc0, sc, X2, g, t);
-    else weigh_tf32<NW, NO, DP>(acc0, dp, X1, g, t);
-  }
+        bool hide = false;
+        if (!COLS && some) hide = w + x >= len || (mask && !mask[w + x]);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t r = static_cast<int64_t>(tile) * BT + f0 + g + 8 * i;
-    if (r >= (COLS ? static_cast<int64_t>(s.klen) : R)) continue;
-    const int64_t fr = COLS ? (static_cast<int64_t>(bi) * s.hkv + h) * s.klen + r : stat0 + r;
-    const int64_t at = (static_cast<int64_t>(blockIdx.y) * A.rows_all + fr) * D;
-    const bool piece = A.part0 != nullptr;
-    T *o0 = nullptr, *o1 = nullptr;
-    if (!piece && COLS) {
-      o0 = static_cast<T*>(A.dk) + bi * A.dk_s[0] + h * A.dk_s[1] + r * A.dk_s[2];
-      o1 = static_cast<T*>(A.dv) + bi * A.dv_s[0] + h * A.dv_s[1] + r * A.dv_s[2];
-    } else if (!piece) {
-      o0 = static_cast<T*>(A.dq) + o_offset(s, bi, h, side_row(s, r));
+        for (int a = 0; a < MT; ++a) {
+          if (COLS) hide = hide_row[a][i];
+          const float p =
+              hide ? 0.f : ex2(fmaf(sc[a][n][j], A.scale_log2, -(COLS ? st_lse[x] : row_lse[a][i])));
+          dp[a][n][j] = hide ? 0.f : p * (dp[a][n][j] - (COLS ? st_delta[x] : row_delta[a][i]));
+          sc[a][n][j] = p;
+        }
+      }
+    if constexpr (BOTH) weigh_tf32<MT, NW, NO, DP>(acc1, sc, X2, g, t);
+    if (second) weigh_tf32<MT, NW, NO, DP>(acc0, sc, X2, g, t);
+    else weigh_tf32<MT, NW, NO, DP>(acc0, dp, X1, g, t);
+  };
+  // a walk over keys stops at the kept length; a key tile with no kept key walks nothing
+  const int64_t wend = COLS ? (fix0 < len ? R : 0) : len;
+  const int64_t w0 = static_cast<int64_t>(part) * W.chunk;
+  const int64_t w1 = wend < w0 + W.chunk ? wend : w0 + W.chunk;
+  float stat[2];  // columns: lse and delta of query w + tid, on their way to a stage
+  auto copy_walked = [&](float* x, int64_t w) {
+    if (COLS) {
+      load_q(x, x + WT * DP, w, WT);
+      const bool in = tid < WT && w + tid < R;
+      stat[0] = in ? A.lse[stat0 + w + tid] : INFINITY;  // rows past the last: P = 0
+      stat[1] = in ? A.delta[stat0 + w + tid] : 0.f;
+    } else {
+      load_kv(x, x + WT * DP, static_cast<int>(w), WT);
     }
-    auto put = [&](float* part, T* o, int d, float v) {
-      if (piece) part[at + d] = v;
-      else bstore(o + d, v);
-    };
+  };
+  auto put_stats = [&](float* x) {
+    if (COLS && tid < WT) {
+      x[2 * WT * DP + tid] = stat[0];
+      x[2 * WT * DP + WT + tid] = stat[1];
+    }
+  };
+  if (STAGES == 2 && w0 < w1) {
+    copy_walked(X, w0);
+    put_stats(X);
+  }
+  int stage = 0;
+  for (int64_t w = w0; w < w1; w += WT) {
+    float* X1 = X + stage * XS;
+    if (STAGES == 1) {
+      __syncthreads();
+      copy_walked(X1, w);
+      put_stats(X1);
+    }
+    cp_async_wait_all();
+    __syncthreads();  // this stage has landed and the other one is read
+    const bool more = STAGES == 2 && w + WT < w1;
+    stage = STAGES == 2 ? stage ^ 1 : 0;
+    if (more) copy_walked(X + stage * XS, w + WT);
+    if (busy) step(X1, w);
+    if (more) put_stats(X + stage * XS);
+  }
+  if constexpr (HALF) {  // both halves' sums, through the fixed tile
+    __syncthreads();
+    if (upper) {
+#pragma unroll
+      for (int n = 0; n < NO; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) F1[(f0 + g + 8 * (j >> 1)) * DP + n * 8 + 2 * t + (j & 1)] = acc0[0][n][j];
+    }
+    __syncthreads();
+    if (upper) return;
 #pragma unroll
     for (int n = 0; n < NO; ++n)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int d = n * 8 + 2 * t + j;
-        if (d >= D) continue;
-        if (second) put(A.part1, o1, d, acc0[n][2 * i + j]);
-        else put(A.part0, o0, d, acc0[n][2 * i + j] * A.scale);
-        if constexpr (BOTH) put(A.part1, o1, d, acc1[n][2 * i + j]);
-      }
+      for (int j = 0; j < 4; ++j) acc0[0][n][j] += F1[(f0 + g + 8 * (j >> 1)) * DP + n * 8 + 2 * t + (j & 1)];
   }
+#pragma unroll
+  for (int a = 0; a < MT; ++a)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t r = fix0 + f0 + a * 16 + g + 8 * i;
+      if (r >= (COLS ? static_cast<int64_t>(s.klen) : R)) continue;
+      const int64_t fr = COLS ? (static_cast<int64_t>(bi) * s.hkv + h) * s.klen + r : stat0 + r;
+      const int64_t at = (static_cast<int64_t>(part) * (COLS ? A.all_keys : A.all_rows) + fr) * D;
+      const bool piece = W.part0 != nullptr;
+      T *o0 = nullptr, *o1 = nullptr;
+      if (!piece && COLS) {
+        o0 = static_cast<T*>(A.dk) + bi * A.dk_s[0] + h * A.dk_s[1] + r * A.dk_s[2];
+        o1 = static_cast<T*>(A.dv) + bi * A.dv_s[0] + h * A.dv_s[1] + r * A.dv_s[2];
+      } else if (!piece) {
+        o0 = static_cast<T*>(A.dq) + o_offset(s, bi, h, side_row(s, r));
+      }
+      auto put = [&](float* pp, T* o, int d, float v) {
+        if (piece) pp[at + d] = v;
+        else bstore(o + d, v);
+      };
+#pragma unroll
+      for (int n = 0; n < NO; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int d = n * 8 + 2 * t + j;
+          if (d >= D) continue;
+          if (second) put(W.part1, o1, d, acc0[a][n][2 * i + j]);
+          else put(W.part0, o0, d, acc0[a][n][2 * i + j] * A.scale);
+          if constexpr (BOTH) put(W.part1, o1, d, acc1[a][n][2 * i + j]);
+        }
+    }
 }
 
-// out[b, h, t, :] = sum of the parts, in order.
+// The columns' CTAs first: their steps are the longer ones.
+template <typename T, int DC>
+__global__ void __launch_bounds__(BShape<DC>::kThreads, BShape<DC>::kResident) xattn_bwd_mma_kernel(const BKernel A) {
+  extern __shared__ __align__(16) float smb[];
+  if (blockIdx.x < A.cols.ctas) bwd_walk<T, DC, true>(A, A.cols, blockIdx.x, smb);
+  else bwd_walk<T, DC, false>(A, A.rows, blockIdx.x - A.cols.ctas, smb);
+}
+
+// out[b, h, t, :] = sum of the parts, in order, for up to three tensors.
+struct BSum {
+  const float* part[3];
+  void* out[3];
+  int64_t rows[3], o[3][3];
+  int parts[3], H[3], L[3], D;
+};
 template <typename T>
-__global__ void __launch_bounds__(256) xattn_sum_parts_kernel(const float* __restrict__ part, int parts, int64_t rows,
-                                                              T* out, int H, int L, int D, int64_t o_b, int64_t o_h,
-                                                              int64_t o_t) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= rows * D) return;
-  const int64_t row = i / D;
-  const int d = static_cast<int>(i - row * D);
-  float s = 0.f;
-  for (int p = 0; p < parts; ++p) s += part[p * rows * D + i];
-  const int64_t bh = row / L, t = row - bh * L, b = bh / H, h = bh - b * H;
-  bstore(out + b * o_b + h * o_h + t * o_t + d, s);
+__global__ void __launch_bounds__(256) xattn_sum_parts_kernel(const BSum A) {
+  int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  grid_dep_wait();
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const int64_t n = A.rows[k] * A.D;
+    if (i >= 0 && i < n) {
+      const int64_t row = i / A.D;
+      const int d = static_cast<int>(i - row * A.D);
+      float s = 0.f;
+      for (int p = 0; p < A.parts[k]; ++p) s += A.part[k][p * n + i];
+      const int64_t bh = row / A.L[k], t = row - bh * A.L[k], b = bh / A.H[k], h = bh - b * A.H[k];
+      bstore(static_cast<T*>(A.out[k]) + b * A.o[k][0] + h * A.o[k][1] + t * A.o[k][2] + d, s);
+    }
+    i -= n;
+  }
 }
 
 // ---------------------------------------------------------------- host side
 
 struct BPlan {
-  int dc, parts[2], chunk[2], tiles[2];  // [0] rows (dQ), [1] columns (dK, dV)
-  size_t ws;
+  int dc, tiles[2], parts[2], chunk[2];  // [0] rows (dQ), [1] columns (dK, dV)
+  size_t at[2], ws;                      // the parts' place in the workspace, behind the row sums
 };
 
 BPlan bwd_plan(const trnsparse_attention_args* a, const XSide& s) {
@@ -254,57 +354,35 @@ BPlan bwd_plan(const trnsparse_attention_args* a, const XSide& s) {
   p.dc = a->head_dim <= 64 ? 1 : a->head_dim <= 128 ? 2 : 4;
   const int64_t R = side_rows(s);
   const int64_t fixed[2] = {R, s.klen}, walk[2] = {s.klen, R};
-  const int64_t slots = (p.dc == 1 ? 4ll : p.dc == 2 ? 2ll : 1ll) * sm_count();  // resident CTAs
+  const int resident = p.dc == 1 ? 2 : 1, bt = p.dc == 4 ? 64 : 128;
   const int64_t rows = a->batch * a->q_heads * a->q_len, keys = a->batch * a->kv_heads * a->k_len;
-  p.ws = sizeof(float) * static_cast<size_t>(rows);
-  size_t parts_ws = 0;
+  p.ws = (sizeof(float) * static_cast<size_t>(rows) + 255) & ~static_cast<size_t>(255);
   for (int i = 0; i < 2; ++i) {
-    p.tiles[i] = static_cast<int>((fixed[i] + 63) / 64);
+    p.tiles[i] = static_cast<int>((fixed[i] + bt - 1) / bt);
     const int64_t ctas = static_cast<int64_t>(p.tiles[i]) * s.nb * s.hkv, steps = (walk[i] + kBwdWalk - 1) / kBwdWalk;
-    const int64_t per = walk_steps(ctas, steps, slots, 32);
+    // both walks run side by side: three and four of the seven products
+    const int64_t per = walk_steps(ctas, steps, sm_count() * (3 + i) / 7, resident, 32);
     p.chunk[i] = static_cast<int>(per * kBwdWalk);
     p.parts[i] = static_cast<int>(steps > 0 ? (steps + per - 1) / per : 1);
-    if (p.parts[i] > 1) {
-      const size_t b = sizeof(float) * static_cast<size_t>(p.parts[i]) * a->head_dim * (i ? 2 * keys : rows);
-      parts_ws = parts_ws > b ? parts_ws : b;  // rows and columns run one after the other
-    }
+    p.at[i] = p.ws;
+    if (p.parts[i] > 1)
+      p.ws += (sizeof(float) * static_cast<size_t>(p.parts[i]) * a->head_dim * (i ? 2 * keys : rows) + 255) &
+              ~static_cast<size_t>(255);
   }
-  p.ws = ((p.ws + 255) & ~static_cast<size_t>(255)) + parts_ws;
   return p;
 }
 
-template <typename T, int DC, bool COLS>
-int bwd_launch(const BKernel& A, int parts, cudaStream_t st) {
-  constexpr size_t smem = sizeof(float) * (2ull * (64 + kBwdWalk) * (DC * 64 + 4) + 2 * kBwdWalk);
-  auto kern = xattn_bwd_mma_kernel<T, DC, COLS>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+template <typename T, int DC>
+int bwd_launch(const BKernel& A, cudaStream_t st) {
+  auto kern = xattn_bwd_mma_kernel<T, DC>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, BShape<DC>::kSmem);
   if (e != cudaSuccess) return cuda_status(e, "cross_attention backward: set smem");
-  const int threads = COLS && DC == 4 ? 256 : 128;
-  if (A.tiles > 0)
-    kern<<<dim3(static_cast<unsigned>(A.tiles) * A.s.nb * A.s.hkv, parts), threads, smem, st>>>(A);
-  TSB_CHECK_LAUNCH("cross_attention backward launch");
-  return TRNSPARSE_OK;
-}
-
-template <typename T, bool COLS>
-int bwd_dispatch(const BKernel& A, int dc, int parts, cudaStream_t st) {
-  if (dc == 1) return bwd_launch<T, 1, COLS>(A, parts, st);
-  if (dc == 2) return bwd_launch<T, 2, COLS>(A, parts, st);
-  return bwd_launch<T, 4, COLS>(A, parts, st);
+  e = launch_pdl(kern, dim3(A.cols.ctas + A.rows.ctas), dim3(BShape<DC>::kThreads), BShape<DC>::kSmem, st, A);
+  return e == cudaSuccess ? TRNSPARSE_OK : cuda_status(e, "cross_attention backward launch");
 }
 
 template <typename T>
-int sum_parts(const float* part, int parts, int64_t rows, void* out, int H, int L, int D, const int64_t* os,
-              cudaStream_t st) {
-  const int64_t n = rows * D;
-  xattn_sum_parts_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(
-      part, parts, rows, static_cast<T*>(out), H, L, D, os[0], os[1], os[2]);
-  TSB_CHECK_LAUNCH("cross_attention backward: sum of parts");
-  return TRNSPARSE_OK;
-}
-
-template <typename T>
-int bwd_simt(const trnsparse_attention_args* a, void* ws, cudaStream_t st) {
+int bwd_general(const trnsparse_attention_args* a, void* ws, cudaStream_t st) {
   XSide s[2];
   int n = 0;
   int rc = make_sides(a, false, s, &n);
@@ -313,13 +391,7 @@ int bwd_simt(const trnsparse_attention_args* a, void* ws, cudaStream_t st) {
   const int Hq = (int)a->q_heads, Hkv = (int)a->kv_heads, Tq = (int)a->q_len, D = (int)a->head_dim;
   const int64_t rows = a->batch * a->q_heads * a->q_len, keys = a->batch * a->kv_heads * a->k_len;
   float* delta = static_cast<float*>(ws);
-  float* part = reinterpret_cast<float*>(static_cast<char*>(ws) +
-                                         ((sizeof(float) * static_cast<size_t>(rows) + 255) & ~static_cast<size_t>(255)));
   const int64_t *gs = a->dout_strides, *os = a->out_strides;
-  xattn_delta_kernel<T><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(
-      static_cast<const T*>(a->dout), static_cast<const T*>(a->out), rows, Hq, Tq, D, gs[0], gs[1], gs[2], os[0], os[1],
-      os[2], delta);
-  TSB_CHECK_LAUNCH("cross_attention backward: row sums");
   BKernel A = {};
   A.s = s[0];
   A.s.o_bi = a->dq_strides[0];
@@ -339,6 +411,8 @@ int bwd_simt(const trnsparse_attention_args* a, void* ws, cudaStream_t st) {
     A.dv_s[i] = a->dv_strides[i];
   }
   A.D = D;
+  A.all_rows = rows;
+  A.all_keys = keys;
   const uintptr_t m = a->dtype == TRNSPARSE_F32 ? 15 : 7;
   const uintptr_t bases = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) |
                           reinterpret_cast<uintptr_t>(a->v) | reinterpret_cast<uintptr_t>(a->dout);
@@ -347,28 +421,41 @@ int bwd_simt(const trnsparse_attention_args* a, void* ws, cudaStream_t st) {
   A.vec = !(bases & m) && !(strides & 3);
   A.scale = static_cast<float>(a->scale);
   A.scale_log2 = static_cast<float>(a->scale * 1.4426950408889634);
-
-  A.tiles = p.tiles[0];
-  A.chunk = p.chunk[0];
-  A.rows_all = rows;
-  A.part0 = p.parts[0] > 1 ? part : nullptr;
-  if (a->dq) {
-    rc = bwd_dispatch<T, false>(A, p.dc, p.parts[0], st);
-    if (rc) return rc;
-    if (A.part0) rc = sum_parts<T>(part, p.parts[0], rows, a->dq, Hq, Tq, D, a->dq_strides, st);
+  BSum sum = {};
+  sum.D = D;
+  for (int i = 0; i < 2; ++i) {
+    if (i ? !a->dk || keys == 0 : !a->dq) continue;
+    BWalk& w = i ? A.cols : A.rows;
+    const int64_t ctas = static_cast<int64_t>(p.tiles[i]) * p.parts[i] * s[0].nb * s[0].hkv;
+    TSB_REQUIRE(ctas < (1ll << 30), "cross_attention backward: too many tiles (%lld)", static_cast<long long>(ctas));
+    w.tiles = p.tiles[i];
+    w.chunk = p.chunk[i];
+    w.parts = p.parts[i];
+    w.ctas = static_cast<unsigned>(ctas);
+    if (w.parts == 1) continue;
+    w.part0 = reinterpret_cast<float*>(static_cast<char*>(ws) + p.at[i]);
+    w.part1 = i ? w.part0 + w.parts * keys * D : nullptr;
+    for (int k = i; k < 1 + 2 * i; ++k) {  // dq; dk and dv
+      sum.part[k] = k == 2 ? w.part1 : w.part0;
+      sum.out[k] = k == 0 ? a->dq : k == 1 ? a->dk : a->dv;
+      sum.rows[k] = i ? keys : rows;
+      sum.parts[k] = w.parts;
+      sum.H[k] = i ? Hkv : Hq;
+      sum.L[k] = i ? static_cast<int>(a->k_len) : Tq;
+      for (int j = 0; j < 3; ++j) sum.o[k][j] = (k == 0 ? a->dq_strides : k == 1 ? a->dk_strides : a->dv_strides)[j];
+    }
   }
-  if (rc || !a->dk || a->k_len == 0) return rc;
-
-  A.tiles = p.tiles[1];
-  A.chunk = p.chunk[1];
-  A.rows_all = keys;
-  A.part0 = p.parts[1] > 1 ? part : nullptr;
-  A.part1 = p.parts[1] > 1 ? part + p.parts[1] * keys * D : nullptr;
-  rc = bwd_dispatch<T, true>(A, p.dc, p.parts[1], st);
-  if (rc || !A.part0) return rc;
-  rc = sum_parts<T>(A.part0, p.parts[1], keys, a->dk, Hkv, (int)a->k_len, D, a->dk_strides, st);
-  if (rc) return rc;
-  return sum_parts<T>(A.part1, p.parts[1], keys, a->dv, Hkv, (int)a->k_len, D, a->dv_strides, st);
+  if (A.rows.ctas + A.cols.ctas == 0) return TRNSPARSE_OK;
+  xattn_delta_kernel<T><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(
+      static_cast<const T*>(a->dout), static_cast<const T*>(a->out), rows, Hq, Tq, D, gs[0], gs[1], gs[2], os[0], os[1],
+      os[2], delta);
+  TSB_CHECK_LAUNCH("cross_attention backward: row sums");
+  rc = p.dc == 1 ? bwd_launch<T, 1>(A, st) : p.dc == 2 ? bwd_launch<T, 2>(A, st) : bwd_launch<T, 4>(A, st);
+  const int64_t elements = (sum.rows[0] + sum.rows[1] + sum.rows[2]) * D;
+  if (rc || elements == 0) return rc;
+  cudaError_t e = launch_pdl(xattn_sum_parts_kernel<T>, dim3(static_cast<unsigned>((elements + 255) / 256)), dim3(256), 0,
+                             st, sum);
+  return e == cudaSuccess ? TRNSPARSE_OK : cuda_status(e, "cross_attention backward: sum of parts");
 }
 
 }  // namespace
@@ -397,5 +484,5 @@ extern "C" int trnsparse_cross_attention_backward(const trnsparse_attention_args
               need);
   cudaStream_t st = as_stream(stream);
   if (xattn_bwd_tc_ok(a)) return xattn_bwd_tc(a, ws, st);
-  return a->dtype == TRNSPARSE_F32 ? bwd_simt<float>(a, ws, st) : bwd_simt<__nv_bfloat16>(a, ws, st);
+  return a->dtype == TRNSPARSE_F32 ? bwd_general<float>(a, ws, st) : bwd_general<__nv_bfloat16>(a, ws, st);
 }

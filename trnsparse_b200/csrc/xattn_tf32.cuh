@@ -18,7 +18,7 @@ namespace tsb {
 namespace {
 
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-  // rounded by integer arithmetic: a conversion instruction an element would cost more than the products
+  // nearest, halves away from zero, in two integer operations
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
   lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
@@ -29,10 +29,10 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-// c[n] += a b[n], b0 and b1 this lane's two elements of tile n
-template <int N>
-__device__ __forceinline__ void mma_3xtf32(float (&c)[N][4], const uint32_t (&ah)[4], const uint32_t (&al)[4],
-                                           const float (&b0)[N], const float (&b1)[N]) {
+// c[m][n0 + n] += a[m] b[n], b0 and b1 this lane's two elements of tile n
+template <int MT, int N, int NC>
+__device__ __forceinline__ void mma_3xtf32(float (&c)[MT][NC][4], int n0, const uint32_t (&ah)[MT][4],
+                                           const uint32_t (&al)[MT][4], const float (&b0)[N], const float (&b1)[N]) {
   uint32_t bh[N][2], bl[N][2];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
@@ -40,53 +40,62 @@ __device__ __forceinline__ void mma_3xtf32(float (&c)[N][4], const uint32_t (&ah
     split_tf32(b1[n], bh[n][1], bl[n][1]);
   }
 #pragma unroll
-  for (int n = 0; n < N; ++n) mma_tf32(c[n], al, bh[n]);
+  for (int i = 0; i < 3; ++i)
 #pragma unroll
-  for (int n = 0; n < N; ++n) mma_tf32(c[n], ah, bl[n]);
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-  for (int n = 0; n < N; ++n) mma_tf32(c[n], ah, bh[n]);
+      for (int n = 0; n < N; ++n) mma_tf32(c[m][n0 + n], i ? ah[m] : al[m], i == 1 ? bl[n] : bh[n]);
 }
 
-// c[n] += F X^T over the first D columns: F the warp's 16 rows, X the NT * 8 walked rows (both DP floats apart).
-template <int NT, int DP>
-__device__ __forceinline__ void scores_tf32(float (&c)[NT][4], const float* F, const float* X, int D, int g, int t) {
-#pragma unroll 2
+// c[m][n] += F X^T over the first D columns: F the warp's 16 MT rows, X the 8 NT walked rows (both DP floats apart).
+template <int MT, int NT, int DP>
+__device__ __forceinline__ void scores_tf32(float (&c)[MT][NT][4], const float* F, const float* X, int D, int g, int t) {
+#pragma unroll (MT == 1 ? 2 : 1)
   for (int k = 0; k < D; k += 8) {
-    uint32_t ah[4], al[4];
-    split_tf32(F[g * DP + k + t], ah[0], al[0]);
-    split_tf32(F[(g + 8) * DP + k + t], ah[1], al[1]);
-    split_tf32(F[g * DP + k + t + 4], ah[2], al[2]);
-    split_tf32(F[(g + 8) * DP + k + t + 4], ah[3], al[3]);
     float b0[NT], b1[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       b0[n] = X[(n * 8 + g) * DP + k + t];
       b1[n] = X[(n * 8 + g) * DP + k + t + 4];
     }
-    mma_3xtf32<NT>(c, ah, al, b0, b1);
+    uint32_t ah[MT][4], al[MT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const float* f = F + (m * 16 + g) * DP + k + t;
+      split_tf32(f[0], ah[m][0], al[m][0]);
+      split_tf32(f[8 * DP], ah[m][1], al[m][1]);
+      split_tf32(f[4], ah[m][2], al[m][2]);
+      split_tf32(f[8 * DP + 4], ah[m][3], al[m][3]);
+    }
+    mma_3xtf32<MT, NT, NT>(c, 0, ah, al, b0, b1);
   }
 }
 
-// acc[n] += P X: P the scores' tiles (16 x 8 NT), X the walked rows, NO tiles of 8 columns.
-template <int NT, int NO, int DP>
-__device__ __forceinline__ void weigh_tf32(float (&acc)[NO][4], const float (&p)[NT][4], const float* X, int g, int t) {
+// acc[m] += P X: P the scores' tiles (16 MT x 8 NT), X the walked rows, NO tiles of 8 columns.
+template <int MT, int NT, int NO, int DP>
+__device__ __forceinline__ void weigh_tf32(float (&acc)[MT][NO][4], const float (&p)[MT][NT][4], const float* X, int g,
+                                           int t) {
+  constexpr int STEP = MT == 1 ? 8 : 4;
 #pragma unroll
   for (int k = 0; k < NT; ++k) {
-    uint32_t ah[4], al[4];
-    split_tf32(p[k][0], ah[0], al[0]);
-    split_tf32(p[k][2], ah[1], al[1]);
-    split_tf32(p[k][1], ah[2], al[2]);
-    split_tf32(p[k][3], ah[3], al[3]);
+    uint32_t ah[MT][4], al[MT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      split_tf32(p[m][k][0], ah[m][0], al[m][0]);
+      split_tf32(p[m][k][2], ah[m][1], al[m][1]);
+      split_tf32(p[m][k][1], ah[m][2], al[m][2]);
+      split_tf32(p[m][k][3], ah[m][3], al[m][3]);
+    }
     const float* x = X + (k * 8 + 2 * t) * DP + g;
 #pragma unroll
-    for (int n0 = 0; n0 < NO; n0 += 8) {
-      float b0[8], b1[8];
+    for (int n0 = 0; n0 < NO; n0 += STEP) {
+      float b0[STEP], b1[STEP];
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
+      for (int n = 0; n < STEP; ++n) {
         b0[n] = x[(n0 + n) * 8];
         b1[n] = x[DP + (n0 + n) * 8];
       }
-      mma_3xtf32<8>(reinterpret_cast<float(&)[8][4]>(acc[n0]), ah, al, b0, b1);
+      mma_3xtf32<MT, STEP, NO>(acc, n0, ah, al, b0, b1);
     }
   }
 }
