@@ -29,45 +29,67 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-// c[m][n0 + n] += a[m] b[n], b0 and b1 this lane's two elements of tile n
-template <int MT, int N, int NC>
-__device__ __forceinline__ void mma_3xtf32(float (&c)[MT][NC][4], int n0, const uint32_t (&ah)[MT][4],
-                                           const uint32_t (&al)[MT][4], const float (&b0)[N], const float (&b1)[N]) {
-  uint32_t bh[N][2], bl[N][2];
+// c[m][n0 + n] += a[m][k] b[k][n] over K products of 8. The matrix unit cuts its sums instead of rounding them, which
+// over a chain of a few hundred keys shrank the results by 4e-6: every K products start from zero, the small terms
+// first, and are added to the sum by a rounded addition.
+template <int MT, int K, int N, int NC, typename B>
+__device__ __forceinline__ void mma_3xtf32(float (&c)[MT][NC][4], int n0, const uint32_t (&ah)[K][MT][4],
+                                           const uint32_t (&al)[K][MT][4], B b) {
+  float s[MT][N][4];
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    split_tf32(b0[n], bh[n][0], bl[n][0]);
-    split_tf32(b1[n], bh[n][1], bl[n][1]);
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < N; ++n) s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    uint32_t bh[N][2], bl[N][2];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const float2 v = b(k, n0 + n);
+      split_tf32(v.x, bh[n][0], bl[n][0]);
+      split_tf32(v.y, bh[n][1], bl[n][1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < N; ++n) mma_tf32(s[m][n], i ? ah[k][m] : al[k][m], i == 1 ? bl[n] : bh[n]);
   }
 #pragma unroll
-  for (int i = 0; i < 3; ++i)
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int n = 0; n < N; ++n) mma_tf32(c[m][n0 + n], i ? ah[m] : al[m], i == 1 ? bl[n] : bh[n]);
+      for (int j = 0; j < 4; ++j) c[m][n0 + n][j] += s[m][n][j];
 }
 
-// c[m][n] += F X^T over the first D columns: F the warp's 16 MT rows, X the 8 NT walked rows (both DP floats apart).
+// c[m][n] += F X^T over the first D columns: F the warp's 16 MT rows, X the 8 NT walked rows (both DP floats apart, zero
+// from column D to the next multiple of 16).
 template <int MT, int NT, int DP>
 __device__ __forceinline__ void scores_tf32(float (&c)[MT][NT][4], const float* F, const float* X, int D, int g, int t) {
-#pragma unroll (MT == 1 ? 2 : 1)
-  for (int k = 0; k < D; k += 8) {
-    float b0[NT], b1[NT];
+  constexpr int STEP = NT < 4 ? NT : 4;
+  const float* f0 = F + g * DP + t;
+  const float* x0 = X + g * DP + t;
+#pragma unroll 1
+  for (int k0 = 0; k0 < D; k0 += 16, f0 += 16, x0 += 16) {
+    uint32_t ah[2][MT][4], al[2][MT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      b0[n] = X[(n * 8 + g) * DP + k + t];
-      b1[n] = X[(n * 8 + g) * DP + k + t + 4];
-    }
-    uint32_t ah[MT][4], al[MT][4];
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const float* f = F + (m * 16 + g) * DP + k + t;
-      split_tf32(f[0], ah[m][0], al[m][0]);
-      split_tf32(f[8 * DP], ah[m][1], al[m][1]);
-      split_tf32(f[4], ah[m][2], al[m][2]);
-      split_tf32(f[8 * DP + 4], ah[m][3], al[m][3]);
-    }
-    mma_3xtf32<MT, NT, NT>(c, 0, ah, al, b0, b1);
+      for (int m = 0; m < MT; ++m) {
+        const float* f = f0 + m * 16 * DP + k * 8;
+        split_tf32(f[0], ah[k][m][0], al[k][m][0]);
+        split_tf32(f[8 * DP], ah[k][m][1], al[k][m][1]);
+        split_tf32(f[4], ah[k][m][2], al[k][m][2]);
+        split_tf32(f[8 * DP + 4], ah[k][m][3], al[k][m][3]);
+      }
+#pragma unroll
+    for (int n0 = 0; n0 < NT; n0 += STEP)
+      mma_3xtf32<MT, 2, STEP, NT>(c, n0, ah, al, [&](int k, int n) {
+        const float* x = x0 + n * 8 * DP + k * 8;
+        return make_float2(x[0], x[4]);
+      });
   }
 }
 
@@ -75,28 +97,26 @@ __device__ __forceinline__ void scores_tf32(float (&c)[MT][NT][4], const float* 
 template <int MT, int NT, int NO, int DP>
 __device__ __forceinline__ void weigh_tf32(float (&acc)[MT][NO][4], const float (&p)[MT][NT][4], const float* X, int g,
                                            int t) {
-  constexpr int STEP = MT == 1 ? 8 : 4;
+  constexpr int STEP = 4;
+  const float* x0 = X + 2 * t * DP + g;
 #pragma unroll
-  for (int k = 0; k < NT; ++k) {
-    uint32_t ah[MT][4], al[MT][4];
+  for (int k0 = 0; k0 < NT; k0 += 2) {
+    uint32_t ah[2][MT][4], al[2][MT][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      split_tf32(p[m][k][0], ah[m][0], al[m][0]);
-      split_tf32(p[m][k][2], ah[m][1], al[m][1]);
-      split_tf32(p[m][k][1], ah[m][2], al[m][2]);
-      split_tf32(p[m][k][3], ah[m][3], al[m][3]);
-    }
-    const float* x = X + (k * 8 + 2 * t) * DP + g;
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-    for (int n0 = 0; n0 < NO; n0 += STEP) {
-      float b0[STEP], b1[STEP];
-#pragma unroll
-      for (int n = 0; n < STEP; ++n) {
-        b0[n] = x[(n0 + n) * 8];
-        b1[n] = x[DP + (n0 + n) * 8];
+      for (int m = 0; m < MT; ++m) {
+        split_tf32(p[m][k0 + k][0], ah[k][m][0], al[k][m][0]);
+        split_tf32(p[m][k0 + k][2], ah[k][m][1], al[k][m][1]);
+        split_tf32(p[m][k0 + k][1], ah[k][m][2], al[k][m][2]);
+        split_tf32(p[m][k0 + k][3], ah[k][m][3], al[k][m][3]);
       }
-      mma_3xtf32<MT, STEP, NO>(acc, n0, ah, al, b0, b1);
-    }
+#pragma unroll
+    for (int n0 = 0; n0 < NO; n0 += STEP)
+      mma_3xtf32<MT, 2, STEP, NO>(acc, n0, ah, al, [&](int k, int n) {
+        const float* x = x0 + (k0 + k) * 8 * DP + n * 8;
+        return make_float2(x[0], x[DP]);
+      });
   }
 }
 
