@@ -14,9 +14,9 @@
 // 16 rows a CTA on the CUDA cores, a thread forming a 2 x 4 tile of scores and a
 // 2 x 4 DC tile of the output from float4 reads of shared memory. More rows are
 // bound by arithmetic: 128 rows a CTA on the tensor cores (3xTF32, xattn_tf32.cuh),
-// 48 TFLOP/s at 2 x 16/16 heads, 1024 x 1024 x 64 (179 us; 308 on the CUDA cores)
-// and 52 with 16/4 heads at head_dim 128 (334 us; 615). The tensor pipe is then half
-// busy: two warps a scheduler, a third of whose instructions are the products.
+// 48 TFLOP/s at 2 x 16/16 heads, 1024 x 1024 x 64 (180 us; 308 on the CUDA cores)
+// and 50 with 16/4 heads at head_dim 128 (345 us; 615). The tensor pipe is then half
+// busy: two warps a scheduler, a quarter of whose instructions are the products.
 // In both the next tile is copied asynchronously. When there are fewer CTAs than
 // fill the GPU the keys are cut into ranges, each writing (O, log-sum-exp) of its
 // part, joined afterwards.
@@ -466,29 +466,27 @@ __global__ void __launch_bounds__(256) combine_pieces_kernel(const float* __rest
 // ---------------------------------------------------------------- host side
 
 struct GeneralPlan {
-  int bm, dc, splits[2], chunk[2], row_tiles[2], pieces;
+  int dc, bm[2], splits[2], chunk[2], row_tiles[2], pieces;
 };
 
 GeneralPlan general_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n) {
   GeneralPlan p = {};
   p.dc = a->head_dim <= 64 ? 1 : a->head_dim <= 128 ? 2 : 4;
-  int64_t most = 0;
-  for (int i = 0; i < n; ++i) most = most > side_rows(s[i]) ? most : side_rows(s[i]);
-  // 16-row CTAs where a 128-row tile would be mostly padding
-  p.bm = most <= 32 ? 16 : 128;
   const int resident = p.dc <= 2 ? 2 : 1;  // CTAs an SM: by registers and shared memory
-  const int64_t keys = p.bm == 16 ? kXKeys : kMmaKeys;
   for (int i = 0; i < n; ++i) {
-    p.row_tiles[i] = static_cast<int>((side_rows(s[i]) + p.bm - 1) / p.bm);
+    p.bm[i] = side_rows(s[i]) <= 32 ? 16 : 128;  // 16-row CTAs where a 128-row tile would be mostly padding
+    const int64_t keys = p.bm[i] == 16 ? kXKeys : kMmaKeys;
+    p.row_tiles[i] = static_cast<int>((side_rows(s[i]) + p.bm[i] - 1) / p.bm[i]);
     const int64_t ctas = static_cast<int64_t>(p.row_tiles[i]) * s[i].nb * s[i].hkv;
     const int64_t tiles = (s[i].klen + keys - 1) / keys;
     int64_t per;
-    if (p.bm == 16) {  // bound by the reads of K and V: three CTAs an SM (walk_steps' fewer: 46 us against 31 at 4096 keys)
+    // bound by the reads of K and V: three CTAs an SM (walk_steps' fewer: 46 us against 31 at 4096 keys)
+    if (p.bm[i] == 16) {
       int64_t splits = ctas > 0 ? (3ll * sm_count() + ctas - 1) / ctas : 1;
       splits = splits < 128 ? splits : 128;
       per = tiles > splits ? (tiles + splits - 1) / splits : 1;
     } else {
-      per = walk_steps(ctas, tiles, sm_count(), resident, 128);
+      per = walk_steps(ctas, tiles, sm_count(), resident, 128, 0.1);
     }
     p.chunk[i] = static_cast<int>(per * keys);
     p.splits[i] = static_cast<int>(tiles > 0 ? (tiles + per - 1) / per : 1);
@@ -566,8 +564,8 @@ int general_forward(const trnsparse_attention_args* a, bool prefix, void* ws, cu
     A.vec = four_aligned(a);
     A.scale = static_cast<float>(a->scale);
     A.scale_log2 = static_cast<float>(a->scale * 1.4426950408889634);
-    rc = a->dtype == TRNSPARSE_F32 ? general_dispatch<float>(A, p.bm, p.dc, p.splits[i], i > 0, st)
-                                   : general_dispatch<__nv_bfloat16>(A, p.bm, p.dc, p.splits[i], i > 0, st);
+    rc = a->dtype == TRNSPARSE_F32 ? general_dispatch<float>(A, p.bm[i], p.dc, p.splits[i], i > 0, st)
+                                   : general_dispatch<__nv_bfloat16>(A, p.bm[i], p.dc, p.splits[i], i > 0, st);
     if (rc) return rc;
     piece += p.splits[i];
   }

@@ -15,11 +15,11 @@
 // repeatable results and no traffic for dQ. Where tiles are fewer than SMs the
 // walks are cut into parts whose fp32 sums a last kernel adds in order.
 //
-// What bounds it: the tensor cores' tf32 rate (3xTF32 in xattn_tf32.cuh), kept 64%
-// busy with two warps a scheduler; the rest goes to the splits and to waits inside a
-// warp's chain of scores, P and sums. 2 x 16/16 heads, 1024 x 1024 x 64: 656 us,
-// 46 TFLOP/s of the seven products (CUDA cores before: 1171 us; row by row tiles of
-// 16 rows a warp, each walk its own launch: 698); 16/4 heads at head_dim 128: 1237 us.
+// What bounds it: the tensor cores' tf32 rate (3xTF32, xattn_tf32.cuh), kept 64% busy
+// with two warps a scheduler; the rest goes to splitting operands and to waits inside
+// a warp's chain of scores, P and sums. 2 x 16/16 heads, 1024 x 1024 x 64: 584 us, 51
+// TFLOP/s of the seven products (on the CUDA cores 1171 us; 16 rows a warp and a
+// launch for each walk 698); 16/4 heads at head_dim 128 1316 us (2440).
 #include "xattn_tf32.cuh"
 
 namespace tsb {
@@ -360,8 +360,9 @@ BPlan bwd_plan(const trnsparse_attention_args* a, const XSide& s) {
   for (int i = 0; i < 2; ++i) {
     p.tiles[i] = static_cast<int>((fixed[i] + bt - 1) / bt);
     const int64_t ctas = static_cast<int64_t>(p.tiles[i]) * s.nb * s.hkv, steps = (walk[i] + kBwdWalk - 1) / kBwdWalk;
-    // both walks run side by side: three and four of the seven products
-    const int64_t per = walk_steps(ctas, steps, sm_count() * (3 + i) / 7, resident, 32);
+    // both walks run side by side: three and four of the seven products. Half a step a part: 108 us against 133 with
+    // a tenth at 2 x 8/2 heads, 333 x 517 x 64
+    const int64_t per = walk_steps(ctas, steps, sm_count() * (3 + i) / 7, resident, 32, 0.5);
     p.chunk[i] = static_cast<int>(per * kBwdWalk);
     p.parts[i] = static_cast<int>(steps > 0 ? (steps + per - 1) / per : 1);
     p.at[i] = p.ws;

@@ -73,10 +73,12 @@ int check_attention(const trnsparse_attention_args* a, const char* what);
 int combine_pieces(const float* part_o, const float* part_lse, int pieces, const trnsparse_attention_args* a,
                    cudaStream_t st);
 
-// Steps of a walk that one of `ctas` CTAs takes when the walks are cut to fill `sms` SMs, `resident` CTAs each. The time
-// is counted in steps of a CTA that has an SM for itself: a step beside r - 1 others takes (1 + r) / 2, a CTA starts and
-// ends in two steps, and each part that is joined afterwards costs half a step.
-inline int64_t walk_steps(int64_t ctas, int64_t steps, int64_t sms, int resident, int64_t most) {
+// Steps of a walk that one of `ctas` CTAs takes when the walks are cut into at most `most` parts to fill `sms` SMs,
+// `resident` CTAs each. The time is counted in steps of a CTA that has an SM for itself: a step beside r - 1 others
+// takes (1 + r) / 2, a CTA starts and ends in two, the join takes two, and each part `part_cost` and the traffic of its
+// CTAs' 128 rows.
+inline int64_t walk_steps(int64_t ctas, int64_t steps, int64_t sms, int resident, int64_t most,
+                          double part_cost) {
   const int64_t slots = sms * resident;
   int64_t best = steps > 0 ? steps : 1;
   double least = 1e300;
@@ -84,7 +86,8 @@ inline int64_t walk_steps(int64_t ctas, int64_t steps, int64_t sms, int resident
     const int64_t per = (steps + n - 1) / n, parts = (steps + per - 1) / per, all = ctas * parts;
     const int64_t waves = all / slots, rest = (all - waves * slots + sms - 1) / sms;
     const double time = 0.5 * static_cast<double>(waves * (1 + resident) + (rest ? 1 + rest : 0));
-    const double cost = time * static_cast<double>(per + 2) + (parts > 1 ? 2.0 + 0.5 * static_cast<double>(parts) : 0.0);
+    const double join = 2.0 + static_cast<double>(parts) * (part_cost + static_cast<double>(ctas) / 128.0);
+    const double cost = time * static_cast<double>(per + 2) + (parts > 1 ? join : 0.0);
     if (cost < least) {
       least = cost;
       best = per;
