@@ -521,3 +521,19 @@ def test_training_run_together_and_captured():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     again = torch.autograd.grad(eager, leaves, d)  # the eager graph still works
     assert all(torch.equal(a, b) for a, b in zip(again, want))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_lengths_of_64_bits_are_clamped_before_they_are_narrowed(dtype):
+    """2^40 and 2^32 have zero low words, -2^40 + 5 a positive one."""
+    g = _gen(91)
+    B, Hq, Hkv, T, S, D = 4, 4, 2, 3, 70, 64
+    wide = torch.tensor([2**40, 2**32, -(2**40) + 5, 33], device="cuda")
+    narrow = torch.tensor([S, S, 0, 33], dtype=torch.int32, device="cuda")
+    q = _randn(g, B, Hq, T, D, dtype=dtype)
+    k, v = (_randn(g, B, Hkv, S, D, dtype=dtype) for _ in range(2))
+    pk, pv = (_randn(g, Hkv, 9, D, dtype=dtype) for _ in range(2))
+    assert torch.equal(ts.cross_attention(q, k, v, wide), ts.cross_attention(q, k, v, narrow))
+    got = ts.shared_prefix_attention(q, pk, pv, k, v, wide)
+    assert torch.equal(got, ts.shared_prefix_attention(q, pk, pv, k, v, narrow))
+    assert ts.cross_attention(q, k, v, wide)[2].eq(0).all() and ts.cross_attention(q, k, v, wide)[0].ne(0).any()

@@ -296,6 +296,13 @@ def _check_lengths(name, lengths, B):
     assert tuple(lengths.shape) == (B,), f"{name}: lengths must be ({B},), got {tuple(lengths.shape)}"
 
 
+def _lengths32(lengths, dev, most):
+    """``lengths`` as the kernels read them; 64-bit values are clamped before they are narrowed (two small launches)."""
+    if lengths.dtype == torch.int64:
+        lengths = lengths.clamp(0, most).to(torch.int32)
+    return _to(lengths, dev).contiguous()
+
+
 def cross_attention(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -331,7 +338,7 @@ def cross_attention(
     scale = float(q.shape[3] ** -0.5 if scale is None else scale)
     dev = _dev_of(q, k, v)
     qd, kd, vd = (_tiles(_to(t, dev)) for t in (q, k, v))
-    lengths = None if key_lengths is None else _to(key_lengths, dev, torch.int32).contiguous()
+    lengths = None if key_lengths is None else _lengths32(key_lengths, dev, Sk)
     mask = None if key_mask is None else _rows(_to(key_mask, dev))
     if _grad_wanted(qd, kd, vd):
         out = _CrossAttentionFn.apply(qd, kd, vd, lengths, mask, scale)
@@ -376,7 +383,7 @@ def shared_prefix_attention(
     scale = float(D ** -0.5 if scale is None else scale)
     dev = _dev_of(q, prefix_k, k_cache)
     qd, pk, pv, kc, vc = (_tiles(_to(t, dev)) for t in (q, prefix_k, prefix_v, k_cache, v_cache))
-    lens = _to(lengths, dev, torch.int32).contiguous()
+    lens = _lengths32(lengths, dev, kc.shape[2])
     out = _like(qd)
     if out.numel():
         a = _attention_args(qd, kc, vc, out, None, lens, None, scale)
