@@ -19,9 +19,13 @@
 // acc1 += P_j X2_j, S_{j+1}, acc0 += dS_j X1_j, dP_{j+1}; rows, with two S
 // buffers: dP_{j+1}, acc0 += dS_j X1_j, S_{j+2}.
 //
-// What bounds it: the walked tiles, 64 KB a step at head_dim 128 from L2 at
-// 40-50 GB/s per SM (about 1.4 us), against 3 (rows) or 4 (columns) products of
-// 0.26 us.
+// What bounds it: the chain of a step. At head_dim 128 a step of rows takes 2260
+// clocks for 3 products of 512, one of columns 3320 for 4: the tensor pipe is busy 70
+// and 63% of the time, and the rest is the pointwise part between the two products of
+// a step (scores out of TMEM, 2^x, P and dS back), as deep as TMEM allows: rows have a
+// second S, columns none, their 512 columns being S, dP, dK and dV. Loads are not
+// waited for (walked tiles: 64 KB a step). 4 x 16 heads, 2048 x 4096 x 128: dQ 324 us
+// and dK, dV 461 us, 1272 and 1192 TFLOP/s of their three and four products.
 //
 // Hidden keys: P and dS are set to zero by selection; in rows the K rows of
 // hidden keys are zeroed in shared memory before dS K, so NaN in padding meets

@@ -4,11 +4,10 @@
 //
 //   O = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m),  s = scale log2(e) q.k
 // in one pass over the key tiles with the running maximum m and sum l of every
-// row. P = 2^(s - m) is rounded to bf16 for its product with V (half a step,
-// 2^-9 relative on average, of the same size as the result's own rounding); l
-// sums the unrounded values in fp32. m moves only when a tile's maximum passes
-// it by more than 2^8, so the accumulator in TMEM is rarely rescaled and P <=
-// 2^8.
+// row. P = 2^(s - m) is rounded to bf16 for its product with V (half a step, at
+// most 2^-8 relative, of the same size as the result's own rounding); l sums the
+// unrounded values in fp32. m moves only when a tile's maximum passes it by more
+// than 2^8, so the accumulator in TMEM is rarely rescaled and P <= 2^8.
 //
 // An item is 256 packed rows (see xattn.cuh: query heads of one key head,
 // tokens, and for a shared prefix all sequences) against the keys of one (batch
@@ -36,6 +35,13 @@
 // tile order (no atomics, results repeat bit for bit). The split depends on the
 // lengths, which stay on the device: no host synchronisation.
 //
+// What bounds it: long rows, the exponentials and the chain scores -> P -> product of
+// a half (a quarter of them as a polynomial on the FMA pipe): 16 heads, 4096 x 4096 x
+// 128 137 us, 1000 TFLOP/s; 4 x 16 heads, 2048 x 4096 x 128 with the row statistics 255
+// us, 1078. Short or ragged items lose 3 to 5 us an item and CTA to its start and end
+// and the join: prompts of 4 x 32/8 heads, 777 x up to 2049 keys 87 + 22 us. Few rows
+// (a shared prefix, 256 rows a key head): memory and that same start and end.
+//
 // Hidden keys (past a length, or masked): scores become -inf by selection, and
 // their V rows are zeroed in shared memory before the product, so NaN or
 // infinity in padding never meets a zero P. Only tiles that hold hidden keys
@@ -49,9 +55,10 @@ constexpr int kFwThreads = 352;
 constexpr int kFwRows = 256;  // rows of an item, two halves of 128
 constexpr int kFwKeys = 128, kFwKeyShift = 7;
 constexpr float kFwLazy = 8.f;
-// 1, 2, 3 measured: 45.4, 43.5, 42.9 us in a decode over 8 ragged sequences, 170, 167, 175 us in prompts of 777 tokens
+// Key tiles that an item's start and end count for: 1, 2, 4 take 109.2, 109.3, 108.8 us in ragged prompts of 777 tokens
+// and 146.6, 147.3, 147.7 us in a step of 96 sequences over a shared prefix of 32768 keys.
 constexpr int kFwItemCost = 2;
-constexpr int kFwLeast = 8;
+constexpr int kFwLeast = 8;  // see fw_plan; 4, 8, 16: 60.1, 62.1, 74.7 us (64 sequences, prefix 8192, own keys to 1024)
 
 template <int HD>
 struct FwLayout {

@@ -20,6 +20,8 @@
 // dw: each thread adds its rows' terms in fp32 registers, a CTA joins its
 // groups in shared memory into one partial row, and a second launch adds the
 // partial rows in a fixed order (no atomics: results repeat bit for bit).
+// 16384 tokens of 2 x 16 bf16 heads of 128: forward and backward 161 us for 671 MB,
+// 4.2 TB/s, 65% of a copy's rate.
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -338,8 +340,8 @@ QkPlan qk_plan(const trnsparse_qk_norm_rope_args* a, bool bwd) {
     }
     return true;
   };
-  // four elements a piece for both types: bf16 pieces of eight need twice the registers (148 in the backward pass,
-  // one CTA an SM: 246 us against 128 at 16384 tokens of 2 x 16 heads of 128)
+  // four elements a piece for both types: bf16 pieces of eight need twice the registers (148 in the backward pass, one
+  // CTA an SM, which took 1.9 times as long at 16384 tokens of 2 x 16 heads of 128)
   p.vec = fits(4) ? 4 : 1;
   const int units = static_cast<int>((a->head_dim + 2 * p.vec - 1) / (2 * p.vec));
   p.lpr = 1;
