@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(DC == 4 ? 256 : 128, DC <= 2 ? 2 : 1) xattn_mm
   float* Ks = Qs + BM * DP;
   float* Vs = Ks + KT * DP;
   const XSide& s = A.s;
-  const int tid = threadIdx.x, wr = (tid >> 5) * 16 * MT, g = (tid & 31) >> 2, t = tid & 3;
+  const int tid = threadIdx.x, lane = tid & 31, wr = (tid >> 5) * 16 * MT, g = lane >> 2, t = lane & 3;
   const int item = blockIdx.x / A.row_tiles, rt = blockIdx.x - item * A.row_tiles;
   const int bi = item / s.hkv, h = item - bi * s.hkv;
   const int64_t R = side_rows(s), r0 = static_cast<int64_t>(rt) * BM;
@@ -326,6 +326,10 @@ __global__ void __launch_bounds__(DC == 4 ? 256 : 128, DC <= 2 ? 2 : 1) xattn_mm
         for (int n = 0; n < NK; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) sc[a][n][j] = 0.f;
+      static_assert(KT == 32, "a lane a key");
+      const bool check = mask || k0 + KT > least;
+      bool seen = true;  // key k0 + lane
+      if (check) seen = k0 + lane < kend && (!mask || mask[k0 + lane]);
       scores_tf32<MT, NK, DP>(sc, Qs + wr * DP, Ks, D, g, t);
 #pragma unroll
       for (int a = 0; a < MT; ++a)
@@ -333,13 +337,14 @@ __global__ void __launch_bounds__(DC == 4 ? 256 : 128, DC <= 2 ? 2 : 1) xattn_mm
         for (int n = 0; n < NK; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) sc[a][n][j] *= A.scale_log2;
-      if (mask || k0 + KT > least) {
+      if (__any_sync(0xffffffffu, check)) {
+        const unsigned keep = __ballot_sync(0xffffffffu, seen);
 #pragma unroll
         for (int n = 0; n < NK; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const int key = k0 + n * 8 + 2 * t + j;
-            const bool hid = key >= kend || (mask && !mask[key]);
+            const int x = n * 8 + 2 * t + j, key = k0 + x;
+            const bool hid = !(keep >> x & 1u);
 #pragma unroll
             for (int a = 0; a < MT; ++a)
 #pragma unroll

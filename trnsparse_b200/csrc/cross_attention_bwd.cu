@@ -15,11 +15,12 @@
 // repeatable results and no traffic for dQ. Where tiles are fewer than SMs the
 // walks are cut into parts whose fp32 sums a last kernel adds in order.
 //
-// What bounds it: the tensor cores' tf32 rate (3xTF32, xattn_tf32.cuh), kept 64% busy
-// with two warps a scheduler; the rest goes to splitting operands and to waits inside
-// a warp's chain of scores, P and sums. 2 x 16/16 heads, 1024 x 1024 x 64: 584 us, 51
-// TFLOP/s of the seven products (on the CUDA cores 1171 us; 16 rows a warp and a
-// launch for each walk 698); 16/4 heads at head_dim 128 1316 us (2440).
+// What bounds it: the tensor cores' tf32 rate (3xTF32, xattn_tf32.cuh), kept about 60%
+// busy with two warps a scheduler; the rest goes to splitting operands and to waits
+// inside a warp's chain of scores, P and sums. 2 x 16/16 heads, 1024 x 1024 x 64: 634 us,
+// 47 TFLOP/s of the seven products (on the CUDA cores 1171 us); 16/4 heads at head_dim
+// 128 1278 us (2440); 2 x 8/2 heads, 333 x 517 x 64, where a CTA an SM is all there is,
+// 96 us (108 with four warps a CTA, two CTAs an SM; that took 584 at the first size).
 #include "xattn_tf32.cuh"
 
 namespace tsb {
@@ -47,8 +48,6 @@ __device__ __forceinline__ float4 bload4(const T* row, int d, int D, bool vec) {
   if (d + 3 < D) r.w = bcvt(row[d + 3]);
   return r;
 }
-constexpr int kBwdWalk = 32;  // walked rows a step
-
 // One of the two walks: a CTA each for `tiles` tiles of every item and `parts` ranges of the walked rows.
 struct BWalk {
   int tiles, chunk, parts;
@@ -87,22 +86,24 @@ __global__ void __launch_bounds__(256) xattn_delta_kernel(const T* __restrict__ 
   if (lane == 0) delta[row] = s;
 }
 
-// Up to head_dim 64 four warps of 32 fixed rows, so that each split of a walked element feeds two products; up to 128
-// eight of 16, as 32 rows' sums would not fit in registers; both with the next walked rows copied behind the arithmetic.
-// Above that, 64 rows (shared memory) and eight warps that share them in pairs: for dQ each takes half the walked keys,
-// the sums are joined at the end; for dK and dV one has each.
+// Eight warps, since one warp a scheduler keeps the tensor pipe 40% busy and two 64%. Up to head_dim 64 a warp has 32
+// fixed rows, so that each split of a walked element feeds two products, and half of the walked ones (the halves' sums
+// are joined at the end); up to 128 16 rows, as 32 rows' sums would not fit in registers; both with the next walked rows
+// copied behind the arithmetic. Above that, 64 rows (shared memory), which warps share in pairs: for dQ each has half
+// the walked keys, for dK and dV one each.
 template <int DC>
 struct BShape {
-  static constexpr int kThreads = DC == 1 ? 128 : 256, kTiles16 = DC == 1 ? 2 : 1, kRows = DC == 4 ? 64 : 128;
-  static constexpr int kStages = DC == 4 ? 1 : 2, kResident = DC == 1 ? 2 : 1, kStride = DC * 64 + 4;
-  static constexpr int kSmem = 4 * (2 * kRows * kStride + kStages * 2 * (kBwdWalk * kStride + kBwdWalk));
+  static constexpr int kThreads = 256, kTiles16 = DC == 1 ? 2 : 1, kRows = DC == 4 ? 64 : 128;
+  static constexpr int kWalk = DC == 1 ? 64 : 32;  // walked rows a step
+  static constexpr int kStages = DC == 4 ? 1 : 2, kStride = DC * 64 + 4;
+  static constexpr int kSmem = 4 * (2 * kRows * kStride + kStages * 2 * (kWalk * kStride + kWalk));
 };
 
 template <typename T, int DC, bool COLS>
 __device__ __forceinline__ void bwd_walk(const BKernel& A, const BWalk& W, unsigned cta, float* smb) {
   using S = BShape<DC>;
-  constexpr int MT = S::kTiles16, BT = S::kRows, WT = kBwdWalk, NT = S::kThreads, STAGES = S::kStages;
-  constexpr bool HALF = !COLS && DC == 4;  // a warp takes half the walked rows
+  constexpr int MT = S::kTiles16, BT = S::kRows, WT = S::kWalk, NT = S::kThreads, STAGES = S::kStages;
+  constexpr bool HALF = DC == 1 || (!COLS && DC == 4);  // a warp takes half the walked rows
   constexpr int DP = S::kStride, WW = HALF ? WT / 2 : WT, NW = WW / 8, NO = DC * 8, CH = DC * 16;
   constexpr int XS = 2 * (WT * DP + WT);  // floats of a stage
   constexpr bool BOTH = COLS && DC != 4;
@@ -110,10 +111,10 @@ __device__ __forceinline__ void bwd_walk(const BKernel& A, const BWalk& W, unsig
   float* F2 = F1 + BT * DP;  // fixed: dO or V
   float* X = F2 + BT * DP;   // walked, a stage: K or Q, V or dO, then (columns) the queries' lse and delta
   const XSide& s = A.s;
-  const int tid = threadIdx.x, g = (tid & 31) >> 2, t = tid & 3;
+  const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int f0 = (tid >> 5) % (BT / 16 / MT) * 16 * MT;  // this warp's fixed rows
-  const bool upper = DC == 4 && tid >= 128;
-  const bool second = COLS && upper;  // holds dV
+  const bool upper = tid >= 128;
+  const bool second = COLS && DC == 4 && upper;  // holds dV
   const int x0 = HALF && upper ? WW : 0;
   const unsigned line = cta / W.parts, part = cta - line * W.parts;
   const int item = line / W.tiles, tile = line - item * W.tiles;
@@ -158,7 +159,7 @@ __device__ __forceinline__ void bwd_walk(const BKernel& A, const BWalk& W, unsig
   else load_q(F1, F2, fix0, BT);
   grid_dep_wait();  // the row sums
   float row_lse[MT][2], row_delta[MT][2];  // rows: of this lane's queries
-  bool hide_row[MT][2], hide_any = false;  // columns: this lane's keys
+  bool hide_row[MT][2];  // columns: this lane's keys
 #pragma unroll
   for (int a = 0; a < MT; ++a)
 #pragma unroll
@@ -169,7 +170,6 @@ __device__ __forceinline__ void bwd_walk(const BKernel& A, const BWalk& W, unsig
       hide_row[a][i] = false;
       if (COLS) {
         hide_row[a][i] = r >= len || (mask && !mask[r]);
-        hide_any = hide_any || hide_row[a][i];
       } else if (r < R) {
         row_lse[a][i] = A.lse[stat0 + r];
         row_delta[a][i] = A.delta[stat0 + r];
@@ -187,7 +187,7 @@ __device__ __forceinline__ void bwd_walk(const BKernel& A, const BWalk& W, unsig
       }
   auto step = [&](const float* x, int64_t w) {
     const float *X1 = x + x0 * DP, *X2 = X1 + WT * DP;
-    const float *st_lse = x + 2 * WT * DP, *st_delta = st_lse + WT;
+    const float *st_lse = x + 2 * WT * DP + x0, *st_delta = st_lse + WT;
     w += x0;
     float sc[MT][NW][4], dp[MT][NW][4];  // scores, then P; dP, then dS: fixed rows by walked rows
 #pragma unroll
@@ -196,16 +196,17 @@ __device__ __forceinline__ void bwd_walk(const BKernel& A, const BWalk& W, unsig
       for (int n = 0; n < NW; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) sc[a][n][j] = dp[a][n][j] = 0.f;
+    bool seen = true;  // rows: key w + lane
+    if (!COLS && (mask || w + WW > len)) seen = lane < WW && w + lane < len && (!mask || mask[w + lane]);
     scores_tf32<MT, NW, DP>(sc, F1 + f0 * DP, X1, D, g, t);
     if (!second) scores_tf32<MT, NW, DP>(dp, F2 + f0 * DP, X2, D, g, t);
-    const bool some = COLS ? hide_any : mask || w + WW > len;
+    const unsigned keep = COLS ? 0u : __ballot_sync(0xffffffffu, seen);
 #pragma unroll
     for (int n = 0; n < NW; ++n)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = j >> 1, x = n * 8 + 2 * t + (j & 1);
-        bool hide = false;
-        if (!COLS && some) hide = w + x >= len || (mask && !mask[w + x]);
+        bool hide = !COLS && !(keep >> x & 1u);
 #pragma unroll
         for (int a = 0; a < MT; ++a) {
           if (COLS) hide = hide_row[a][i];
@@ -260,20 +261,29 @@ __device__ __forceinline__ void bwd_walk(const BKernel& A, const BWalk& W, unsig
     if (busy) step(X1, w);
     if (more) put_stats(X + stage * XS);
   }
-  if constexpr (HALF) {  // both halves' sums, through the fixed tile
+  if constexpr (HALF) {  // both halves' sums, through the fixed tiles
     __syncthreads();
-    if (upper) {
 #pragma unroll
-      for (int n = 0; n < NO; ++n)
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) F1[(f0 + g + 8 * (j >> 1)) * DP + n * 8 + 2 * t + (j & 1)] = acc0[0][n][j];
+      for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int n = 0; n < NO; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int at = (f0 + a * 16 + g + 8 * (j >> 1)) * DP + n * 8 + 2 * t + (j & 1);
+            if (i == 0 && upper) {
+              F1[at] = acc0[a][n][j];
+              if constexpr (BOTH) F2[at] = acc1[a][n][j];
+            }
+            if (i == 1) {
+              acc0[a][n][j] += F1[at];
+              if constexpr (BOTH) acc1[a][n][j] += F2[at];
+            }
+          }
+      if (i == 0) __syncthreads();
+      if (i == 0 && upper) return;
     }
-    __syncthreads();
-    if (upper) return;
-#pragma unroll
-    for (int n = 0; n < NO; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc0[0][n][j] += F1[(f0 + g + 8 * (j >> 1)) * DP + n * 8 + 2 * t + (j & 1)];
   }
 #pragma unroll
   for (int a = 0; a < MT; ++a)
@@ -310,7 +320,7 @@ __device__ __forceinline__ void bwd_walk(const BKernel& A, const BWalk& W, unsig
 
 // The columns' CTAs first: their steps are the longer ones.
 template <typename T, int DC>
-__global__ void __launch_bounds__(BShape<DC>::kThreads, BShape<DC>::kResident) xattn_bwd_mma_kernel(const BKernel A) {
+__global__ void __launch_bounds__(BShape<DC>::kThreads, 1) xattn_bwd_mma_kernel(const BKernel A) {
   extern __shared__ __align__(16) float smb[];
   if (blockIdx.x < A.cols.ctas) bwd_walk<T, DC, true>(A, A.cols, blockIdx.x, smb);
   else bwd_walk<T, DC, false>(A, A.rows, blockIdx.x - A.cols.ctas, smb);
@@ -354,16 +364,17 @@ BPlan bwd_plan(const trnsparse_attention_args* a, const XSide& s) {
   p.dc = a->head_dim <= 64 ? 1 : a->head_dim <= 128 ? 2 : 4;
   const int64_t R = side_rows(s);
   const int64_t fixed[2] = {R, s.klen}, walk[2] = {s.klen, R};
-  const int resident = p.dc == 1 ? 2 : 1, bt = p.dc == 4 ? 64 : 128;
+  const int bt = p.dc == 4 ? BShape<4>::kRows : BShape<1>::kRows;
+  const int64_t wt = p.dc == 1 ? BShape<1>::kWalk : BShape<2>::kWalk;
   const int64_t rows = a->batch * a->q_heads * a->q_len, keys = a->batch * a->kv_heads * a->k_len;
   p.ws = (sizeof(float) * static_cast<size_t>(rows) + 255) & ~static_cast<size_t>(255);
   for (int i = 0; i < 2; ++i) {
     p.tiles[i] = static_cast<int>((fixed[i] + bt - 1) / bt);
-    const int64_t ctas = static_cast<int64_t>(p.tiles[i]) * s.nb * s.hkv, steps = (walk[i] + kBwdWalk - 1) / kBwdWalk;
+    const int64_t ctas = static_cast<int64_t>(p.tiles[i]) * s.nb * s.hkv, steps = (walk[i] + wt - 1) / wt;
     // both walks run side by side: three and four of the seven products. Half a step a part: 108 us against 133 with
     // a tenth at 2 x 8/2 heads, 333 x 517 x 64
-    const int64_t per = walk_steps(ctas, steps, sm_count() * (3 + i) / 7, resident, 32, 0.5);
-    p.chunk[i] = static_cast<int>(per * kBwdWalk);
+    const int64_t per = walk_steps(ctas, steps, sm_count() * (3 + i) / 7, 1, 32, 0.5);
+    p.chunk[i] = static_cast<int>(per * wt);
     p.parts[i] = static_cast<int>(steps > 0 ? (steps + per - 1) / per : 1);
     p.at[i] = p.ws;
     if (p.parts[i] > 1)
