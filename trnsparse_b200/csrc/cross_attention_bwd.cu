@@ -17,7 +17,7 @@
 //
 // What bounds it: the tensor cores' tf32 rate (3xTF32, xattn_tf32.cuh), kept about 60%
 // busy with two warps a scheduler; the rest goes to splitting operands and to waits
-// inside a warp's chain of scores, P and sums. 2 x 16/16 heads, 1024 x 1024 x 64: 634 us,
+// inside a warp's chain of scores, P and sums. 2 x 16/16 heads, 1024 x 1024 x 64: 644 us,
 // 47 TFLOP/s of the seven products (on the CUDA cores 1171 us); 16/4 heads at head_dim
 // 128 1278 us (2440); 2 x 8/2 heads, 333 x 517 x 64, where a CTA an SM is all there is,
 // 96 us (108 with four warps a CTA, two CTAs an SM; that took 584 at the first size).
