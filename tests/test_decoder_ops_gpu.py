@@ -537,3 +537,19 @@ def test_lengths_of_64_bits_are_clamped_before_they_are_narrowed(dtype):
     got = ts.shared_prefix_attention(q, pk, pv, k, v, wide)
     assert torch.equal(got, ts.shared_prefix_attention(q, pk, pv, k, v, narrow))
     assert ts.cross_attention(q, k, v, wide)[2].eq(0).all() and ts.cross_attention(q, k, v, wide)[0].ne(0).any()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_walks_without_steps_leave_zero_gradients(D):
+    """Sequences without keys, and lengths that end before a range of the walk begins, in fp32."""
+    g = _gen(92)
+    B, Hq, Hkv, T, S = 16, 4, 2, 130, 1500
+    lengths = torch.tensor([0, 1, 0, 40, S, 0, 0, 64] * 2, dtype=torch.int32, device="cuda")
+    q, k, v = (_randn(g, B, h, n, D).requires_grad_() for h, n in ((Hq, T), (Hkv, S), (Hkv, S)))
+    dout = _randn(g, B, Hq, T, D)
+    for _ in range(3):
+        dq, dk, dv = torch.autograd.grad(ts.cross_attention(q, k, v, lengths), (q, k, v), dout)
+        for b, n in enumerate(lengths.tolist()):
+            assert dk[b, :, n:].eq(0).all() and dv[b, :, n:].eq(0).all()
+            assert n > 0 or dq[b].eq(0).all()
+            assert n == 0 or dv[b, :, :n].ne(0).any()

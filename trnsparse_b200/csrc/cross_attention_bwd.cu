@@ -262,6 +262,7 @@ __device__ __forceinline__ void bwd_walk(const BKernel& A, const BWalk& W, unsig
     if (more) put_stats(X + stage * XS);
   }
   if constexpr (HALF) {  // both halves' sums, through the fixed tiles
+    cp_async_wait_all();  // a walk without steps has not waited for them
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
