@@ -39,7 +39,7 @@
 // a half (a quarter of them as a polynomial on the FMA pipe): 16 heads, 4096 x 4096 x
 // 128 137 us, 1000 TFLOP/s; 4 x 16 heads, 2048 x 4096 x 128 with the row statistics 255
 // us, 1078. Short or ragged items lose 3 to 5 us an item and CTA to its start and end
-// and the join: prompts of 4 x 32/8 heads, 777 x up to 2049 keys 87 + 22 us. Few rows
+// and the join: prompts of 4 x 32/8 heads, 777 x up to 2049 keys 87 + 12 us. Few rows
 // (a shared prefix, 256 rows a key head): memory and that same start and end.
 //
 // Hidden keys (past a length, or masked): scores become -inf by selection, and
@@ -608,15 +608,16 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
   }
 }
 
-// Joins the pieces of every row of the split part. A thread has 4 elements of a row, rows fastest, as the slots are
-// laid out (whole lines for 32 rows); a block has up to 32 rows and 8 groups of 4 elements. One side: rows of a split item (items that one CTA finished are done). Two sides:
-// 32 packed rows of the prefix's items of a key head, which are rows of one or more sequences' own items.
-// BATCH pieces of a thread are in flight together (a load takes about a microsecond here, so what counts is how many
-// follow one another): 8 where an item has few rows and many pieces, or a prefix's; 2 where large items were cut
-// once, so that more threads fit on an SM.
-template <int BATCH>
-__global__ void __launch_bounds__(256, BATCH > 2 ? 2 : 5) xattn_join_kernel(const __grid_constant__ FwArgs A) {
-  __shared__ __align__(16) uint2 tile[32][8];
+// Joins the pieces of every row of the split part. A thread has 4 elements of a row in U places 32 elements apart, rows
+// fastest, as the slots are laid out (whole lines for 32 rows); a block has up to 32 rows and 8 U groups of 4 elements.
+// One side: rows of a split item (items that one CTA finished are done). Two sides: 32 packed rows of the prefix's
+// items of a key head, which are rows of one or more sequences' own items.
+// A load takes about a microsecond here, so what counts is how many follow one another: BATCH pieces of a thread are in
+// flight together, 8 where an item has few rows and many pieces, or a prefix's; 2 in U = 4 places where large items
+// were cut once.
+template <int BATCH, int U>
+__global__ void __launch_bounds__(256, U > 1 ? 3 : 2) xattn_join_kernel(const __grid_constant__ FwArgs A) {
+  __shared__ __align__(16) uint2 tile[32][8 * U];
   const FwSide& L = A.side[0];  // whose rows the blocks walk
   const FwSide& S = A.side[A.sides - 1];
   const int item = A.sides == 1 ? blockIdx.x + L.first : blockIdx.x;
@@ -625,42 +626,52 @@ __global__ void __launch_bounds__(256, BATCH > 2 ? 2 : 5) xattn_join_kernel(cons
   const int64_t R = side_rows(L.s), row0 = static_cast<int64_t>(rt) * L.tile_rows + blockIdx.y * 32;
   const int rows = static_cast<int>(min(static_cast<int64_t>(32), min(R, static_cast<int64_t>(rt + 1) * L.tile_rows) - row0));
   if (rows <= 0) return;
-  const int c0 = blockIdx.z * 8, cw = min(8, A.D / 4 - c0);
+  const int c0 = blockIdx.z * 8 * U, cw = min(8 * U, A.D / 4 - c0);
   grid_dep_wait();
   const int n = fw_tiles(L, bi);
   const int2 p = n > 0 ? L.pieces[item - L.first] : make_int2(0, -1);
   if (A.sides == 1 && n > 0 && p.x == p.y) return;
-  for (int i = threadIdx.x; i < rows * cw; i += blockDim.x) {
-    const int c = i / rows, r = i - c * rows, c4 = c0 + c;
+  for (int i = threadIdx.x; i < rows * min(8, cw); i += blockDim.x) {
+    const int c = i / rows, r = i - c * rows;
     const int64_t row = row0 + r;
     float mx = -INFINITY, den = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 acc[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](const float* slots, const float* lse, int stride, int at, int count, auto&& slot_of) {
       for (int k0 = 0; k0 < count; k0 += BATCH) {
         float ls[BATCH];
-        float4 o[BATCH];
+        float4 o[BATCH][U];
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
           ls[k] = -INFINITY;
-          o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int u = 0; u < U; ++u) o[k][u] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (k0 + k < count) {
             const int64_t slot = slot_of(k0 + k);
             ls[k] = lse[slot * stride + at];
-            o[k] = *reinterpret_cast<const float4*>(slots + slot * stride * A.D +
-                                                    (static_cast<int64_t>(c4) * stride + at) * 4);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+              if (U == 1 || c + 8 * u < cw)
+                o[k][u] = *reinterpret_cast<const float4*>(
+                    slots + slot * stride * A.D + (static_cast<int64_t>(c0 + c + 8 * u) * stride + at) * 4);
           }
         }
         float mn = mx;
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) mn = max3_nan(mn, mn, ls[k]);
-        const float base = mn == -INFINITY ? 0.f : mn, c = exp2f(mx - base);
-        den *= c;
-        acc = make_float4(acc.x * c, acc.y * c, acc.z * c, acc.w * c);
+        const float base = mn == -INFINITY ? 0.f : mn, f = exp2f(mx - base);
+        den *= f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) acc[u] = make_float4(acc[u].x * f, acc[u].y * f, acc[u].z * f, acc[u].w * f);
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
           const float w = exp2f(ls[k] - base);
           den += w;
-          acc = make_float4(fmaf(w, o[k].x, acc.x), fmaf(w, o[k].y, acc.y), fmaf(w, o[k].z, acc.z), fmaf(w, o[k].w, acc.w));
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            acc[u] = make_float4(fmaf(w, o[k][u].x, acc[u].x), fmaf(w, o[k][u].y, acc[u].y),
+                                 fmaf(w, o[k][u].z, acc[u].z), fmaf(w, o[k][u].w, acc[u].w));
         }
         mx = mn;
       }
@@ -686,14 +697,18 @@ __global__ void __launch_bounds__(256, BATCH > 2 ? 2 : 5) xattn_join_kernel(cons
     pieces(p, L, item, blockIdx.y * 32 + r);
     if (A.sides > 1) pieces(own, S, own_item, own_at);
     const float inv = den == 0.f ? 0.f : 1.f / den;
-    const uint2 v = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-    if (rows == 32) tile[r][c] = v;
-    else *reinterpret_cast<uint2*>(A.out + o_offset(S.s, ob, h, x) + c4 * 4) = v;
-    if (A.lse != nullptr && c4 == 0) A.lse[flat_row(S.s, ob, h, x)] = den == 0.f ? -INFINITY : mx + log2f(den);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint2 v =
+          make_uint2(pack_bf16(acc[u].x * inv, acc[u].y * inv), pack_bf16(acc[u].z * inv, acc[u].w * inv));
+      if (rows == 32) tile[r][c + 8 * u] = v;
+      else if (c + 8 * u < cw) *reinterpret_cast<uint2*>(A.out + o_offset(S.s, ob, h, x) + (c0 + c + 8 * u) * 4) = v;
+    }
+    if (A.lse != nullptr && c0 + c == 0) A.lse[flat_row(S.s, ob, h, x)] = den == 0.f ? -INFINITY : mx + log2f(den);
   }
   if (rows < 32) return;
   __syncthreads();
-  // 32 rows leave in 64 contiguous bytes each
+  // 32 rows leave in 64 U contiguous bytes each
   for (int i = threadIdx.x; i < 32 * (cw / 2); i += blockDim.x) {
     const int r = i / (cw / 2), u = i - r * (cw / 2);
     XRow x = fw_row(L, row0 + r);
@@ -702,7 +717,8 @@ __global__ void __launch_bounds__(256, BATCH > 2 ? 2 : 5) xattn_join_kernel(cons
       ob = x.b2;
       x.b2 = 0;
     }
-    *reinterpret_cast<uint4*>(A.out + o_offset(S.s, ob, h, x) + c0 * 4 + u * 8) = *reinterpret_cast<const uint4*>(&tile[r][u * 2]);
+    *reinterpret_cast<uint4*>(A.out + o_offset(S.s, ob, h, x) + c0 * 4 + u * 8) =
+        *reinterpret_cast<const uint4*>(&tile[r][u * 2]);
   }
 }
 
@@ -879,8 +895,11 @@ int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, c
   const int blocks = n == 1 ? l.split_items : W.items;
   if (blocks == 0) return TRNSPARSE_OK;
   const int threads = W.item_rows >= 32 ? 256 : (W.item_rows * 8 + 31) & ~31;
-  auto kern = n == 1 && W.item_rows >= 32 ? xattn_join_kernel<2> : xattn_join_kernel<8>;
-  cudaError_t e = launch_pdl(kern, dim3(blocks, (W.item_rows + 31) / 32, (a->head_dim / 4 + 7) / 8), dim3(threads), 0, st, J);
+  const bool large = n == 1 && W.item_rows >= 32;
+  auto kern = large ? xattn_join_kernel<2, 4> : xattn_join_kernel<8, 1>;
+  const unsigned groups = large ? 32 : 8;  // of 4 elements a block
+  cudaError_t e = launch_pdl(kern, dim3(blocks, (W.item_rows + 31) / 32, (a->head_dim / 4 + groups - 1) / groups),
+                             dim3(threads), 0, st, J);
   if (e != cudaSuccess) return cuda_status(e, "attention (tensor cores): join");
   return debug_sync(st, "attention (tensor cores): join");
 }
