@@ -35,6 +35,8 @@ from .ops import (
 )
 from .screening import density_screen, schwarz_bounds, screen_quartets, sparsity_stats
 
+# The reference's names, and no others: `import *` stays a drop-in. The decoder operators (cross_attention,
+# qk_norm_rope, shared_prefix_attention) are reached by name.
 __all__ = [
     "CSRMatrix",
     "COOMatrix",
@@ -48,9 +50,6 @@ __all__ = [
     "bsr_spmm",
     "screened_spmm",
     "block_sparse_attention_tiled",
-    "qk_norm_rope",
-    "cross_attention",
-    "shared_prefix_attention",
     "sparse_add",
     "sparse_scale",
     "sparse_transpose",
