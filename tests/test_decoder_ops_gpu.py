@@ -553,3 +553,19 @@ def test_walks_without_steps_leave_zero_gradients(D):
             assert dk[b, :, n:].eq(0).all() and dv[b, :, n:].eq(0).all()
             assert n > 0 or dq[b].eq(0).all()
             assert n == 0 or dv[b, :, :n].ne(0).any()
+
+
+@pytest.mark.parametrize("dtype,B,Hq,Hkv,Sq,Sk,D,kind", [
+    (F32, 3, 8, 2, 100, 700, 64, "both"),      # several ranges of keys and of rows
+    (F32, 1, 4, 4, 257, 33, 128, "mask"),      # one row past two tiles, one key past a tile
+    (F32, 2, 2, 1, 600, 1300, 48, "lengths"),
+    (F32, 1, 2, 2, 300, 500, 256, "both"),
+    (F32, 2, 4, 1, 8, 900, 64, "lengths"),     # 32 packed rows: the last of the few-rows form
+    (F32, 2, 4, 1, 9, 900, 96, "mask"),        # 36: the first of the other
+    (F32, 1, 1, 1, 128, 128, 65, "none"),      # rows that do not start on 16 bytes
+    (F32, 1, 1, 1, 64, 6000, 64, "none"),      # long sums
+    (BF16, 1, 2, 1, 150, 200, 200, "lengths"),
+    (BF16, 2, 2, 1, 70, 300, 36, "both"),
+])
+def test_cross_attention_at_the_tiles_of_the_split_products(dtype, B, Hq, Hkv, Sq, Sk, D, kind):
+    test_cross_attention(dtype, B, Hq, Hkv, Sq, Sk, D, kind)

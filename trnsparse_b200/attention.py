@@ -321,8 +321,8 @@ def cross_attention(
     ``(batch,)`` integers, the leading keys of each sequence that count
     (clamped to ``[0, k_len]``). ``key_mask``: ``(batch, k_len)`` bool, True
     where a key counts; given both, a key must pass both. What hidden keys
-    hold (NaN included) does not matter; a row without keys is zero, and so
-    are its gradients. ``scale`` defaults to ``head_dim ** -0.5``. The result
+    hold (NaN included) does not matter, the others are finite; a row without
+    keys is zero, and so are its gradients. ``scale`` defaults to ``head_dim ** -0.5``. The result
     has ``q``'s layout; softmax in float32. Differentiable in ``q``, ``k``,
     ``v``; gradients are summed in a fixed order.
     """
@@ -365,7 +365,7 @@ def shared_prefix_attention(
     integers, how many of them are filled (clamped to ``[0, capacity]``), the
     new tokens included: token t of T attends the whole prefix and the first
     ``lengths - T + 1 + t`` own keys. Rows behind a length are never read into
-    a result. float32 or bfloat16, head_dim up to 256, any strides (a slice of
+    a result; what is read is finite. float32 or bfloat16, head_dim up to 256, any strides (a slice of
     a larger cache needs no copy). A row without any key is zero. For serving:
     operands that require gradients are refused.
     """
