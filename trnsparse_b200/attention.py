@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -62,6 +63,18 @@ def _to(t: torch.Tensor | None, dev: torch.device, dtype: torch.dtype | None = N
 
 def _grad_wanted(*ts: torch.Tensor | None) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def _refuse_dropped(name: str, operands: tuple, constants: dict) -> None:
+    """Refuses derivatives that the kernels would drop: tangents of forward mode on any operand (``requires_grad`` does
+    not show them), and gradients of ``constants``, which the operator is not differentiable in."""
+    if forward_ad._current_level >= 0:
+        for t in (*operands, *constants.values()):
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no forward-mode derivative: an operand has a tangent")
+    for what, t in constants.items():
+        if isinstance(t, torch.Tensor) and _grad_wanted(t):
+            raise RuntimeError(f"{name} is not differentiable in {what}: detach it")
 
 
 def _result(out: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
@@ -170,7 +183,8 @@ def qk_norm_rope(
     float64 on the device (other types are converted at every call). Angles
     are formed in 64 bits, everything else in 32, rounded once.
     Differentiable in ``q``, ``k`` and the weights; gradients of the weights
-    are summed in a fixed order.
+    are summed in a fixed order. An ``inv_freq`` or ``eps`` that requires a
+    gradient, and forward-mode tangents, are refused.
     """
     assert q.dim() == 4 and k.dim() == 4, f"qk_norm_rope: q and k must be 4-D, got {tuple(q.shape)}, {tuple(k.shape)}"
     B, _, S, D = q.shape
@@ -194,6 +208,7 @@ def qk_norm_rope(
         if w.dtype not in _DTYPES or (wdt is not None and w.dtype != wdt):
             raise TypeError("qk_norm_rope: weights must be float32 or bfloat16, both alike")
         wdt = w.dtype
+    _refuse_dropped("qk_norm_rope", (q, k, q_weight, k_weight), {"inv_freq": inv_freq, "eps": eps})
     dev = _dev_of(q, k)
     qd, kd = _rows(_to(q, dev)), _rows(_to(k, dev))
     qw, kw = (None if w is None else _to(w, dev).contiguous() for w in (q_weight, k_weight))
@@ -324,7 +339,8 @@ def cross_attention(
     hold (NaN included) does not matter, the others are finite; a row without
     keys is zero, and so are its gradients. ``scale`` defaults to ``head_dim ** -0.5``. The result
     has ``q``'s layout; softmax in float32. Differentiable in ``q``, ``k``,
-    ``v``; gradients are summed in a fixed order.
+    ``v``; gradients are summed in a fixed order. A ``scale`` that requires a
+    gradient, and forward-mode tangents, are refused.
     """
     name = "cross_attention"
     _check_attention(name, q, k, v)
@@ -335,6 +351,7 @@ def cross_attention(
         if key_mask.dtype != torch.bool:
             raise TypeError(f"{name}: key_mask must be bool, got {key_mask.dtype}")
         assert tuple(key_mask.shape) == (B, Sk), f"{name}: key_mask must be ({B}, {Sk}), got {tuple(key_mask.shape)}"
+    _refuse_dropped(name, (q, k, v), {"scale": scale})
     scale = float(q.shape[3] ** -0.5 if scale is None else scale)
     dev = _dev_of(q, k, v)
     qd, kd, vd = (_tiles(_to(t, dev)) for t in (q, k, v))
@@ -367,7 +384,7 @@ def shared_prefix_attention(
     ``lengths - T + 1 + t`` own keys. Rows behind a length are never read into
     a result; what is read is finite. float32 or bfloat16, head_dim up to 256, any strides (a slice of
     a larger cache needs no copy). A row without any key is zero. For serving:
-    operands that require gradients are refused.
+    operands that require gradients or have forward-mode tangents are refused.
     """
     name = "shared_prefix_attention"
     _check_attention(name, q, k_cache, v_cache)
@@ -380,6 +397,7 @@ def shared_prefix_attention(
     _check_lengths(name, lengths, q.shape[0])
     if _grad_wanted(q, prefix_k, prefix_v, k_cache, v_cache):
         raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or detach its operands")
+    _refuse_dropped(name, (q, prefix_k, prefix_v, k_cache, v_cache), {"scale": scale})
     scale = float(D ** -0.5 if scale is None else scale)
     dev = _dev_of(q, prefix_k, k_cache)
     qd, pk, pv, kc, vc = (_tiles(_to(t, dev)) for t in (q, prefix_k, prefix_v, k_cache, v_cache))
