@@ -305,6 +305,12 @@ def _check_attention(name, q, k, v):
     _check_dtype(name, q, k, v)
 
 
+def _check_scale(name, scale, D):
+    scale = float(D ** -0.5 if scale is None else scale)
+    assert abs(scale) <= 1e38, f"{name}: scale must be finite in float32, got {scale}"  # a NaN fails too
+    return scale
+
+
 def _check_lengths(name, lengths, B):
     if lengths.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name}: lengths must be int32 or int64, got {lengths.dtype}")
@@ -337,8 +343,8 @@ def cross_attention(
     (clamped to ``[0, k_len]``). ``key_mask``: ``(batch, k_len)`` bool, True
     where a key counts; given both, a key must pass both. What hidden keys
     hold (NaN included) does not matter, the others are finite; a row without
-    keys is zero, and so are its gradients. ``scale`` defaults to ``head_dim ** -0.5``. The result
-    has ``q``'s layout; softmax in float32. Differentiable in ``q``, ``k``,
+    keys is zero, and so are its gradients. ``scale``, any finite number,
+    defaults to ``head_dim ** -0.5``. The result has ``q``'s layout; softmax in float32. Differentiable in ``q``, ``k``,
     ``v``; gradients are summed in a fixed order. A ``scale`` that requires a
     gradient, and forward-mode tangents, are refused.
     """
@@ -352,7 +358,7 @@ def cross_attention(
             raise TypeError(f"{name}: key_mask must be bool, got {key_mask.dtype}")
         assert tuple(key_mask.shape) == (B, Sk), f"{name}: key_mask must be ({B}, {Sk}), got {tuple(key_mask.shape)}"
     _refuse_dropped(name, (q, k, v), {"scale": scale})
-    scale = float(q.shape[3] ** -0.5 if scale is None else scale)
+    scale = _check_scale(name, scale, q.shape[3])
     dev = _dev_of(q, k, v)
     qd, kd, vd = (_tiles(_to(t, dev)) for t in (q, k, v))
     lengths = None if key_lengths is None else _lengths32(key_lengths, dev, Sk)
@@ -398,7 +404,7 @@ def shared_prefix_attention(
     if _grad_wanted(q, prefix_k, prefix_v, k_cache, v_cache):
         raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or detach its operands")
     _refuse_dropped(name, (q, prefix_k, prefix_v, k_cache, v_cache), {"scale": scale})
-    scale = float(D ** -0.5 if scale is None else scale)
+    scale = _check_scale(name, scale, D)
     dev = _dev_of(q, prefix_k, k_cache)
     qd, pk, pv, kc, vc = (_tiles(_to(t, dev)) for t in (q, prefix_k, prefix_v, k_cache, v_cache))
     lens = _lengths32(lengths, dev, kc.shape[2])

@@ -20,6 +20,8 @@
 // In both the next tile is copied asynchronously. When there are fewer CTAs than
 // fill the GPU the keys are cut into ranges, each writing (O, log-sum-exp) of its
 // part, joined afterwards.
+#include <math.h>
+
 #include "xattn_tf32.cuh"
 
 namespace tsb {
@@ -619,6 +621,9 @@ int check_attention(const trnsparse_attention_args* a, const char* what) {
                   a->q_heads < (1 << 16) && a->q_len < (1ll << 30) &&
                   a->batch * a->q_heads < (1ll << 30) && a->batch * a->q_heads * a->q_len < (1ll << 30),
               "%s: sizes out of range", what);
+  // the kernels scale by this in fp32; a NaN would pass the tensor cores' lower bound on it as if it were 0
+  TSB_REQUIRE(isfinite(static_cast<float>(a->scale * 1.4426950408889634)), "%s: scale %g is not finite in fp32", what,
+              a->scale);
   if (a->dtype != TRNSPARSE_F32 && a->dtype != TRNSPARSE_BF16)
     return fail(TRNSPARSE_ERR_DTYPE, "%s: dtype %d not supported (F32, BF16)", what, a->dtype);
   return TRNSPARSE_OK;
