@@ -30,3 +30,18 @@ def test_attention_scale_is_finite(scale):
                      "trnsparse_cross_attention_backward"):
             assert getattr(lib, name)(C.byref(a), None, 0, None) == _lib.ERR_ARG
             assert b"scale" in lib.trnsparse_last_error()
+
+
+@pytest.mark.parametrize("field,value,code", [
+    ("position_type", 2, _lib.ERR_DTYPE), ("position_type", -1, _lib.ERR_DTYPE),
+    ("batch", 1 << 33, _lib.ERR_ARG),  # batch * seq would pass 64 bits
+])
+def test_qk_norm_rope_positions_and_sizes(field, value, code):
+    """Refused by all three entry points, also where there is no head to work on."""
+    lib = _lib.load()
+    a = _lib.QkNormRopeArgs()
+    a.batch, a.seq, a.head_dim, a.rotary_dim, a.dtype, a.weight_dtype = 1, (1 << 31) - 1, 64, 64, _lib.F32, _lib.F32
+    setattr(a, field, value)
+    assert lib.trnsparse_qk_norm_rope(C.byref(a), None) == code
+    assert lib.trnsparse_qk_norm_rope_backward(C.byref(a), None, 0, None) == code
+    assert lib.trnsparse_qk_norm_rope_workspace_size(C.byref(a)) == 0

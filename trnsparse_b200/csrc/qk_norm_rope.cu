@@ -402,7 +402,7 @@ int qk_dispatch(const QkArgs& A, const QkPlan& p, bool f32, cudaStream_t st) {
 
 int qk_check(const trnsparse_qk_norm_rope_args* a) {
   TSB_REQUIRE(a != nullptr, "qk_norm_rope: null arguments");
-  TSB_REQUIRE(a->batch >= 0 && a->seq >= 0 && a->seq < (1ll << 31) && a->heads[0] >= 0 && a->heads[1] >= 0 &&
+  TSB_REQUIRE(a->batch >= 0 && a->batch < (1ll << 31) && a->seq >= 0 && a->seq < (1ll << 31) && a->heads[0] >= 0 && a->heads[1] >= 0 &&
                   a->heads[0] < 32768 && a->heads[1] < 32768,
               "qk_norm_rope: bad sizes");
   TSB_REQUIRE(a->head_dim >= 1 && a->head_dim <= 256, "qk_norm_rope: head_dim must be in [1, 256] (got %lld)",
@@ -413,6 +413,8 @@ int qk_check(const trnsparse_qk_norm_rope_args* a) {
     return fail(TRNSPARSE_ERR_DTYPE, "qk_norm_rope: dtype %d not supported (F32, BF16)", a->dtype);
   if (a->weight_dtype != TRNSPARSE_F32 && a->weight_dtype != TRNSPARSE_BF16)
     return fail(TRNSPARSE_ERR_DTYPE, "qk_norm_rope: weight dtype %d not supported (F32, BF16)", a->weight_dtype);
+  if (a->position_type != TRNSPARSE_I32 && a->position_type != TRNSPARSE_I64)
+    return fail(TRNSPARSE_ERR_DTYPE, "qk_norm_rope: position type %d not supported (I32, I64)", a->position_type);
   return TRNSPARSE_OK;
 }
 
