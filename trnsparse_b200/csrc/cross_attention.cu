@@ -72,7 +72,7 @@ struct XKernel {
   float *lse, *part_o, *part_lse;  // part_*: this side's first piece (null: one piece, written to out)
   int64_t rows_all;                // rows of one piece
   int D, row_tiles, chunk, vec;
-  float scale, scale_log2;
+  float scale_log2;
 };
 
 template <typename T, int BM, int NT, int DC>
@@ -569,7 +569,6 @@ int general_forward(const trnsparse_attention_args* a, bool prefix, void* ws, cu
     A.row_tiles = p.row_tiles[i];
     A.chunk = p.chunk[i];
     A.vec = four_aligned(a);
-    A.scale = static_cast<float>(a->scale);
     A.scale_log2 = static_cast<float>(a->scale * 1.4426950408889634);
     rc = a->dtype == TRNSPARSE_F32 ? general_dispatch<float>(A, p.bm[i], p.dc, p.splits[i], i > 0, st)
                                    : general_dispatch<__nv_bfloat16>(A, p.bm[i], p.dc, p.splits[i], i > 0, st);

@@ -67,7 +67,7 @@ struct BwArgs {
   int64_t s0[3], s1[3];      // their strides
   float *part0, *part1;      // fp32 parts [parts][rows][D], or null
   int64_t part_rows;
-  int B, Hq, Hkv, G, Sq, Sk, D, q_tiles, k_tiles, parts, chunk;
+  int Hq, Hkv, G, Sq, Sk, D, q_tiles, k_tiles, parts, chunk;
   int mul_h[4], mul_b[4];    // q, dout, k, v
   float scale, scale_log2;
 };
@@ -802,7 +802,6 @@ int xattn_bwd_tc(const trnsparse_attention_args* a, void* ws, cudaStream_t st) {
   A.mask_stride = a->key_mask_stride;
   A.nlse = lse;
   A.ndelta = delta;
-  A.B = (int)B;
   A.Hq = (int)Hq;
   A.Hkv = (int)Hk;
   A.G = (int)(Hq / Hk);

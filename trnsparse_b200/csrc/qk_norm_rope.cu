@@ -379,12 +379,9 @@ QkPlan qk_plan(const trnsparse_qk_norm_rope_args* a, bool bwd) {
 
 template <typename T, int VEC, int KU, bool INTER, bool BWD>
 int qk_launch(const QkArgs& A, const QkPlan& p, cudaStream_t st) {
+  // 256 / lpr groups of D floats: 8 KB at most over all plans (head_dim 256 on 32 lanes, 8 on one)
   const size_t smem = BWD ? sizeof(float) * static_cast<size_t>(kQkThreads / p.lpr) * A.D : 0;
   auto kern = qk_norm_rope_kernel<T, VEC, KU, INTER, BWD>;
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return cuda_status(e, "qk_norm_rope: set smem");
-  }
   kern<<<dim3(p.grid_x, p.chunks[0] + p.chunks[1]), kQkThreads, smem, st>>>(A, p.lpr);
   TSB_CHECK_LAUNCH("qk_norm_rope launch");
   return TRNSPARSE_OK;
