@@ -58,6 +58,9 @@ constexpr float kFwLazy = 8.f;
 // Key tiles that an item's start and end count for: 1, 2, 4 take 109.2, 109.3, 108.8 us in ragged prompts of 777 tokens
 // and 146.6, 147.3, 147.7 us in a step of 96 sequences over a shared prefix of 32768 keys.
 constexpr int kFwItemCost = 2;
+// Tiles after which a row's sum goes to its word in shared memory: terms are added one by one to a sum that then
+// stays below 2^15 P <= 2^23; terms of 1 added to one sum all along would be lost from 2^24 keys on.
+constexpr int kFwSumTiles = 256;
 constexpr int kFwLeast = 8;  // see fw_plan; 4, 8, 16: 60.1, 62.1, 74.7 us (64 sequences, prefix 8192, own keys to 1024)
 
 template <int HD>
@@ -68,7 +71,8 @@ struct FwLayout {
   static constexpr int kQ = 0;
   static constexpr int kRing = 2 * kTile;
   static constexpr int kBar = kRing + kStages * kTile;
-  static constexpr int kSmem = kBar + 512;
+  static constexpr int kSum = kBar + 512;  // float [256]
+  static constexpr int kSmem = kSum + 1024;
   static constexpr uint32_t kTmemO = 256;  // S / P: [0, 128) and [128, 256); O: [256, +HD) and [384, +HD)
 };
 
@@ -80,7 +84,7 @@ struct FwBars {
   int abort_flag;
 };
 
-static_assert(sizeof(FwBars) <= 512, "FwLayout::kSmem");
+static_assert(sizeof(FwBars) <= 512, "FwLayout::kSum");
 
 template <int HD>
 __global__ void __launch_bounds__(kFwThreads, 1)
@@ -314,6 +318,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
     const uint32_t t_s = tmem + half * 128 + lane_base, t_o = tmem + Lay::kTmemO + half * 128 + lane_base;
     const float sl = A.scale_log2;
     uint8_t* const q_tile = sb + Lay::kQ + half * Lay::kTile;
+    float* const sums = reinterpret_cast<float*>(sb + Lay::kSum);
     // a wait that gave up ends the whole warp's work (its lanes vote and exchange below)
     int seg_no = 0, tile_no = 0;
     int v_slot = 1, v_use = 0;  // ring position of the current tile's V
@@ -404,6 +409,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
       const uint8_t* mask = s.mask ? s.mask + g.bi * s.mask_stride : nullptr;
       const bool warp_live = __any_sync(0xffffffffu, live);
       float m = -INFINITY, l = 0.f;
+      sums[threadIdx.x] = 0.f;
       for (int j = g.k0; j < g.k1; ++j, ++tile_no) {
         const int key0 = j * kFwKeys;
         // clean: every key of the tile counts; part: some are hidden from a row of this warp
@@ -483,6 +489,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
           const float corr = ex2(m - mu);  // 1 when m stays, 0 before the first key
           // s_full of this tile implies the previous P V has completed: O may be rescaled
           if (j > g.k0 && __any_sync(0xffffffffu, mnew != m)) {
+            sums[threadIdx.x] *= corr;
 #pragma unroll 1
             for (int c = 0; c < HD / 16; ++c) {
               uint32_t o[16];
@@ -532,6 +539,10 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
           unpack2(sum_a, s0, s1);
           unpack2(sum_b, s2, s3);
           l = (s0 + s1) + (s2 + s3);
+          if ((j - g.k0) % kFwSumTiles == kFwSumTiles - 1) {
+            sums[threadIdx.x] += l;
+            l = 0.f;
+          }
           tmem_wait_st();
         } else {
           mbar_arrive(&B.p_half[half]);
@@ -546,6 +557,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
       ++seg_no;
       tc_fence_after();
       if (warp_live) {
+        l += sums[threadIdx.x];
         const float inv = m == -INFINITY ? 0.f : 1.f / l;  // no key: zero
         const float ls = m == -INFINITY ? -INFINITY : m + log2f(l);
         const XRow x = fw_row(sd, live ? row : 0);
