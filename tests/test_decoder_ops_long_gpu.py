@@ -16,7 +16,7 @@ BF16 = torch.bfloat16
 
 def _ones(B, Sq, Sk, D, lengths=None):
     """Queries, keys and values of ones, the keys of all sequences the same memory. The result is 1: the scores are
-    equal, P is 1, and 16 ones (a product's step) added to a multiple of 16 below 2^28 are exact in fp32."""
+    equal, P is 1, and sums of ones are exact in fp32 up to 2^24."""
     q = torch.ones(B, 1, Sq, D, device="cuda", dtype=BF16)
     k = torch.ones(1, 1, Sk, D, device="cuda", dtype=BF16).expand(B, 1, Sk, D)
     out = ts.cross_attention(q, k, k, lengths)
@@ -27,3 +27,39 @@ def _ones(B, Sq, Sk, D, lengths=None):
 def test_row_sums_pass_2_to_the_24():
     """148 items of 17 rows: a whole one for every CTA."""
     _ones(148, 17, 1 << 25, 8)
+
+
+@pytest.mark.parametrize("B,Sq,D", [(148, 17, 64), (148, 200, 128), (3, 40, 64)])
+def test_long_sums_do_not_shrink(B, Sq, D):
+    """2^21 keys, values of mean 1, whole on a CTA or cut. The tensor core cuts a product to the accumulator's last place:
+    less than 2^-25 of the sum each, so at most 2^-8 of it over the 2^17 keys of one accumulator. The other roundings
+    (P and the result, half a step 2^-8 each) go both ways: their mean over N results stays below 4 2^-8 / sqrt(N)."""
+    g = torch.Generator(device="cuda").manual_seed(111)
+    n = 1 << 21
+    q, k = (torch.randn(1, 1, s, D, generator=g, device="cuda").to(BF16) for s in (Sq, n))
+    v = (1 + torch.randn(1, 1, n, D, generator=g, device="cuda")).to(BF16)
+    out = ts.cross_attention(*(t.expand(B, *t.shape[1:]) for t in (q, k, v)))
+    assert all(torch.equal(out[i], out[0]) for i in range(1, B) if B == 148)
+    ref = torch.cat([torch.softmax(r.double() @ k[0, 0].double().T * D ** -0.5, -1) @ v[0, 0].double()
+                     for r in q[0, 0].split(20)])
+    for o in out[:3, 0].double():
+        bias = ((o - ref) * ref.sign()).mean().item() / ref.abs().mean().item()
+        assert abs(bias) <= 2.0 ** -8 + 4 * 2.0 ** -8 / ref.numel() ** 0.5
+        assert ((o - ref).norm() / ref.norm()).item() <= 2 * 2.0 ** -8
+
+
+def test_flushed_sums_follow_a_rising_maximum():
+    """The scores rise by 40 over the keys, a maximum that moves between and after flushes; the last keys decide."""
+    n, D = 1 << 19, 64
+    g = torch.Generator(device="cuda").manual_seed(112)
+    k = torch.zeros(1, 1, n, D, device="cuda")
+    k[..., 0] = torch.linspace(0, 40, n, device="cuda")
+    k, v = k.to(BF16), torch.randn(1, 1, n, D, generator=g, device="cuda").to(BF16)
+    q = torch.zeros(148, 1, 17, D, device="cuda", dtype=BF16)
+    rise = torch.tensor([1.0, 0.0, -1.0, 0.25], device="cuda")
+    q[:, 0, :4, 0] = rise.to(BF16)
+    out = ts.cross_attention(q, k.expand(148, 1, n, D), v.expand(148, 1, n, D), scale=1.0)
+    p = torch.softmax(rise[:, None].double() * k[0, 0, :, 0].double(), -1)
+    ref, mass = p @ v[0, 0].double(), p @ v[0, 0].double().abs()
+    # P rounded to bf16, the result too, and the chain's cuts (above)
+    check(out[0, 0, :4], ref, 3 * 2.0 ** -8 * mass, "out")

@@ -58,9 +58,11 @@ constexpr float kFwLazy = 8.f;
 // Key tiles that an item's start and end count for: 1, 2, 4 take 109.2, 109.3, 108.8 us in ragged prompts of 777 tokens
 // and 146.6, 147.3, 147.7 us in a step of 96 sequences over a shared prefix of 32768 keys.
 constexpr int kFwItemCost = 2;
-// Tiles after which a row's sum goes to its word in shared memory: terms are added one by one to a sum that then
-// stays below 2^15 P <= 2^23; terms of 1 added to one sum all along would be lost from 2^24 keys on.
-constexpr int kFwSumTiles = 256;
+// Tiles after which a row's accumulator and sum are added to fp32 sums in memory and start from zero again. The tensor
+// core cuts what it adds to the accumulator's last place, so sums of one sign shrink with the chain: 0.07% after 2^17
+// keys, 0.25% after 2^19, 1% after 2^21 (values of mean 1), and terms below 2^-25 of the sum vanish. The row's sum is
+// added to term by term, where terms below 2^-24 of it vanish.
+constexpr int kFwFlushTiles = 1024;
 constexpr int kFwLeast = 8;  // see fw_plan; 4, 8, 16: 60.1, 62.1, 74.7 us (64 sequences, prefix 8192, own keys to 1024)
 
 template <int HD>
@@ -71,8 +73,8 @@ struct FwLayout {
   static constexpr int kQ = 0;
   static constexpr int kRing = 2 * kTile;
   static constexpr int kBar = kRing + kStages * kTile;
-  static constexpr int kSum = kBar + 512;  // float [256]
-  static constexpr int kSmem = kSum + 1024;
+  static constexpr int kFlushed = kBar + 512;  // float [2][256]
+  static constexpr int kSmem = kFlushed + 2048;
   static constexpr uint32_t kTmemO = 256;  // S / P: [0, 128) and [128, 256); O: [256, +HD) and [384, +HD)
 };
 
@@ -84,7 +86,7 @@ struct FwBars {
   int abort_flag;
 };
 
-static_assert(sizeof(FwBars) <= 512, "FwLayout::kSum");
+static_assert(sizeof(FwBars) <= 512, "FwLayout::kFlushed");
 
 template <int HD>
 __global__ void __launch_bounds__(kFwThreads, 1)
@@ -318,7 +320,29 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
     const uint32_t t_s = tmem + half * 128 + lane_base, t_o = tmem + Lay::kTmemO + half * 128 + lane_base;
     const float sl = A.scale_log2;
     uint8_t* const q_tile = sb + Lay::kQ + half * Lay::kTile;
-    float* const sums = reinterpret_cast<float*>(sb + Lay::kSum);
+    // This row's flushed sum, the maximum it refers to, and its flushed accumulator (four elements in 16 bytes, a warp's
+    // rows side by side).
+    float* const flushed_l = reinterpret_cast<float*>(sb + Lay::kFlushed);
+    float* const flushed_m = flushed_l + kFwRows;
+    // The accumulator plus f times the flushed one: kept there with zeros in TMEM, or left in TMEM at the end of an item.
+    auto move_sums = [&](float f, bool first, bool out) {
+      float4* at = reinterpret_cast<float4*>(A.flush + static_cast<int64_t>(blockIdx.x) * kFwRows * HD) + threadIdx.x;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 4, at += kFwRows) {
+        uint32_t o[4];
+        tmem_ld4(t_o + c, o);
+        tmem_wait_ld();
+        float4 a = first ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
+        a = make_float4(fmaf(a.x, f, __uint_as_float(o[0])), fmaf(a.y, f, __uint_as_float(o[1])),
+                        fmaf(a.z, f, __uint_as_float(o[2])), fmaf(a.w, f, __uint_as_float(o[3])));
+        if (out) {
+          *at = a;
+          a = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        tmem_st4(t_o + c, __float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(a.z), __float_as_uint(a.w));
+      }
+      tmem_wait_st();
+    };
     // a wait that gave up ends the whole warp's work (its lanes vote and exchange below)
     int seg_no = 0, tile_no = 0;
     int v_slot = 1, v_use = 0;  // ring position of the current tile's V
@@ -409,7 +433,6 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
       const uint8_t* mask = s.mask ? s.mask + g.bi * s.mask_stride : nullptr;
       const bool warp_live = __any_sync(0xffffffffu, live);
       float m = -INFINITY, l = 0.f;
-      sums[threadIdx.x] = 0.f;
       for (int j = g.k0; j < g.k1; ++j, ++tile_no) {
         const int key0 = j * kFwKeys;
         // clean: every key of the tile counts; part: some are hidden from a row of this warp
@@ -454,6 +477,15 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
             }
             tmem_wait_st();
           }
+          // s_full of this tile implies the previous P V has completed
+          if (j > g.k0 && (j - g.k0) % kFwFlushTiles == 0) {
+            const bool first = j - g.k0 == kFwFlushTiles;
+            const float was = first ? -INFINITY : flushed_m[threadIdx.x], f = was == -INFINITY ? 0.f : ex2(was - m);
+            move_sums(f, first, true);
+            flushed_l[threadIdx.x] = first ? l : fmaf(flushed_l[threadIdx.x], f, l);
+            flushed_m[threadIdx.x] = m;
+            l = 0.f;
+          }
           // Scores come in chunks of 32 columns, and the first two are read again once the maximum is known:
           // all 128 do not fit beside the rest of a thread's 168 registers, and a spill is slow (224 KB of
           // shared memory leave local memory no L1). A chunk is in flight while the one before is used. One in
@@ -489,7 +521,6 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
           const float corr = ex2(m - mu);  // 1 when m stays, 0 before the first key
           // s_full of this tile implies the previous P V has completed: O may be rescaled
           if (j > g.k0 && __any_sync(0xffffffffu, mnew != m)) {
-            sums[threadIdx.x] *= corr;
 #pragma unroll 1
             for (int c = 0; c < HD / 16; ++c) {
               uint32_t o[16];
@@ -539,10 +570,6 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
           unpack2(sum_a, s0, s1);
           unpack2(sum_b, s2, s3);
           l = (s0 + s1) + (s2 + s3);
-          if ((j - g.k0) % kFwSumTiles == kFwSumTiles - 1) {
-            sums[threadIdx.x] += l;
-            l = 0.f;
-          }
           tmem_wait_st();
         } else {
           mbar_arrive(&B.p_half[half]);
@@ -557,7 +584,11 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
       ++seg_no;
       tc_fence_after();
       if (warp_live) {
-        l += sums[threadIdx.x];
+        if (g.k1 - g.k0 > kFwFlushTiles) {
+          const float was = flushed_m[threadIdx.x], f = was == -INFINITY ? 0.f : ex2(was - m);
+          l = fmaf(flushed_l[threadIdx.x], f, l);
+          move_sums(f, false, false);
+        }
         const float inv = m == -INFINITY ? 0.f : 1.f / l;  // no key: zero
         const float ls = m == -INFINITY ? -INFINITY : m + log2f(l);
         const XRow x = fw_row(sd, live ? row : 0);
@@ -739,7 +770,7 @@ struct FwLaunch {
   bool few;
   int sides, side[2], grid, whole, split_items, slot_rows;
   int64_t items[2];
-  size_t o, lse, item_o[2], item_lse[2], pieces[2];  // byte offsets in the workspace
+  size_t o, lse, flush, item_o[2], item_lse[2], pieces[2];  // byte offsets in the workspace
 };
 struct FwPlan {
   int launches;
@@ -759,12 +790,13 @@ FwPlan fw_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n) {
     l.sides = p.launches == 2 ? 1 : n;
     l.few = few[p.launches == 2 ? i : 0];
     const int64_t tile_rows = l.few ? kFewRows : kFwRows, shift = l.few ? kFewKeyShift : kFwKeyShift;
-    int64_t most = 0, tiles = 0, items = 0;
+    int64_t most = 0, tiles = 0, items = 0, longest = 0;
     for (int j = 0; j < l.sides; ++j) {
       const XSide& x = s[l.side[j] = p.launches == 2 ? i : j];
       const int64_t R = side_rows(x);
       l.items[j] = (R + tile_rows - 1) / tile_rows * x.nb * x.hkv;
       items += l.items[j];
+      longest = longest > (x.klen >> shift) ? longest : x.klen >> shift;
       tiles += l.items[j] * ((x.klen + (1ll << shift) - 1) >> shift);
       most = most > R ? most : R;
     }
@@ -787,6 +819,7 @@ FwPlan fw_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n) {
     };
     l.o = take(sizeof(float) * 2 * l.grid * l.slot_rows * D);
     l.lse = take(sizeof(float) * 2 * l.grid * l.slot_rows);
+    l.flush = take(!l.few && longest >= kFwFlushTiles ? sizeof(float) * l.grid * kFwRows * (D <= 64 ? 64 : 128) : 0);
     for (int j = 0; j < l.sides; ++j) {
       const int64_t R = side_rows(s[l.side[j]]), rows = R < tile_rows ? R : tile_rows;
       l.item_o[j] = take(n > 1 ? sizeof(float) * l.items[j] * rows * D : 0);
@@ -885,6 +918,7 @@ int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, c
       rc = few_rows_launch(A, l.grid, i > 0, st);
     } else {
       A.item_cost = kFwItemCost;
+      A.flush = reinterpret_cast<float*>(w + l.flush);
       XMap m[4];
       for (int j = 0; j < l.sides && !rc; ++j) {
         FwSide& S = A.side[j];
