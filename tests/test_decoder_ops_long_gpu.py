@@ -63,3 +63,19 @@ def test_flushed_sums_follow_a_rising_maximum():
     ref, mass = p @ v[0, 0].double(), p @ v[0, 0].double().abs()
     # P rounded to bf16, the result too, and the chain's cuts (above)
     check(out[0, 0, :4], ref, 3 * 2.0 ** -8 * mass, "out")
+
+
+def test_an_item_that_takes_more_than_a_second():
+    """Sequence 0 has 2^28 keys, 739 others one (1.3 us a tile: 2.8 s). The CTA that has it has five items; the roles
+    that are through with their part of the first one (the list of items, the warps of rows 128 to 255) wait for the
+    others, longer than a pipeline stage ever takes. The last key of sequence 0 outweighs all others together."""
+    B, Sk, D = 740, 1 << 28, 8
+    k = torch.zeros(1, 1, Sk, D, device="cuda", dtype=BF16)
+    v = torch.ones(1, 1, Sk, D, device="cuda", dtype=BF16)
+    k[..., -1, :], v[..., -1, :], v[..., 0, :] = 16, 2, 3
+    lengths = torch.ones(B, dtype=torch.int32, device="cuda")
+    lengths[0] = Sk
+    q = torch.ones(B, 1, 17, D, device="cuda", dtype=BF16)
+    out = ts.cross_attention(q, k.expand(B, 1, Sk, D), v.expand(B, 1, Sk, D), lengths, scale=1.0)
+    assert _lib.device_error() == 0
+    assert (out[0] == 2).all() and (out[1:] == 3).all()  # exp(-128) 2^28 is nothing

@@ -63,6 +63,10 @@ constexpr int kFwItemCost = 2;
 // keys, 0.25% after 2^19, 1% after 2^21 (values of mean 1), and terms below 2^-25 of the sum vanish. The row's sum is
 // added to term by term, where terms below 2^-24 of it vanish.
 constexpr int kFwFlushTiles = 1024;
+// The list's writer, and the softmax warps of a half without rows, wait until the others are through with a segment. A
+// tile takes 1 to 3 us, so an item of 50 million keys takes the second that bounds the waits for a pipeline stage: these
+// two waits are bounded by 20 us a tile more.
+constexpr uint64_t kFwTileNs = 20000;
 constexpr int kFwLeast = 8;  // see fw_plan; 4, 8, 16: 60.1, 62.1, 74.7 us (64 sequences, prefix 8192, own keys to 1024)
 
 template <int HD>
@@ -131,7 +135,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
   // The i-th segment of the list (false: the list was given up). One reader of each consumer then arrives on
   // seg_empty.
   auto read_seg = [&](int i, FwSeg& g) {
-    if (!mbar_wait(&B.seg_full[i % kFwSegs], (i / kFwSegs) & 1)) return false;
+    if (!mbar_wait(&B.seg_full[i % kFwSegs], (i / kFwSegs) & 1, A.seg_ns)) return false;
     g = B.seg[i % kFwSegs];
     return true;
   };
@@ -148,7 +152,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
         for (int i = 0;; ++i) {
           const bool whole = cur.w < A.whole, more = cur.next(g);
           if (!more) g.side = -1;
-          if (i >= kFwSegs && !mbar_wait(&B.seg_empty[i % kFwSegs], (i / kFwSegs - 1) & 1)) {
+          if (i >= kFwSegs && !mbar_wait(&B.seg_empty[i % kFwSegs], (i / kFwSegs - 1) & 1, A.seg_ns)) {
             atomicExch(&B.abort_flag, 1);
             break;
           }
@@ -919,6 +923,9 @@ int xattn_tc_forward(const trnsparse_attention_args* a, bool prefix, void* ws, c
     } else {
       A.item_cost = kFwItemCost;
       A.flush = reinterpret_cast<float*>(w + l.flush);
+      A.seg_ns = kWaitNs;
+      for (int j = 0; j < l.sides; ++j)
+        A.seg_ns += kFwTileNs * static_cast<uint64_t>((A.side[j].s.klen >> kFwKeyShift) + 1);
       XMap m[4];
       for (int j = 0; j < l.sides && !rc; ++j) {
         FwSide& S = A.side[j];

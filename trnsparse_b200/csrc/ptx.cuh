@@ -111,13 +111,14 @@ __device__ __forceinline__ bool wait_flag_geq(const long long* f, long long seq,
   return false;
 }
 
-// Bounded wait for the phase with the given parity to complete.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
+// Bounded wait for the phase with the given parity to complete: `ns` is the limit where more than a pipeline stage is
+// waited for.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint64_t ns = kWaitNs) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = global_ns();
   for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63u) == 0 && global_ns() - t0 > kWaitNs) break;
+    if ((i & 63u) == 0 && global_ns() - t0 > ns) break;
   }
   record_device_error(DEVERR_MBAR_TIMEOUT);
   return false;

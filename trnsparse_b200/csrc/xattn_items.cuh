@@ -48,6 +48,7 @@ struct FwArgs {
   int sides, D, whole;  // whole: items per CTA taken whole (one side only)
   int item_cost;        // see fw_cost
   int keep;             // the call has two sides: finished items go to their slots
+  uint64_t seg_ns;      // limit of the waits that last as long as a segment of another role
   float* flush;         // per CTA of the 256-row form, [HD / 4][256][4]: see kFwFlushTiles
   __nv_bfloat16* out;
   float* lse;
