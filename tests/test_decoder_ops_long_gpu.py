@@ -79,3 +79,48 @@ def test_an_item_that_takes_more_than_a_second():
     out = ts.cross_attention(q, k.expand(B, 1, Sk, D), v.expand(B, 1, Sk, D), lengths, scale=1.0)
     assert _lib.device_error() == 0
     assert (out[0] == 2).all() and (out[1:] == 3).all()  # exp(-128) 2^28 is nothing
+
+
+def _bias(got, ref):
+    """Mean error along the reference, and what the cuts of 2^17 products and the mean of the roundings allow."""
+    got, ref = got.double().flatten(), ref.flatten()
+    return abs(((got - ref) * ref.sign()).mean().item()) / ref.abs().mean().item(), 2.0 ** -8 * (1 + 4 / ref.numel() ** 0.5)
+
+
+def test_long_sums_of_dq_do_not_shrink():
+    """2^21 keys that are the values too: dq is the keys' covariance times dout, a sum that grows all along."""
+    g = torch.Generator(device="cuda").manual_seed(113)
+    B, Sq, n, D = 148, 17, 1 << 21, 64
+    q, dout = (torch.randn(1, 1, Sq, D, generator=g, device="cuda").to(BF16) for _ in range(2))
+    k = torch.randn(1, 1, n, D, generator=g, device="cuda").to(BF16)
+    leaf = q.expand(B, 1, Sq, D).contiguous().requires_grad_(True)
+    out = ts.cross_attention(leaf, k.expand(B, 1, n, D), k.expand(B, 1, n, D))
+    dq, = torch.autograd.grad(out, leaf, dout.expand(B, 1, Sq, D))
+    kd, do = k[0, 0].double(), dout[0, 0].double()
+    p = torch.softmax(q[0, 0].double() @ kd.T * D ** -0.5, -1)
+    delta = (do * out[0, 0].detach().double()).sum(-1, keepdim=True)
+    ref = (p * (do @ kd.T - delta)) @ kd * D ** -0.5
+    for i in (0, 1, B - 1):
+        got, most = _bias(dq[i, 0], ref)
+        assert got <= most
+
+
+def test_long_sums_of_dk_and_dv_do_not_shrink():
+    """2^21 query rows: dv is a sum of positive terms, dk of the queries' covariance."""
+    g = torch.Generator(device="cuda").manual_seed(114)
+    B, Sq, n, D = 75, 1 << 21, 100, 8
+    q = torch.randn(1, 1, Sq, D, generator=g, device="cuda").to(BF16)
+    k = 0.2 * torch.randn(1, 1, n, D, generator=g, device="cuda")
+    k = k.to(BF16).expand(B, 1, n, D).contiguous().requires_grad_(True)
+    v = torch.randn(1, 1, n, D, generator=g, device="cuda").to(BF16).expand(B, 1, n, D).contiguous().requires_grad_(True)
+    dout = (q + 1).to(BF16)
+    out = ts.cross_attention(q.expand(B, 1, Sq, D), k, v)
+    dk, dv = torch.autograd.grad(out, (k, v), dout.expand(B, 1, Sq, D))
+    qd, do, kd, vd = (t.detach()[0, 0].double() for t in (q, dout, k, v))
+    p = torch.softmax(qd @ kd.T * D ** -0.5, -1)
+    delta = (do * out[0, 0].detach().double()).sum(-1, keepdim=True)
+    refs = (p * (do @ vd.T - delta)).T @ qd * D ** -0.5, p.T @ do
+    for i in (0, B - 1):
+        for grad, ref in zip((dk, dv), refs):
+            got, most = _bias(grad[i, 0], ref)
+            assert got <= most

@@ -699,6 +699,10 @@ __global__ void __launch_bounds__(256) xattn_sum_bf16_kernel(const float* __rest
       make_uint4(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]), pack_bf16(s[4], s[5]), pack_bf16(s[6], s[7]));
 }
 
+// Steps of an accumulator: the tensor core cuts what it adds to the accumulator's last place, and longer chains of one
+// sign shrink visibly (kFwFlushTiles in cross_attention_tc.cu has the figures).
+constexpr int64_t kBwMostSteps = 1024;
+
 struct BwPlan {
   int q_tiles, k_tiles, parts[2], chunk[2], units[2];  // [0] rows, [1] columns
   size_t delta, part, total;
@@ -715,9 +719,10 @@ BwPlan bw_plan(const trnsparse_attention_args* a) {
   const int64_t rows[2] = {a->batch * a->q_heads * a->q_len, 2 * a->batch * a->kv_heads * a->k_len};
   size_t part = 0;
   for (int i = 0; i < 2; ++i) {
-    // cut the walks where tiles are fewer than SMs; a part is at least four steps
+    // cut the walks where tiles are fewer than SMs; a part is at least four steps and at most kBwMostSteps
     int64_t parts = items[i] > 0 ? sms / items[i] : 1;
     if (parts > steps[i] / 4) parts = steps[i] / 4;
+    if (parts * kBwMostSteps < steps[i]) parts = (steps[i] + kBwMostSteps - 1) / kBwMostSteps;
     if (parts < 1) parts = 1;
     const int64_t chunk = steps[i] > 0 ? (steps[i] + parts - 1) / parts : 1;
     p.chunk[i] = static_cast<int>(chunk);
