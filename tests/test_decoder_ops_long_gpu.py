@@ -14,12 +14,12 @@ pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
 
 
-def _ones(B, Sq, Sk, D, lengths=None):
+def _ones(B, Sq, Sk, D, dtype=BF16):
     """Queries, keys and values of ones, the keys of all sequences the same memory. The result is 1: the scores are
     equal, P is 1, and sums of ones are exact in fp32 up to 2^24."""
-    q = torch.ones(B, 1, Sq, D, device="cuda", dtype=BF16)
-    k = torch.ones(1, 1, Sk, D, device="cuda", dtype=BF16).expand(B, 1, Sk, D)
-    out = ts.cross_attention(q, k, k, lengths)
+    q = torch.ones(B, 1, Sq, D, device="cuda", dtype=dtype)
+    k = torch.ones(1, 1, Sk, D, device="cuda", dtype=dtype).expand(B, 1, Sk, D)
+    out = ts.cross_attention(q, k, k)
     check(out, torch.ones_like(out, dtype=torch.float64), torch.full_like(out, 2.0 ** -8, dtype=torch.float64), "out")
     assert _lib.device_error() == 0
 
@@ -124,3 +124,8 @@ def test_long_sums_of_dk_and_dv_do_not_shrink():
         for grad, ref in zip((dk, dv), refs):
             got, most = _bias(grad[i, 0], ref)
             assert got <= most
+
+
+def test_fp32_sums_pass_2_to_the_24():
+    """More items of one token than the GPU holds CTAs, so that no range of keys is cut to fill it."""
+    _ones(450, 1, 1 << 25, 1, torch.float32)

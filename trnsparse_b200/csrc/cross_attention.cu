@@ -29,6 +29,8 @@ namespace {
 
 constexpr int kXKeys = 64;    // keys a tile: 16-row form
 constexpr int kMmaKeys = 32;  // and 128-row form
+// Keys of a range at most: terms are added to a range's sums in fp32, where equal ones are lost from 2^24 on.
+constexpr int64_t kMostKeys = 1 << 20;
 
 __device__ __forceinline__ float xcvt(float v) { return v; }
 __device__ __forceinline__ float xcvt(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -495,6 +497,7 @@ GeneralPlan general_plan(const trnsparse_attention_args* a, const XSide (&s)[2],
     } else {
       per = walk_steps(ctas, tiles, sm_count(), resident, 128, 0.1);
     }
+    if (per > kMostKeys / keys) per = kMostKeys / keys;
     p.chunk[i] = static_cast<int>(per * keys);
     p.splits[i] = static_cast<int>(tiles > 0 ? (tiles + per - 1) / per : 1);
     p.pieces += p.splits[i];
