@@ -129,3 +129,28 @@ def test_long_sums_of_dk_and_dv_do_not_shrink():
 def test_fp32_sums_pass_2_to_the_24():
     """More items of one token than the GPU holds CTAs, so that no range of keys is cut to fill it."""
     _ones(450, 1, 1 << 25, 1, torch.float32)
+
+
+@pytest.mark.parametrize("B,H,Hkv,prefix", [
+    (300, 16, 1, False),
+    (300, 16, 1, True),  # 4800 rows of the prefix
+    (16, 20, 20, True),  # 16 rows of the prefix, one of each sequence
+])
+def test_long_sums_of_few_rows_do_not_shrink(B, H, Hkv, prefix):
+    """One token over 2^23 keys, in so many items that every CTA has a whole one; with a short prefix before them, too."""
+    g = torch.Generator(device="cuda").manual_seed(115)
+    n, D = 1 << 23, 64
+    q, k = (torch.randn(1, h, s, D, generator=g, device="cuda").to(BF16) for h, s in ((H, 1), (1, n)))
+    v = torch.empty(1, 1, n, D, device="cuda", dtype=BF16).normal_(1.0, 1.0, generator=g)
+    kd, vd = k[0, 0].double(), v[0, 0].double()
+    q, ck, cv = q.expand(B, H, 1, D), k.expand(B, Hkv, n, D), v.expand(B, Hkv, n, D)
+    if prefix:
+        out = ts.shared_prefix_attention(q, ck[0, :, :7], cv[0, :, :7], ck, cv, torch.full((B,), n, device="cuda"))
+        kd, vd = torch.cat((kd[:7], kd)), torch.cat((vd[:7], vd))
+    else:
+        out = ts.cross_attention(q, ck, cv)
+    ref = torch.cat([torch.softmax(r @ kd.T * D ** -0.5, -1) @ vd for r in q[0, :, 0].double().split(4)])
+    for i in (0, 1, B - 1):
+        got, most = _bias(out[i, :, 0], ref)
+        assert got <= most
+    assert _lib.device_error() == 0

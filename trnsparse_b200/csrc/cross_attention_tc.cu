@@ -67,6 +67,9 @@ constexpr int kFwFlushTiles = 1024;
 // tile takes 1 to 3 us, so an item of 50 million keys takes the second that bounds the waits for a pipeline stage: these
 // two waits are bounded by 20 us a tile more.
 constexpr uint64_t kFwTileNs = 20000;
+// Key tiles that a CTA of the few-rows form walks at most: 2^21 keys, of which a warp's accumulators add 2^19 (0.25%
+// low). It has no flushing (its registers are full); the calls beyond, milliseconds long, take the 256-row form.
+constexpr int64_t kFewMostTiles = 1 << (21 - kFewKeyShift);
 constexpr int kFwLeast = 8;  // see fw_plan; 4, 8, 16: 60.1, 62.1, 74.7 us (64 sequences, prefix 8192, own keys to 1024)
 
 template <int HD>
@@ -785,7 +788,11 @@ struct FwPlan {
 FwPlan fw_plan(const trnsparse_attention_args* a, const XSide (&s)[2], int n) {
   FwPlan p = {};
   bool few[2] = {false, false};
-  for (int i = 0; i < n; ++i) few[i] = side_rows(s[i]) <= kFewRows;
+  for (int i = 0; i < n; ++i) {
+    const int64_t item = (s[i].klen + (1ll << kFewKeyShift) - 1) >> kFewKeyShift;
+    const int64_t run = item * s[i].nb * s[i].hkv / few_rows_grid();  // where it is below an item, no CTA has a whole one
+    few[i] = side_rows(s[i]) <= kFewRows && (item < run ? item : run) <= kFewMostTiles;
+  }
   p.launches = n > 1 && few[0] != few[1] ? 2 : 1;
   size_t at = 0;
   const size_t D = static_cast<size_t>(a->head_dim);
