@@ -612,8 +612,9 @@ TRNSPARSE_API int trnsparse_qk_norm_rope_backward(const trnsparse_qk_norm_rope_a
  * q_heads, q_len, head_dim); k, v, dk, dv (batch, kv_heads, k_len, head_dim);
  * unit stride along head_dim, the other strides (batch, head, token) in
  * elements. q_heads is a multiple of kv_heads: query head i reads key head
- * i / (q_heads / kv_heads). F32 or BF16; softmax and sums in fp32. scale is any
- * number that is finite in fp32 (0 and negative ones too).
+ * i / (q_heads / kv_heads). F32 or BF16; softmax and sums in fp32; BF16 rounds the
+ * probabilities (backward: and the scores' gradients) to bf16 before their products.
+ * scale is any number that is finite in fp32 (0 and negative ones too).
  *   key_lengths: [batch] kept keys of each sequence (clamped to [0, k_len]), or
  *                NULL (all).
  *   key_mask:    [batch] rows of k_len bytes, 0 = hidden, row stride

@@ -15,12 +15,15 @@
 // repeatable results and no traffic for dQ. Where tiles are fewer than SMs the
 // walks are cut into parts whose fp32 sums a last kernel adds in order.
 //
-// What bounds it: the tensor cores' tf32 rate (3xTF32, xattn_tf32.cuh), kept about 60%
-// busy with two warps a scheduler; the rest goes to splitting operands and to waits
+// What bounds it: the tensor cores' tf32 rate (3xTF32, xattn_tf32.cuh), with the tensor
+// pipe 51% busy on two warps a scheduler; the rest goes to splitting operands and to waits
 // inside a warp's chain of scores, P and sums. 2 x 16/16 heads, 1024 x 1024 x 64: 644 us,
 // 47 TFLOP/s of the seven products (on the CUDA cores 1171 us); 16/4 heads at head_dim
 // 128 1278 us (2440); 2 x 8/2 heads, 333 x 517 x 64, where a CTA an SM is all there is,
-// 96 us (108 with four warps a CTA, two CTAs an SM; that took 584 at the first size).
+// 96 us (108 with four warps a CTA, two CTAs an SM; that took 584 at the first size: the
+// eight-warp form is faster for small calls only, and taken for all). 255 registers; at
+// head_dim up to 64 350 bytes a thread are spilled and 510 read back, above 128 350 and 480
+// (fp32), in between none.
 #include "xattn_tf32.cuh"
 
 namespace tsb {
@@ -86,7 +89,7 @@ __global__ void __launch_bounds__(256) xattn_delta_kernel(const T* __restrict__ 
   if (lane == 0) delta[row] = s;
 }
 
-// Eight warps, since one warp a scheduler keeps the tensor pipe 40% busy and two 64%. Up to head_dim 64 a warp has 32
+// Eight warps, two a scheduler, so that one's products cover the other's exponentials. Up to head_dim 64 a warp has 32
 // fixed rows, so that each split of a walked element feeds two products, and half of the walked ones (the halves' sums
 // are joined at the end); up to 128 16 rows, as 32 rows' sums would not fit in registers; both with the next walked rows
 // copied behind the arithmetic. Above that, 64 rows (shared memory), which warps share in pairs: for dQ each has half

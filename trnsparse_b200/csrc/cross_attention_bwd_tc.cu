@@ -3,7 +3,8 @@
 //   P = 2^(s2 - lse), dP = dO V^T, dS = P (dP - D), D = rowsum(dO o O),
 //   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO   (dK, dV over the group's heads).
 // P and dS are formed in fp32 and rounded to bf16 once, as operands of their
-// products (half a step each, of the size of the results' own rounding).
+// products (half a step each, of the size of the results' own rounding: errors of
+// 2.4e-3 of the gradients' size where that rounding alone makes 1.7e-3).
 //
 // Two launches of one kernel, each owning what it writes (fixed order, no
 // atomics, seven products for the mathematics' five):

@@ -6,8 +6,8 @@
 // 1024 multiply-adds). A 128-row tcgen05 tile would be padding and one chain S -> softmax -> P V per 128 keys; here
 // the rows are the 16 of an m16n8k16 product and every warp has keys of its own, so four chains run in a CTA and
 // eight on an SM, and nothing but the loads is waited for:
-//   warp 4       the list of (item, keys), and TMA: tiles of 64 keys, K and V together, through a ring (64 to 96 KB
-//                in flight a CTA, two CTAs an SM)
+//   warp 4       the list of (item, keys), and TMA: tiles of 64 keys, K and V together, through a ring (80 KB in
+//                flight a CTA at head_dim 64, 64 KB at 128; two CTAs an SM)
 //   warps 0-3    16 keys each of a tile: S by ldmatrix and mma, softmax in registers with the warp's own running
 //                maximum and sum, P V with P as it lies in registers; the four partial results of an item are
 //                joined through shared memory.

@@ -5,8 +5,9 @@
 //   O = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m),  s = scale log2(e) q.k
 // in one pass over the key tiles with the running maximum m and sum l of every
 // row. P = 2^(s - m) is rounded to bf16 for its product with V (half a step, at
-// most 2^-8 relative, of the same size as the result's own rounding); l sums the
-// unrounded values in fp32. m moves only when a tile's maximum passes it by more
+// most 2^-8 relative, of the same size as the result's own rounding: the result's
+// error grows from 1.7e-3 to 2.3e-3 of its size; unrounded P would take a second
+// product for its low part); l sums the unrounded values in fp32. m moves only when a tile's maximum passes it by more
 // than 2^8, so the accumulator in TMEM is rarely rescaled and P <= 2^8.
 //
 // An item is 256 packed rows (see xattn.cuh: query heads of one key head,
@@ -70,7 +71,9 @@ constexpr uint64_t kFwTileNs = 20000;
 // Key tiles that a CTA of the few-rows form walks at most: 2^21 keys, of which a warp's accumulators add 2^19 (0.25%
 // low). It has no flushing (its registers are full); the calls beyond, milliseconds long, take the 256-row form.
 constexpr int64_t kFewMostTiles = 1 << (21 - kFewKeyShift);
-constexpr int kFwLeast = 8;  // see fw_plan; 4, 8, 16: 60.1, 62.1, 74.7 us (64 sequences, prefix 8192, own keys to 1024)
+// Tiles of a CTA at least, see fw_plan. 4, 8, 16: 43.6, 50.2, 63.8 us for 64 sequences over a prefix of 2048 and own keys
+// up to 512; 65.2, 65.7, 79.2 over 8192 and 1024; 89.4, 81.7, 92.7 for 96 sequences there; the same over 32768 and 2048.
+constexpr int kFwLeast = 8;
 
 template <int HD>
 struct FwLayout {

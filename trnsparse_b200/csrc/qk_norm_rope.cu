@@ -11,7 +11,8 @@
 // What bounds it: memory; x is read and y written once (backward: x, dy read,
 // dx written). The one costly scalar part is the angle: p f_j in 64 bits (a
 // 32-bit product is off by a radian near p = 10^7), taken modulo a full turn in
-// 64 bits and only then rounded, so far positions keep 2^-24 of a turn. It
+// 64 bits and only then rounded, by 2^-26 of a turn at most: an angle is off by up to
+// 9.4e-8 at any position, less than a step of fp32. It
 // depends on the token and the pair alone, so a group of lanes owns one token,
 // keeps its cosines and sines in registers and walks over the token's heads.
 // Lane l of a group holds unit l: VEC elements from each side of VEC pairs, so

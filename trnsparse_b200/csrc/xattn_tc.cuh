@@ -155,7 +155,8 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 
 // 2^x of two elements on the FMA pipe, x <= 120 or so: x = n + f with n the nearest integer (adding 1.5 2^23
 // leaves it in the low mantissa bits), 2^f on [-1/2, 1/2] by a degree-4 minimax polynomial (relative error
-// 2.6e-6, fitted by weighted least squares for this file; P is rounded to bf16 at 2^-9 afterwards), and n added
+// 2.6e-6, fitted by weighted least squares for this file; P is rounded to bf16, half a step up to 2^-8, afterwards, the
+// row's sum takes it as it is), and n added
 // to the exponent. x below -126 gives 0, NaN gives NaN.
 __device__ __forceinline__ void exp2_poly2(uint64_t x2, float& a, float& b) {
   float xa, xb, la, lb;
@@ -222,7 +223,7 @@ int allow_smem(K kern, int bytes, unsigned long long* done, const char* what) {
 }
 
 // Strides (batch, head, token) the tensor maps and 16-byte accesses take: multiples of 8 elements, not
-// negative, below 2^39 elements; a dimension of one entry has no stride to look at.
+// negative, below 2^38 elements; a dimension of one entry has no stride to look at.
 inline bool strides_ok(const int64_t* s, int64_t nb, int64_t nh, int64_t nt, bool keys) {
   const int64_t n[3] = {nb, nh, nt};
   for (int i = 0; i < 3; ++i) {
