@@ -606,7 +606,7 @@ xattn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           uint32_t v[32];
           if (worked) {
             tmem_ld32(tmem + (a ? Lay::kTmemAcc1 : Lay::kTmemAcc0) + lane_base + d0, v);
-            tmem_wait_ld();
+            tmem_wait_ld32(v);
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0u;

@@ -7,8 +7,9 @@
 // row. P = 2^(s - m) is rounded to bf16 for its product with V (half a step, at
 // most 2^-8 relative, of the same size as the result's own rounding: the result's
 // error grows from 1.7e-3 to 2.3e-3 of its size; unrounded P would take a second
-// product for its low part); l sums the unrounded values in fp32. m moves only when a tile's maximum passes it by more
-// than 2^8, so the accumulator in TMEM is rarely rescaled and P <= 2^8.
+// product for its low part); l sums the unrounded values in fp32. m moves only when
+// a tile's maximum passes it by more than 2^8, so the accumulator in TMEM is rarely
+// rescaled and P <= 2^8.
 //
 // An item is 256 packed rows (see xattn.cuh: query heads of one key head,
 // tokens, and for a shared prefix all sequences) against the keys of one (batch
@@ -341,7 +342,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
       for (int c = 0; c < HD; c += 4, at += kFwRows) {
         uint32_t o[4];
         tmem_ld4(t_o + c, o);
-        tmem_wait_ld();
+        tmem_wait_ld4(o);
         float4 a = first ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
         a = make_float4(fmaf(a.x, f, __uint_as_float(o[0])), fmaf(a.y, f, __uint_as_float(o[1])),
                         fmaf(a.z, f, __uint_as_float(o[2])), fmaf(a.w, f, __uint_as_float(o[3])));
@@ -535,7 +536,7 @@ xattn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tk0, const __grid_consta
             for (int c = 0; c < HD / 16; ++c) {
               uint32_t o[16];
               tmem_ld16(t_o + c * 16, o);
-              tmem_wait_ld();
+              tmem_wait_ld16(o);
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
               tmem_st16(t_o + c * 16, o);
